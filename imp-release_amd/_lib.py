@@ -20,6 +20,7 @@ LIB_PATH = os.environ.get('IMP_HIP_LIB') or os.path.join(_HERE, 'csrc', 'libimp_
 MODEL_IDS = {'GM': 0, 'DGNNS': 1, 'AdaGMN': 2}
 NORM_IDS = {'in': 0, 'bn': 1}
 ACT_IDS = {'relu': 0, 'gelu': 1, 'lrelu': 2}
+DTYPE_IDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}          # the operators with gradients (ops.py)
 
 # every symbol include/imp_hip.h declares (tests check that the library exports all of them)
 SYMBOLS = [
@@ -29,6 +30,8 @@ SYMBOLS = [
     'imp_compute_matches', 'imp_pool', 'imp_score_mass', 'imp_pool_select', 'imp_pool_select_pair', 'imp_masked_commit', 'imp_gather_rows', 'imp_match_pair', 'imp_set_counts', 'imp_match_tail', 'imp_match_tail_scores', 'imp_pool_pair', 'imp_loop_lockstep', 'imp_loop_lockstep_uncertainty', 'imp_op_linear', 'imp_op_layer_gemm', 'imp_op_fused_mlp',
     'imp_op_attention', 'imp_time_attention', 'imp_time_attention_clock', 'imp_time_sinkhorn', 'imp_resident_status', 'imp_resident_health', 'imp_set_resident_verify', 'imp_resident_repaired', 'imp_resident_postmortem', 'imp_ctx_option', 'imp_debug_hold_cus', 'imp_range_events', 'imp_set_range_recovery', 'imp_range_recovered', 'imp_range_take', 'imp_tag_wraps', 'imp_time_layer_gemm', 'imp_estimate_pose', 'imp_pose_stats',
     'imp_sp_create', 'imp_sp_destroy', 'imp_sp_set_weight', 'imp_sp_finalize', 'imp_sp_detect', 'imp_sp_describe', 'imp_sp_dense', 'imp_sp_op_conv',
+    'imp_attn_workspace', 'imp_attn_forward', 'imp_attn_backward', 'imp_group_norm_act_workspace', 'imp_group_norm_act_forward', 'imp_group_norm_act_backward',
+    'imp_log_probs_workspace', 'imp_log_probs_forward', 'imp_log_probs_backward',
 ]
 
 
@@ -82,6 +85,12 @@ class ImpLoopPairU(C.Structure):
     _fields_ = [('pts0', C.c_void_p), ('pts1', C.c_void_p), ('K0', C.c_void_p), ('K1', C.c_void_p), ('indices0', C.c_void_p), ('mscores0', C.c_void_p),
                 ('kept0', C.c_void_p), ('kept1', C.c_void_p), ('R', C.c_double * 9), ('t', C.c_double * 3), ('found', C.c_int32),
                 ('n_iterations', C.c_int32), ('n_kept0', C.c_int32), ('n_kept1', C.c_int32), ('n_indices', C.c_int32), ('reserved', C.c_int32)]
+
+
+class ImpAttnDesc(C.Structure):
+    """include/imp_hip.h imp_attn_desc"""
+    _fields_ = [(n, C.c_int32) for n in ('dtype', 'batch', 'nq', 'nk', 'heads', 'kv_heads', 'head_dim')] + [('scale', C.c_float)] + [
+        (n, C.c_int64 * 3) for n in ('q_stride', 'k_stride', 'v_stride')] + [(n, C.c_void_p) for n in ('key_mask', 'q_lens', 'k_lens')]
 
 
 class ImpConfig(C.Structure):
@@ -173,6 +182,16 @@ def lib():
     L.imp_sp_describe.argtypes = [P, I, P, P, P, P]
     L.imp_sp_dense.argtypes = [P, P, P, P, P]
     L.imp_sp_op_conv.argtypes = [P, I, P, I, I, I, P, I, I, P]
+    U, L64 = C.c_uint64, C.c_int64
+    L.imp_attn_workspace.argtypes = [C.POINTER(ImpAttnDesc), I, C.POINTER(U)]
+    L.imp_attn_forward.argtypes = [C.POINTER(ImpAttnDesc), P, P, P, P, P, P, U, I, P]
+    L.imp_attn_backward.argtypes = [C.POINTER(ImpAttnDesc), P, P, P, P, P, P, P, P, P, P, U, I, P]
+    L.imp_group_norm_act_workspace.argtypes = [I, I, I, I, I, I, C.POINTER(U)]
+    L.imp_group_norm_act_forward.argtypes = [I, I, I, I, I, P, P, P, P, F, I, P, P, P, U, I, P]
+    L.imp_group_norm_act_backward.argtypes = [I, I, I, I, I, P, P, P, P, I, P, P, P, P, P, P, U, I, P]
+    L.imp_log_probs_workspace.argtypes = [L64, I, I, I, C.POINTER(U)]
+    L.imp_log_probs_forward.argtypes = [I, L64, I, L64, P, P, P, I, P, P, P, P, P, P, U, I, P]
+    L.imp_log_probs_backward.argtypes = [I, L64, I, L64, P, P, P, P, P, P, P, P, P, P, U, I, P]
     _lib = L
     return L
 

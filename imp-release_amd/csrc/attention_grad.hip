@@ -1,0 +1,823 @@
+// Multi-head attention with gradients (C-ABI imp_attn_forward / imp_attn_backward; gfx950): fp32 / fp16 / bf16, shared key heads, strided q | k | v,
+// key masks and per-pair lengths.  It stands beside the inference kernels (attention_f16x3.hip, attention_f32.hip: fp32, 4 heads, no gradient).
+//
+//   S = scale q.k   P = softmax of S over the kept keys   O = P V   lse = log sum exp S               (a row without a kept key: O = 0, lse = -inf)
+//   backward, with P recomputed from S and lse:  D = rowsum(dO O)   dV = P^T dO   dS = P (dO V^T - D)   dQ = scale dS K   dK = scale dS^T Q
+//
+// Three kernels of one shape.  A workgroup (4 waves) OWNS 128 rows of one side - a wave 32 of them, one per lane column of the 32x32x16 MFMA, held as
+// B-operand fragments in registers - and walks over tiles of the other side in LDS:
+//   forward  owns queries, walks keys:   S^T = K Q^T,                     O^T  += V^T P^T
+//   dQ       owns queries, walks keys:   S^T = K Q^T, dP^T = V dO^T,      dQ^T += K^T dS^T
+//   dK / dV  owns keys, walks queries:   S = Q K^T, dP = dO V^T,          dV^T += dO^T P, dK^T += Q^T dS
+// The owned row is always the lane, so softmax statistics, masks and output rows are per-lane values; the first product leaves P / dS in the
+// registers in exactly the order the second one takes its B operand (row 16 s + 8 (e / 4) + 4 half + e % 4 <-> register 8 s + e), and its A operand comes from
+// the SAME row-major LDS tile through the transpose read.  dQ recomputes S and dP (7 products backward instead of 5) so that no gradient is accumulated with
+// atomics: every sum has a fixed order and results repeat bit for bit.  Shared key heads: the G query heads of a key head are interleaved as rows
+// r = q G + g of one problem, so dK / dV sum over them in registers and one query of many heads still fills a tile.
+// Few rows: the walk is cut in shares (partials in the caller's workspace, joined in a fixed order by a second launch).
+//
+// Arithmetic: bf16 inputs one bf16 MFMA per product, P and dS rounded to bf16 (half a step of 2^-8, the inputs' own precision); fp16 forward one f16 MFMA; fp16
+// backward two bf16 planes per operand (hi + lo: all 11 bits, and dS far below the fp16 range keeps them) and three products; fp32 three bf16 planes
+// (24 bits, the full fp32 exponent range: no operand limit) and six products - what is dropped is below 2^-26.  Accumulators, softmax statistics and D fp32.
+#include "../../include/imp_hip.h"
+#include "imp_kernels.h"
+
+int imp_fail(int code, const char* msg);   // context.hip: sets imp_last_error()
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int OWN = 128;                 // owned rows per workgroup
+
+struct AttnOp {
+    const void *q, *k, *v, *out, *dout;  // out: read by the backward
+    void *o, *dq, *dk, *dv;
+    float *lse, *delta, *part, *part_lse;
+    const uint8_t* mask;
+    const int32_t *q_lens, *k_lens;
+    int64_t qs[3], ks[3], vs[3];         // batch, token, head strides in elements
+    int B, nq, nk, H, Hkv, G, dh;
+    float scale;
+    int shares;
+};
+
+template <typename E> struct Vec8;
+template <> struct Vec8<__bf16> { using type = bf16x8; };
+template <> struct Vec8<_Float16> { using type = f16x8; };
+
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// c += a b over the planes, the small products first
+template <int NP, typename V>
+__device__ __forceinline__ f32x16 mfma_planes(const V (&a)[NP], const V (&b)[NP], f32x16 c) {
+    if constexpr (NP == 3) {
+        c = mfma(a[1], b[1], c);
+        c = mfma(a[0], b[2], c);
+        c = mfma(a[2], b[0], c);
+    }
+    if constexpr (NP >= 2) {
+        c = mfma(a[0], b[1], c);
+        c = mfma(a[1], b[0], c);
+    }
+    return mfma(a[0], b[0], c);
+}
+
+// the same with the small products in an accumulator of their own (added once at the end): a sum over the channels is then rounded once per k-step at its
+// full size, not once per product - what dS = P (dP - D) keeps after the cancellation is decided here
+template <int NP, typename V>
+__device__ __forceinline__ void mfma_apart(const V (&a)[NP], const V (&b)[NP], f32x16& c, f32x16& small) {
+    if constexpr (NP == 3) {
+        small = mfma(a[1], b[1], small);
+        small = mfma(a[0], b[2], small);
+        small = mfma(a[2], b[0], small);
+    }
+    if constexpr (NP >= 2) {
+        small = mfma(a[0], b[1], small);
+        small = mfma(a[1], b[0], small);
+    }
+    c = mfma(a[0], b[0], c);
+}
+
+template <int NP, typename E>
+__device__ __forceinline__ void split8(const float (&x)[8], typename Vec8<E>::type (&p)[NP]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float r = x[i];
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            const E h = (E)r;
+            p[j][i] = h;
+            r -= (float)h;
+        }
+    }
+}
+
+// eight consecutive elements as they lie in memory
+template <typename T> struct Chunk;
+template <> struct Chunk<float> {
+    f32x4 a, b;
+    __device__ void load(const float* p) { a = *(const f32x4*)p; b = *(const f32x4*)(p + 4); }
+    __device__ void zero() { a = f32x4{0, 0, 0, 0}; b = a; }
+    __device__ void get(float (&x)[8]) const { for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[i + 4] = b[i]; } }
+};
+template <typename T> struct Chunk16 {
+    u32x4 a;
+    __device__ void load(const T* p) { a = *(const u32x4*)p; }
+    __device__ void zero() { a = u32x4{0, 0, 0, 0}; }
+    __device__ void get(float (&x)[8]) const {
+        const auto v = __builtin_bit_cast(typename Vec8<T>::type, a);
+        for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
+    }
+};
+template <> struct Chunk<__bf16> : Chunk16<__bf16> {};
+template <> struct Chunk<_Float16> : Chunk16<_Float16> {};
+
+template <typename T, int NP, typename E>
+__device__ __forceinline__ void to_planes(const Chunk<T>& c, typename Vec8<E>::type (&p)[NP]) {
+    if constexpr (NP == 1 && sizeof(T) == 2) {
+        p[0] = __builtin_bit_cast(typename Vec8<E>::type, c.a);
+    } else {
+        float x[8];
+        c.get(x);
+        split8<NP, E>(x, p);
+    }
+}
+
+template <typename T> __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+    if constexpr (sizeof(T) == 4) {
+        *(f32x4*)p = f32x4{a, b, c, d};
+    } else {
+        typedef T v4 __attribute__((ext_vector_type(4)));
+        *(v4*)p = v4{(T)a, (T)b, (T)c, (T)d};
+    }
+}
+
+__device__ __forceinline__ int clamp_len(const int32_t* lens, int b, int n) { return lens ? min(max(lens[b], 0), n) : n; }
+
+// row r = q G + g of key head hk (query side)
+__device__ __forceinline__ int64_t q_row(const AttnOp& p, const int64_t (&st)[3], int b, int hk, int r) {
+    const int q = r / p.G, g = r - q * p.G;
+    return b * st[0] + q * st[1] + (int64_t)(hk * p.G + g) * st[2];
+}
+__device__ __forceinline__ int64_t dense_row(const AttnOp& p, int b, int hk, int r) {        // row index in [B][nq][H]
+    const int q = r / p.G, g = r - q * p.G;
+    return ((int64_t)b * p.nq + q) * p.H + hk * p.G + g;
+}
+__device__ __forceinline__ int64_t stat_row(const AttnOp& p, int b, int hk, int r) {         // index in [B][H][nq]
+    const int q = r / p.G, g = r - q * p.G;
+    return ((int64_t)b * p.H + hk * p.G + g) * p.nq + q;
+}
+
+template <typename E> using lds_tile_t = E*;
+
+// A operand of the first product: row = lane % 32 of the 32-row sub-tile, 8 columns of k-step s
+template <typename E, int NP, int LD, int PLANE>
+__device__ __forceinline__ void read_rows(const E* tile, int sub, int s, int lane, typename Vec8<E>::type (&f)[NP]) {
+    const E* a = tile + (sub * 32 + (lane & 31)) * LD + 16 * s + 8 * (lane >> 5);
+#pragma unroll
+    for (int j = 0; j < NP; ++j) f[j] = *(const typename Vec8<E>::type*)(a + j * PLANE);
+}
+// A operand of the second product: the tile transposed, channel = 32 dt + lane % 32, slot e of half h = row 16 s + 8 (e / 4) + 4 h + e % 4
+template <typename E, int NP, int LD, int PLANE>
+__device__ __forceinline__ void read_cols(const E* tile, int sub, int s, int dt, int lane, typename Vec8<E>::type (&f)[NP]) {
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const E* a = tile + (sub * 32 + 16 * s + 4 * (lane >> 5) + ((lane & 15) >> 2)) * LD + 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + j * PLANE));
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + j * PLANE + 8 * LD));
+        f[j] = __builtin_bit_cast(typename Vec8<E>::type, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+}
+
+// the owned row of this lane as B-operand fragments (zeros when the row is dead or past the head's channels)
+template <typename T, typename E, int NP, int DHP>
+__device__ __forceinline__ void load_owned(const T* row, bool live, int dh, int half, typename Vec8<E>::type (&f)[DHP / 16][NP]) {
+#pragma unroll
+    for (int s = 0; s < DHP / 16; ++s) {
+        Chunk<T> c;
+        const int col = 16 * s + 8 * half;
+        if (live && col < dh) c.load(row + col);
+        else c.zero();
+        to_planes<T, NP, E>(c, f[s]);
+    }
+}
+
+// One tile of the walked side: 256 threads fetch R rows x DHP columns of two matrices into registers, and store them as planes
+template <typename T, typename E, int NP, int DHP, int R>
+struct Stage {
+    static constexpr int CPR = DHP / 8, N = (R * CPR + 255) / 256, LD = DHP + 8, PLANE = R * LD;
+    Chunk<T> x[N], y[N];
+    // addr(i, row, live) -> pointers of both matrices' rows
+    template <typename F> __device__ void fetch(int tid, int dh, F addr) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = tid + 256 * i, row = c / CPR, col = (c % CPR) * 8;
+            x[i].zero();
+            y[i].zero();
+            const T *px, *py;
+            if ((R * CPR % 256 == 0 || row < R) && col < dh && addr(row, px, py)) {
+                x[i].load(px + col);
+                y[i].load(py + col);
+            }
+        }
+    }
+    __device__ void store(int tid, E* X, E* Y) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = tid + 256 * i, row = c / CPR, col = (c % CPR) * 8;
+            if (R * CPR % 256 == 0 || row < R) {
+                typename Vec8<E>::type p[NP];
+                to_planes<T, NP, E>(x[i], p);
+#pragma unroll
+                for (int j = 0; j < NP; ++j) *(typename Vec8<E>::type*)(X + j * PLANE + row * LD + col) = p[j];
+                to_planes<T, NP, E>(y[i], p);
+#pragma unroll
+                for (int j = 0; j < NP; ++j) *(typename Vec8<E>::type*)(Y + j * PLANE + row * LD + col) = p[j];
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 0.f;
+    return z;
+}
+
+// registers 8 s .. 8 s + 7 of a first product's result as the planes of a B operand
+template <int NP, typename E>
+__device__ __forceinline__ void pack(const f32x16& v, int s, typename Vec8<E>::type (&p)[NP]) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = v[8 * s + e];
+    split8<NP, E>(x, p);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------- forward
+template <typename T, typename E, int NP, int DHP, int R>
+__global__ __launch_bounds__(256, 1) void attn_fwd_kernel(AttnOp p) {
+    using V = typename Vec8<E>::type;
+    using St = Stage<T, E, NP, DHP, R>;
+    constexpr int LD = St::LD, PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32;
+    __shared__ __attribute__((aligned(16))) E Ks[NP * PLANE], Vs[NP * PLANE];
+    __shared__ __attribute__((aligned(16))) float kb[R];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
+    const int b = blockIdx.y / p.Hkv, hk = blockIdx.y % p.Hkv, share = blockIdx.z;
+    const int nrows = p.nq * p.G, klen = clamp_len(p.k_lens, b, p.nk), live_rows = clamp_len(p.q_lens, b, p.nq) * p.G;
+    const int own0 = blockIdx.x * OWN, r = own0 + 32 * wave + (lane & 31);
+    const bool live = r < live_rows;
+    const int tiles = (klen + R - 1) / R;
+    int t0 = 0, t1 = own0 < live_rows ? tiles : 0;
+    if (p.shares > 1 && t1) { t0 = (int)((int64_t)tiles * share / p.shares); t1 = (int)((int64_t)tiles * (share + 1) / p.shares); }
+
+    V qf[KS][NP];
+    load_owned<T, E, NP, DHP>((const T*)p.q + (live ? q_row(p, p.qs, b, hk, r) : 0), live, p.dh, half, qf);
+    const T* kbase = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
+    const T* vbase = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
+    const uint8_t* mask = p.mask ? p.mask + (int64_t)b * p.nk : nullptr;
+    const float c = p.scale * LOG2E;
+
+    f32x16 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] = zero16();
+    float m = -INFINITY, l = 0.f;
+    St st;
+    auto fetch = [&](int t) {
+        st.fetch(tid, p.dh, [&](int row, const T*& px, const T*& py) {
+            const int key = t * R + row;
+            if (key >= klen || (mask && !mask[key])) return false;
+            px = kbase + key * p.ks[1];
+            py = vbase + key * p.vs[1];
+            return true;
+        });
+    };
+    if (t0 < t1) fetch(t0);
+    for (int t = t0; t < t1; ++t) {
+        __syncthreads();
+        st.store(tid, Ks, Vs);
+        if (tid < R) { const int key = t * R + tid; kb[tid] = key < klen && (!mask || mask[key]) ? 0.f : -INFINITY; }
+        __syncthreads();
+        if (t + 1 < t1) fetch(t + 1);
+        f32x16 s[NT];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            f32x16 s1 = zero16();
+            s[n] = zero16();
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                V f[NP];
+                read_rows<E, NP, LD, PLANE>(Ks, n, k, lane, f);
+                mfma_apart<NP, V>(f, qf[k], s[n], s1);
+            }
+            if constexpr (NP > 1) s[n] += s1;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 bias = *(const f32x4*)(kb + 32 * n + 8 * g + 4 * half);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[n][4 * g + i] = __builtin_fmaf(s[n][4 * g + i], c, bias[i]);
+                    mx = fmaxf(mx, s[n][4 * g + i]);
+                }
+            }
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - mu);
+        m = mn;
+        if (__ballot(alpha != 1.f)) {
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d] *= alpha;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[n][i] = __builtin_amdgcn_exp2f(s[n][i] - mu);
+                l += s[n][i];
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                V pf[NP];
+                pack<NP, E>(s[n], k, pf);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    V f[NP];
+                    read_cols<E, NP, LD, PLANE>(Vs, n, k, d, lane, f);
+                    o[d] = mfma_planes<NP, V>(f, pf, o[d]);
+                }
+            }
+        }
+    }
+    l += __shfl_xor(l, 32);
+    if (r >= nrows) return;
+    if (!live) {                         // past its count, beside live rows of the workgroup
+        l = 0.f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] = zero16();
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l, lse = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+    const int64_t row = dense_row(p, b, hk, r), rows = (int64_t)p.B * p.nq * p.H;
+    if (p.shares > 1) {
+        float* out = p.part + (share * rows + row) * p.dh;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int col = 32 * d + 8 * g + 4 * half;
+                if (col < p.dh) store4(out + col, o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv);
+            }
+        if (!half) p.part_lse[share * rows + row] = lse;
+    } else {
+        T* out = (T*)p.o + row * p.dh;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int col = 32 * d + 8 * g + 4 * half;
+                if (col < p.dh) store4(out + col, o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv);
+            }
+        if (!half && p.lse) p.lse[stat_row(p, b, hk, r)] = lse;
+    }
+}
+
+// joins the shares of a row: one wave per row, the shares' weights exp(lse_s - lse)
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnOp p) {
+    const int64_t rows = (int64_t)p.B * p.nq * p.H, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (row >= rows) return;
+    const float mine = lane < p.shares ? p.part_lse[lane * rows + row] : -INFINITY;
+    float m = mine;
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const float mu = m == -INFINITY ? 0.f : m;
+    float sum = __builtin_amdgcn_exp2f((mine - mu) * LOG2E);
+    const float w = sum;
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    for (int c0 = 0; c0 < p.dh; c0 += 64) {
+        float acc = 0.f;
+        const int c = c0 + lane;
+        for (int s = 0; s < p.shares; ++s) {
+            const float ws = __shfl(w, s);
+            if (c < p.dh && ws != 0.f) acc += ws * p.part[(s * rows + row) * p.dh + c];
+        }
+        if (c < p.dh) ((T*)p.o)[row * p.dh + c] = (T)(acc * inv);
+    }
+    if (lane == 0 && p.lse) {
+        const int h = (int)(row % p.H);
+        const int64_t bq = row / p.H;
+        p.lse[((bq / p.nq) * p.H + h) * p.nq + bq % p.nq] = sum == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(sum) * LN2;
+    }
+}
+
+// --------------------------------------------------------------------------------------------------------------------- backward
+// D = rowsum(dO O): 16 lanes per row of [B][nq][H][dh]
+template <typename T>
+__global__ __launch_bounds__(256) void attn_delta_kernel(AttnOp p) {
+    const int64_t rows = (int64_t)p.B * p.nq * p.H, row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (row >= rows) return;
+    const int col = (threadIdx.x & 15) * 8;
+    float sum = 0.f;
+    if (col < p.dh) {
+        Chunk<T> a, b;
+        a.load((const T*)p.out + row * p.dh + col);
+        b.load((const T*)p.dout + row * p.dh + col);
+        float x[8], y[8];
+        a.get(x);
+        b.get(y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(x[i], y[i], sum);
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    if ((threadIdx.x & 15) == 0) {
+        const int h = (int)(row % p.H);
+        const int64_t bq = row / p.H;
+        p.delta[((bq / p.nq) * p.H + h) * p.nq + bq % p.nq] = sum;
+    }
+}
+
+// the exponent reference of a row: lse in log2 units, +inf (P = 0) for rows that do not exist or have no key
+__device__ __forceinline__ float row_ref(float lse) { return lse == -INFINITY ? INFINITY : lse * LOG2E; }
+
+template <typename T, typename E, int NP, int DHP, int R>
+__global__ __launch_bounds__(256, 1) void attn_dq_kernel(AttnOp p) {
+    using V = typename Vec8<E>::type;
+    using St = Stage<T, E, NP, DHP, R>;
+    constexpr int LD = St::LD, PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32;
+    __shared__ __attribute__((aligned(16))) E Ks[NP * PLANE], Vs[NP * PLANE];
+    __shared__ __attribute__((aligned(16))) float kb[R];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
+    const int b = blockIdx.y / p.Hkv, hk = blockIdx.y % p.Hkv, share = blockIdx.z;
+    const int nrows = p.nq * p.G, klen = clamp_len(p.k_lens, b, p.nk), live_rows = clamp_len(p.q_lens, b, p.nq) * p.G;
+    const int own0 = blockIdx.x * OWN, r = own0 + 32 * wave + (lane & 31);
+    const int tiles = (klen + R - 1) / R;
+    int t0 = 0, t1 = own0 < live_rows ? tiles : 0;
+    if (p.shares > 1 && t1) { t0 = (int)((int64_t)tiles * share / p.shares); t1 = (int)((int64_t)tiles * (share + 1) / p.shares); }
+
+    float ref = INFINITY, delta = 0.f;
+    if (r < live_rows) {
+        const int64_t at = stat_row(p, b, hk, r);
+        ref = row_ref(p.lse[at]);
+        delta = p.delta[at];
+    }
+    const bool live = ref != INFINITY;
+    if (!live) delta = 0.f;
+    V qf[KS][NP], of[KS][NP];
+    load_owned<T, E, NP, DHP>((const T*)p.q + (live ? q_row(p, p.qs, b, hk, r) : 0), live, p.dh, half, qf);
+    load_owned<T, E, NP, DHP>((const T*)p.dout + (live ? dense_row(p, b, hk, r) * p.dh : 0), live, p.dh, half, of);
+    const T* kbase = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
+    const T* vbase = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
+    const uint8_t* mask = p.mask ? p.mask + (int64_t)b * p.nk : nullptr;
+    const float c = p.scale * LOG2E;
+    f32x16 dq[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) dq[d] = zero16();
+    St st;
+    auto fetch = [&](int t) {
+        st.fetch(tid, p.dh, [&](int row, const T*& px, const T*& py) {
+            const int key = t * R + row;
+            if (key >= klen || (mask && !mask[key])) return false;
+            px = kbase + key * p.ks[1];
+            py = vbase + key * p.vs[1];
+            return true;
+        });
+    };
+    if (t0 < t1) fetch(t0);
+    for (int t = t0; t < t1; ++t) {
+        __syncthreads();
+        st.store(tid, Ks, Vs);
+        if (tid < R) { const int key = t * R + tid; kb[tid] = key < klen && (!mask || mask[key]) ? 0.f : -INFINITY; }
+        __syncthreads();
+        if (t + 1 < t1) fetch(t + 1);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            f32x16 s = zero16(), dp = zero16(), s1 = zero16(), dp1 = zero16();
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                V f[NP];
+                read_rows<E, NP, LD, PLANE>(Ks, n, k, lane, f);
+                mfma_apart<NP, V>(f, qf[k], s, s1);
+                read_rows<E, NP, LD, PLANE>(Vs, n, k, lane, f);
+                mfma_apart<NP, V>(f, of[k], dp, dp1);
+            }
+            if constexpr (NP > 1) { s += s1; dp += dp1; }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 bias = *(const f32x4*)(kb + 32 * n + 8 * g + 4 * half);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], c, -ref) + bias[i]);
+                    s[4 * g + i] = pr * (dp[4 * g + i] - delta);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                V df[NP];
+                pack<NP, E>(s, k, df);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    V f[NP];
+                    read_cols<E, NP, LD, PLANE>(Ks, n, k, d, lane, f);
+                    dq[d] = mfma_planes<NP, V>(f, df, dq[d]);
+                }
+            }
+        }
+    }
+    if (r >= nrows) return;
+    const int64_t row = dense_row(p, b, hk, r), rows = (int64_t)p.B * p.nq * p.H;
+    if (!live) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d) dq[d] = zero16();
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int col = 32 * d + 8 * g + 4 * half;
+            if (col < p.dh) {
+                const float x0 = dq[d][4 * g] * p.scale, x1 = dq[d][4 * g + 1] * p.scale, x2 = dq[d][4 * g + 2] * p.scale, x3 = dq[d][4 * g + 3] * p.scale;
+                if (p.shares > 1) store4(p.part + (share * rows + row) * p.dh + col, x0, x1, x2, x3);
+                else store4((T*)p.dq + row * p.dh + col, x0, x1, x2, x3);
+            }
+        }
+}
+
+template <typename T, typename E, int NP, int DHP, int R>
+__global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnOp p) {
+    using V = typename Vec8<E>::type;
+    using St = Stage<T, E, NP, DHP, R>;
+    constexpr int LD = St::LD, PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32;
+    __shared__ __attribute__((aligned(16))) E Qs[NP * PLANE], Os[NP * PLANE];
+    __shared__ __attribute__((aligned(16))) float refs[R], deltas[R];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
+    const int b = blockIdx.y / p.Hkv, hk = blockIdx.y % p.Hkv, share = blockIdx.z;
+    const int klen = clamp_len(p.k_lens, b, p.nk), live_rows = clamp_len(p.q_lens, b, p.nq) * p.G;
+    const int own0 = blockIdx.x * OWN, key = own0 + 32 * wave + (lane & 31);
+    const bool live = key < klen && (!p.mask || p.mask[(int64_t)b * p.nk + key]);
+    const int tiles = (live_rows + R - 1) / R;
+    int t0 = 0, t1 = own0 < klen ? tiles : 0;
+    if (p.shares > 1 && t1) { t0 = (int)((int64_t)tiles * share / p.shares); t1 = (int)((int64_t)tiles * (share + 1) / p.shares); }
+
+    V kf[KS][NP], vf[KS][NP];
+    load_owned<T, E, NP, DHP>((const T*)p.k + (live ? b * p.ks[0] + key * p.ks[1] + hk * p.ks[2] : 0), live, p.dh, half, kf);
+    load_owned<T, E, NP, DHP>((const T*)p.v + (live ? b * p.vs[0] + key * p.vs[1] + hk * p.vs[2] : 0), live, p.dh, half, vf);
+    const float c = p.scale * LOG2E, off = live ? 0.f : -INFINITY;
+    f32x16 dk[DT], dv[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
+    St st;
+    auto row_live = [&](int r) { return r < live_rows && p.lse[stat_row(p, b, hk, r)] != -INFINITY; };
+    auto fetch = [&](int t) {
+        st.fetch(tid, p.dh, [&](int row, const T*& px, const T*& py) {
+            const int r = t * R + row;
+            if (!row_live(r)) return false;
+            px = (const T*)p.q + q_row(p, p.qs, b, hk, r);
+            py = (const T*)p.dout + dense_row(p, b, hk, r) * p.dh;
+            return true;
+        });
+    };
+    if (t0 < t1) fetch(t0);
+    for (int t = t0; t < t1; ++t) {
+        __syncthreads();
+        st.store(tid, Qs, Os);
+        if (tid < R) {
+            const int r = t * R + tid;
+            float ref = INFINITY, dl = 0.f;
+            if (r < live_rows) {
+                const int64_t at = stat_row(p, b, hk, r);
+                ref = row_ref(p.lse[at]);
+                if (ref != INFINITY) dl = p.delta[at];
+            }
+            refs[tid] = ref;
+            deltas[tid] = dl;
+        }
+        __syncthreads();
+        if (t + 1 < t1) fetch(t + 1);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            f32x16 s = zero16(), dp = zero16(), s1 = zero16(), dp1 = zero16();
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                V f[NP];
+                read_rows<E, NP, LD, PLANE>(Qs, n, k, lane, f);
+                mfma_apart<NP, V>(f, kf[k], s, s1);
+                read_rows<E, NP, LD, PLANE>(Os, n, k, lane, f);
+                mfma_apart<NP, V>(f, vf[k], dp, dp1);
+            }
+            if constexpr (NP > 1) { s += s1; dp += dp1; }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 ref = *(const f32x4*)(refs + 32 * n + 8 * g + 4 * half);
+                const f32x4 dl = *(const f32x4*)(deltas + 32 * n + 8 * g + 4 * half);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], c, -ref[i]) + off);
+                    s[4 * g + i] = pr;
+                    dp[4 * g + i] = pr * (dp[4 * g + i] - dl[i]);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                V pf[NP], df[NP];
+                pack<NP, E>(s, k, pf);
+                pack<NP, E>(dp, k, df);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    V f[NP];
+                    read_cols<E, NP, LD, PLANE>(Os, n, k, d, lane, f);
+                    dv[d] = mfma_planes<NP, V>(f, pf, dv[d]);
+                    read_cols<E, NP, LD, PLANE>(Qs, n, k, d, lane, f);
+                    dk[d] = mfma_planes<NP, V>(f, df, dk[d]);
+                }
+            }
+        }
+    }
+    if (key >= p.nk) return;
+    const int64_t row = ((int64_t)b * p.nk + key) * p.Hkv + hk, rows = (int64_t)p.B * p.nk * p.Hkv;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int col = 32 * d + 8 * g + 4 * half;
+            if (col < p.dh) {
+                const float x0 = dk[d][4 * g] * p.scale, x1 = dk[d][4 * g + 1] * p.scale, x2 = dk[d][4 * g + 2] * p.scale, x3 = dk[d][4 * g + 3] * p.scale;
+                const float y0 = dv[d][4 * g], y1 = dv[d][4 * g + 1], y2 = dv[d][4 * g + 2], y3 = dv[d][4 * g + 3];
+                if (p.shares > 1) {
+                    store4(p.part + (2 * share * rows + row) * p.dh + col, x0, x1, x2, x3);
+                    store4(p.part + ((2 * share + 1) * rows + row) * p.dh + col, y0, y1, y2, y3);
+                } else {
+                    store4((T*)p.dk + row * p.dh + col, x0, x1, x2, x3);
+                    store4((T*)p.dv + row * p.dh + col, y0, y1, y2, y3);
+                }
+            }
+        }
+}
+
+// out[i] = sum over the shares, in their order (4 elements per thread; n % 4 == 0)
+template <typename T>
+__global__ __launch_bounds__(256) void attn_sum_kernel(const float* part, int64_t n, int64_t stride, int shares, T* out) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    f32x4 a = *(const f32x4*)(part + i);
+    for (int s = 1; s < shares; ++s) a += *(const f32x4*)(part + s * stride + i);
+    store4(out + i, a[0], a[1], a[2], a[3]);
+}
+
+// ------------------------------------------------------------------------------------------------------------------------- host
+// shares of the walk: enough workgroups for two per CU, each with at least four tiles of the walk
+int shares_for(int64_t blocks, int64_t walked) {
+    const int64_t want = (512 + blocks - 1) / blocks, most = walked / 256;
+    const int64_t s = want < most ? want : most;
+    return s < 1 ? 1 : (s > 64 ? 64 : (int)s);
+}
+
+struct Plan { int fwd, dq, dkv; int64_t q_rows, k_rows; size_t fwd_bytes, bwd_bytes; };
+Plan plan(const imp_attn_desc& d) {
+    Plan p;
+    const int64_t heads = (int64_t)d.batch * d.kv_heads, rows = (int64_t)d.nq * (d.heads / d.kv_heads);
+    const int64_t qb = (rows + OWN - 1) / OWN * heads, kbk = ((int64_t)d.nk + OWN - 1) / OWN * heads;
+    p.fwd = shares_for(qb, d.nk);
+    p.dq = p.fwd;
+    p.dkv = shares_for(kbk, rows);
+    p.q_rows = (int64_t)d.batch * d.nq * d.heads;
+    p.k_rows = (int64_t)d.batch * d.nk * d.kv_heads;
+    p.fwd_bytes = p.fwd > 1 ? (size_t)p.fwd * p.q_rows * (d.head_dim + 1) * 4 : 0;
+    const size_t a = p.dq > 1 ? (size_t)p.dq * p.q_rows * d.head_dim * 4 : 0, b = p.dkv > 1 ? (size_t)p.dkv * 2 * p.k_rows * d.head_dim * 4 : 0;
+    p.bwd_bytes = ((size_t)p.q_rows * 4 + 15) / 16 * 16 + (a > b ? a : b);
+    return p;
+}
+
+const char* bad_desc(const imp_attn_desc* d) {
+    if (!d) return "null description";
+    if (d->dtype != IMP_DTYPE_F32 && d->dtype != IMP_DTYPE_F16 && d->dtype != IMP_DTYPE_BF16) return "unknown dtype";
+    if (d->batch < 1 || d->nq < 1 || d->nk < 1 || d->heads < 1 || d->kv_heads < 1) return "sizes must be at least 1";
+    if (d->heads % d->kv_heads) return "heads must be a multiple of kv_heads";
+    if (d->head_dim < 8 || d->head_dim > 128 || d->head_dim % 8) return "head_dim must be a multiple of 8 up to 128";
+    if ((int64_t)d->batch * d->kv_heads > 65535) return "batch x kv_heads must be at most 65535";
+    if ((int64_t)d->nq * (d->heads / d->kv_heads) > (1 << 30) || d->nk > (1 << 30)) return "too many rows";
+    if ((int64_t)d->batch * d->nq * d->heads > ((int64_t)1 << 33)) return "too many rows";
+    const int unit = d->dtype == IMP_DTYPE_F32 ? 4 : 8;
+    for (int i = 0; i < 3; ++i)
+        if (d->q_stride[i] % unit || d->k_stride[i] % unit || d->v_stride[i] % unit || d->q_stride[i] < 0 || d->k_stride[i] < 0 || d->v_stride[i] < 0)
+            return "strides must be multiples of 16 bytes";
+    return nullptr;
+}
+bool unaligned(std::initializer_list<const void*> ptrs) {
+    for (const void* p : ptrs) if ((uintptr_t)p & 15) return true;
+    return false;
+}
+
+AttnOp op_of(const imp_attn_desc& d) {
+    AttnOp p = {};
+    p.mask = d.key_mask; p.q_lens = d.q_lens; p.k_lens = d.k_lens;
+    for (int i = 0; i < 3; ++i) { p.qs[i] = d.q_stride[i]; p.ks[i] = d.k_stride[i]; p.vs[i] = d.v_stride[i]; }
+    p.B = d.batch; p.nq = d.nq; p.nk = d.nk; p.H = d.heads; p.Hkv = d.kv_heads; p.G = d.heads / d.kv_heads; p.dh = d.head_dim;
+    p.scale = d.scale;
+    return p;
+}
+
+// which: 0 forward, 1 dQ, 2 dK / dV
+template <typename T, typename E, int NP, int DHP, int R>
+void launch(int which, const AttnOp& p, hipStream_t st) {
+    const int64_t own = which == 2 ? p.nk : (int64_t)p.nq * p.G;
+    const dim3 grid((unsigned)((own + OWN - 1) / OWN), (unsigned)(p.B * p.Hkv), (unsigned)p.shares);
+    if (which == 0) attn_fwd_kernel<T, E, NP, DHP, R><<<grid, 256, 0, st>>>(p);
+    else if (which == 1) attn_dq_kernel<T, E, NP, DHP, R><<<grid, 256, 0, st>>>(p);
+    else attn_dkv_kernel<T, E, NP, DHP, R><<<grid, 256, 0, st>>>(p);
+}
+template <typename T, typename E, int NP, int R>
+void launch_dh(int which, const AttnOp& p, hipStream_t st) {
+    if (p.dh <= 32) launch<T, E, NP, 32, R>(which, p, st);
+    else if (p.dh <= 64) launch<T, E, NP, 64, R>(which, p, st);
+    else launch<T, E, NP, 128, R>(which, p, st);
+}
+void launch_any(int dtype, int which, const AttnOp& p, hipStream_t st) {
+    if (dtype == IMP_DTYPE_F32) launch_dh<float, __bf16, 3, 32>(which, p, st);
+    else if (dtype == IMP_DTYPE_BF16) launch_dh<__bf16, __bf16, 1, 64>(which, p, st);
+    else if (which == 0) launch_dh<_Float16, _Float16, 1, 64>(which, p, st);
+    else launch_dh<_Float16, __bf16, 2, 32>(which, p, st);
+}
+
+int on_device(int device) {
+    hipError_t e = hipSetDevice(device);
+    return e == hipSuccess ? 0 : imp_fail(IMP_E_HIP, hipGetErrorString(e));
+}
+int launched(const char* what) {
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess) return IMP_OK;
+    (void)what;
+    return imp_fail(IMP_E_HIP, hipGetErrorString(e));
+}
+
+}  // namespace
+
+extern "C" {
+
+int imp_attn_workspace(const imp_attn_desc* d, int backward, uint64_t* bytes) {
+    if (const char* why = bad_desc(d)) return imp_fail(IMP_E_ARG, why);
+    if (!bytes) return imp_fail(IMP_E_ARG, "imp_attn_workspace: null argument");
+    const Plan pl = plan(*d);
+    *bytes = backward ? pl.bwd_bytes : pl.fwd_bytes;
+    return IMP_OK;
+}
+
+int imp_attn_forward(const imp_attn_desc* d, const void* q, const void* k, const void* v, void* out, float* lse, void* workspace, uint64_t workspace_bytes,
+                     int device, void* stream) {
+    if (const char* why = bad_desc(d)) return imp_fail(IMP_E_ARG, why);
+    if (!q || !k || !v || !out) return imp_fail(IMP_E_ARG, "imp_attn_forward: null argument");
+    const Plan pl = plan(*d);
+    if (unaligned({q, k, v, out, workspace})) return imp_fail(IMP_E_ARG, "imp_attn_forward: pointers must be aligned to 16 bytes");
+    if (workspace_bytes < pl.fwd_bytes || (pl.fwd_bytes && !workspace)) return imp_fail(IMP_E_NOMEM, "imp_attn_forward: workspace too small (imp_attn_workspace)");
+    if (int rc = on_device(device)) return rc;
+    AttnOp p = op_of(*d);
+    p.q = q; p.k = k; p.v = v; p.o = out; p.lse = lse;
+    p.shares = pl.fwd;
+    p.part = (float*)workspace;
+    p.part_lse = p.part + (int64_t)pl.fwd * pl.q_rows * d->head_dim;
+    const hipStream_t st = (hipStream_t)stream;
+    launch_any(d->dtype, 0, p, st);
+    if (pl.fwd > 1) {
+        const unsigned grid = (unsigned)((pl.q_rows + 3) / 4);
+        if (d->dtype == IMP_DTYPE_F32) attn_join_kernel<float><<<grid, 256, 0, st>>>(p);
+        else if (d->dtype == IMP_DTYPE_BF16) attn_join_kernel<__bf16><<<grid, 256, 0, st>>>(p);
+        else attn_join_kernel<_Float16><<<grid, 256, 0, st>>>(p);
+    }
+    return launched("imp_attn_forward");
+}
+
+int imp_attn_backward(const imp_attn_desc* d, const void* q, const void* k, const void* v, const void* out, const float* lse, const void* dout, void* dq,
+                      void* dk, void* dv, void* workspace, uint64_t workspace_bytes, int device, void* stream) {
+    if (const char* why = bad_desc(d)) return imp_fail(IMP_E_ARG, why);
+    if (!q || !k || !v || !out || !lse || !dout || (!dq && !dk && !dv) || (!dk != !dv)) return imp_fail(IMP_E_ARG, "imp_attn_backward: null argument");
+    const Plan pl = plan(*d);
+    if (unaligned({q, k, v, out, dout, dq, dk, dv, workspace})) return imp_fail(IMP_E_ARG, "imp_attn_backward: pointers must be aligned to 16 bytes");
+    if (workspace_bytes < pl.bwd_bytes || !workspace) return imp_fail(IMP_E_NOMEM, "imp_attn_backward: workspace too small (imp_attn_workspace)");
+    if (int rc = on_device(device)) return rc;
+    AttnOp p = op_of(*d);
+    p.q = q; p.k = k; p.v = v; p.out = out; p.lse = const_cast<float*>(lse); p.dout = dout; p.dq = dq; p.dk = dk; p.dv = dv;
+    p.delta = (float*)workspace;
+    p.part = (float*)((char*)workspace + ((size_t)pl.q_rows * 4 + 15) / 16 * 16);
+    const hipStream_t st = (hipStream_t)stream;
+    const int dt = d->dtype;
+    auto each = [&](auto f) {
+        if (dt == IMP_DTYPE_F32) f((float*)nullptr);
+        else if (dt == IMP_DTYPE_BF16) f((__bf16*)nullptr);
+        else f((_Float16*)nullptr);
+    };
+    each([&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        attn_delta_kernel<T><<<(unsigned)((pl.q_rows + 15) / 16), 256, 0, st>>>(p);
+    });
+    auto join = [&](int64_t rows, int parts, int which, void* to) {
+        const int64_t n = rows * d->head_dim;
+        each([&](auto* t) {
+            using T = std::remove_pointer_t<decltype(t)>;
+            attn_sum_kernel<T><<<(unsigned)((n / 4 + 255) / 256), 256, 0, st>>>(p.part + which * n, n, parts * n, p.shares, (T*)to);
+        });
+    };
+    if (dk) {
+        p.shares = pl.dkv;
+        launch_any(dt, 2, p, st);
+        if (p.shares > 1) { join(pl.k_rows, 2, 0, dk); join(pl.k_rows, 2, 1, dv); }
+    }
+    if (dq) {
+        p.shares = pl.dq;
+        launch_any(dt, 1, p, st);
+        if (p.shares > 1) join(pl.q_rows, 1, 0, dq);
+    }
+    return launched("imp_attn_backward");
+}
+
+}  // extern "C"

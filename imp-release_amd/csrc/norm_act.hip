@@ -1,0 +1,396 @@
+// Group norm with an activation on token-major (channels-last) data, forward and backward (C-ABI imp_group_norm_act_forward / _backward; gfx950).
+// x [batch][n][channels] fp32 / fp16 / bf16, `groups` groups of neighbouring channels, statistics over the tokens of a batch element and the channels of a group
+// (groups == channels: the InstanceNorm of the matcher's MLPs, nets/layers.py:59-77), optional affine weight / bias, optional per-element token counts:
+//   xh = (x - mean) rstd, rstd = 1 / sqrt(var + eps) (biased variance), z = w xh + b, y = act(z)
+//   dz = dy act'(z), g = w dz:   dx = rstd (g - mean(g) - xh mean(g xh))    dw = sum dz xh    db = sum dz
+// Tokens past an element's count do not exist: not read, 0 in y and dx.
+//
+// Sums are taken in 64 bits around the group's first element (no cancellation, and the sign of x - mean, where the slope of relu / lrelu jumps, is that of the
+// exact mean: the mean is kept as two floats).  Bound by memory: x is read for the statistics and again to normalise (from the 256-MB cache where it fits).
+#include "../../include/imp_hip.h"
+#include "imp_kernels.h"
+
+int imp_fail(int code, const char* msg);   // context.hip: sets imp_last_error()
+
+namespace {
+
+struct NormOp {
+    const void *x, *dy;
+    void *y, *dx;
+    const float *w, *b;
+    const int32_t* lens;
+    float4* stats;                      // [batch][groups] mean (two floats), rstd (two floats)
+    double2* part;                      // [batch][channels][chunks]
+    double2* chan;                      // backward: [batch][channels] sums over the tokens
+    float2* mom;                        // backward: [batch][groups] mean(g), mean(g xh)
+    float *dw, *db;
+    int B, N, C, G, cg, act;
+    float eps;
+    int tc, chunks, rows;               // thread columns (a power of two), token chunks, tokens per chunk
+};
+
+template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
+
+__device__ __forceinline__ int len_of(const NormOp& p, int b) { return p.lens ? min(max(p.lens[b], 0), p.N) : p.N; }
+
+__device__ __forceinline__ float act_of(int act, float z) {
+    switch (act) {
+        case IMP_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
+        case IMP_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+        case IMP_ACT_LRELU: return z > 0.f ? z : 0.1f * z;
+        case IMP_ACT_SILU: return z / (1.f + __expf(-z));
+        default: return z;
+    }
+}
+// act'(z); `above`: whether z > 0 in the precise sense
+__device__ __forceinline__ float slope_of(int act, float z, bool above) {
+    switch (act) {
+        case IMP_ACT_RELU: return above ? 1.f : 0.f;
+        case IMP_ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.3989422804014327f;
+        case IMP_ACT_LRELU: return above ? 1.f : 0.1f;
+        case IMP_ACT_SILU: { const float s = 1.f / (1.f + __expf(-z)); return s * (1.f + z * (1.f - s)); }
+        default: return 1.f;
+    }
+}
+
+// what a thread needs of its V channels
+template <int V> struct Chan {
+    float mh[V], ml[V], rh[V], w[V], b[V];
+    __device__ void load(const NormOp& p, int bi, int c0) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float4 s = p.stats[(int64_t)bi * p.G + (c0 + i) / p.cg];
+            mh[i] = s.x; ml[i] = s.y; rh[i] = s.z;
+            w[i] = p.w ? p.w[c0 + i] : 1.f;
+            b[i] = p.b ? p.b[c0 + i] : 0.f;
+        }
+    }
+    __device__ float xh(float x, int i) const { return ((x - mh[i]) - ml[i]) * rh[i]; }
+};
+// z > 0.  Without an affine part that is the sign of x - mean; with one, z next to 0 is formed again in 64 bits
+__device__ __forceinline__ bool above_zero(const NormOp& p, int bi, int c, float x, float mh, float ml, float xh, float w, float b) {
+    const float a = xh * w, z = a + b;
+    if (!p.b && !p.w) return xh > 0.f;
+    if (fabsf(z) > 1e-5f * (fabsf(a) + fabsf(b))) return z > 0.f;
+    const float4 s = p.stats[(int64_t)bi * p.G + c / p.cg];
+    return (((double)x - mh) - ml) * ((double)s.z + s.w) * w + b > 0.0;
+}
+
+// tokens [r0, r1) of batch element b, V channels from c0: 256 threads = tc columns x 256 / tc token rows
+struct Place { int b, c0, tr, step, r0, r1; bool on; };
+template <int V> __device__ __forceinline__ Place place(const NormOp& p, int rows) {
+    Place q;
+    q.b = blockIdx.z;
+    q.c0 = (blockIdx.y * p.tc + (int)(threadIdx.x % p.tc)) * V;
+    q.tr = threadIdx.x / p.tc;
+    q.step = 256 / p.tc;
+    q.r0 = blockIdx.x * rows;
+    q.r1 = min(q.r0 + rows, p.N);
+    q.on = q.c0 < p.C;
+    return q;
+}
+
+// sums over the token rows of a workgroup -> part[b][c][chunk]
+template <int V> __device__ __forceinline__ void write_part(const NormOp& p, const Place& q, const double (&s)[V], const double (&t)[V]) {
+    __shared__ double2 sm[256];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        __syncthreads();
+        sm[threadIdx.x] = double2{s[i], t[i]};
+        for (int o = 128; o >= p.tc; o >>= 1) {
+            __syncthreads();
+            if (threadIdx.x < o) { sm[threadIdx.x].x += sm[threadIdx.x + o].x; sm[threadIdx.x].y += sm[threadIdx.x + o].y; }
+        }
+        if (threadIdx.x < p.tc && q.on) p.part[((int64_t)q.b * p.C + q.c0 + i) * p.chunks + blockIdx.x] = sm[threadIdx.x];
+    }
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(256) void norm_sums_kernel(NormOp p) {
+    const Place q = place<V>(p, p.rows);
+    const T* x = (const T*)p.x + (int64_t)q.b * p.N * p.C;
+    const int end = min(q.r1, len_of(p, q.b));
+    float piv[V];
+    double s[V], t[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) { s[i] = 0; t[i] = 0; piv[i] = q.on ? (float)x[(q.c0 + i) / p.cg * p.cg] : 0.f; }
+    if (q.on)
+        for (int r = q.r0 + q.tr; r < end; r += q.step) {
+            const Pack<T, V> v = *(const Pack<T, V>*)(x + (int64_t)r * p.C + q.c0);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const double d = (float)v.v[i] - piv[i];
+                s[i] += d;
+                t[i] += d * d;
+            }
+        }
+    write_part<V>(p, q, s, t);
+}
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+// one wave per (batch element, group)
+template <typename T>
+__global__ __launch_bounds__(256) void norm_stats_kernel(NormOp p) {
+    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (at >= (int64_t)p.B * p.G) return;
+    const int b = (int)(at / p.G), g = (int)(at % p.G);
+    const double2* part = p.part + ((int64_t)b * p.C + (int64_t)g * p.cg) * p.chunks;
+    const int64_t n = (int64_t)p.cg * p.chunks;
+    double s = 0, t = 0;
+    for (int64_t i = lane; i < n; i += 64) { s += part[i].x; t += part[i].y; }
+    s = wave_sum(s);
+    t = wave_sum(t);
+    if (lane) return;
+    const int len = len_of(p, b);
+    const double cnt = (double)len * p.cg, off = cnt > 0 ? s / cnt : 0, var = cnt > 0 ? t / cnt - off * off : 0;
+    const double mean = (double)(float)((const T*)p.x)[(int64_t)b * p.N * p.C + (int64_t)g * p.cg] + off;
+    const double r = 1.0 / sqrt((var < 0 ? 0 : var) + (double)p.eps);
+    float4 o;
+    o.x = (float)mean; o.y = (float)(mean - (double)o.x);
+    o.z = (float)r; o.w = (float)(r - (double)o.z);
+    p.stats[at] = o;
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(256) void norm_apply_kernel(NormOp p) {
+    const Place q = place<V>(p, p.rows);
+    if (!q.on) return;
+    const int len = len_of(p, q.b);
+    const T* x = (const T*)p.x + (int64_t)q.b * p.N * p.C + q.c0;
+    T* y = (T*)p.y + (int64_t)q.b * p.N * p.C + q.c0;
+    Chan<V> ch;
+    ch.load(p, q.b, q.c0);
+    for (int r = q.r0 + q.tr; r < q.r1; r += q.step) {
+        Pack<T, V> o;
+        if (r < len) {
+            const Pack<T, V> v = *(const Pack<T, V>*)(x + (int64_t)r * p.C);
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.v[i] = (T)act_of(p.act, __builtin_fmaf(ch.xh((float)v.v[i], i), ch.w[i], ch.b[i]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.v[i] = (T)0.f;
+        }
+        *(Pack<T, V>*)(y + (int64_t)r * p.C) = o;
+    }
+}
+
+template <int V> __device__ __forceinline__ float dz_of(const NormOp& p, const Chan<V>& ch, int b, int c, int i, float x, float dy, float& xh) {
+    xh = ch.xh(x, i);
+    const float z = __builtin_fmaf(xh, ch.w[i], ch.b[i]);
+    const bool jump = p.act == IMP_ACT_RELU || p.act == IMP_ACT_LRELU;
+    return dy * slope_of(p.act, z, jump && above_zero(p, b, c, x, ch.mh[i], ch.ml[i], xh, ch.w[i], ch.b[i]));
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(256) void norm_grad_sums_kernel(NormOp p) {
+    const Place q = place<V>(p, p.rows);
+    const T* x = (const T*)p.x + (int64_t)q.b * p.N * p.C + q.c0;
+    const T* dy = (const T*)p.dy + (int64_t)q.b * p.N * p.C + q.c0;
+    const int end = min(q.r1, len_of(p, q.b));
+    double s[V], t[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) { s[i] = 0; t[i] = 0; }
+    if (q.on) {
+        Chan<V> ch;
+        ch.load(p, q.b, q.c0);
+        for (int r = q.r0 + q.tr; r < end; r += q.step) {
+            const Pack<T, V> v = *(const Pack<T, V>*)(x + (int64_t)r * p.C), d = *(const Pack<T, V>*)(dy + (int64_t)r * p.C);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float xh;
+                const double dz = dz_of<V>(p, ch, q.b, q.c0 + i, i, (float)v.v[i], (float)d.v[i], xh);
+                s[i] += dz;
+                t[i] += dz * xh;
+            }
+        }
+    }
+    write_part<V>(p, q, s, t);
+}
+
+// one wave per (batch element, group): sums per channel, and the two means of the group
+__global__ __launch_bounds__(256) void norm_grad_means_kernel(NormOp p) {
+    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (at >= (int64_t)p.B * p.G) return;
+    const int b = (int)(at / p.G), g = (int)(at % p.G);
+    double m1 = 0, m2 = 0;
+    for (int c = g * p.cg; c < (g + 1) * p.cg; ++c) {
+        const double2* part = p.part + ((int64_t)b * p.C + c) * p.chunks;
+        double s = 0, t = 0;
+        for (int i = lane; i < p.chunks; i += 64) { s += part[i].x; t += part[i].y; }
+        s = wave_sum(s);
+        t = wave_sum(t);
+        if (lane == 0) p.chan[(int64_t)b * p.C + c] = double2{s, t};
+        const double w = p.w ? p.w[c] : 1.0;
+        m1 += w * s;
+        m2 += w * t;
+    }
+    const double cnt = (double)len_of(p, b) * p.cg;
+    if (lane == 0) p.mom[at] = float2{cnt > 0 ? (float)(m1 / cnt) : 0.f, cnt > 0 ? (float)(m2 / cnt) : 0.f};
+}
+
+__global__ __launch_bounds__(256) void norm_affine_kernel(NormOp p) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= p.C) return;
+    double s = 0, t = 0;
+    for (int b = 0; b < p.B; ++b) { const double2 v = p.chan[(int64_t)b * p.C + c]; s += v.x; t += v.y; }
+    if (p.db) p.db[c] = (float)s;
+    if (p.dw) p.dw[c] = (float)t;
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(256) void norm_grad_kernel(NormOp p) {
+    const Place q = place<V>(p, p.rows);
+    if (!q.on) return;
+    const int len = len_of(p, q.b);
+    const int64_t base = (int64_t)q.b * p.N * p.C + q.c0;
+    const T *x = (const T*)p.x + base, *dy = (const T*)p.dy + base;
+    T* dx = (T*)p.dx + base;
+    Chan<V> ch;
+    ch.load(p, q.b, q.c0);
+    float m1[V], m2[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) { const float2 m = p.mom[(int64_t)q.b * p.G + (q.c0 + i) / p.cg]; m1[i] = m.x; m2[i] = m.y; }
+    for (int r = q.r0 + q.tr; r < q.r1; r += q.step) {
+        Pack<T, V> o;
+        if (r < len) {
+            const Pack<T, V> v = *(const Pack<T, V>*)(x + (int64_t)r * p.C), d = *(const Pack<T, V>*)(dy + (int64_t)r * p.C);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float xh;
+                const float dz = dz_of<V>(p, ch, q.b, q.c0 + i, i, (float)v.v[i], (float)d.v[i], xh);
+                o.v[i] = (T)((dz * ch.w[i] - m1[i] - xh * m2[i]) * ch.rh[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.v[i] = (T)0.f;
+        }
+        *(Pack<T, V>*)(dx + (int64_t)r * p.C) = o;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------------- host
+// vectors of 16 bytes where a row is a whole number of them
+int vec_of(int dtype, int C) { const int v = dtype == IMP_DTYPE_F32 ? 4 : 8; return C % v == 0 ? v : 1; }
+
+struct Shape { int vec, tc, cols, chunks, rows, achunks, arows; };
+Shape shape_of(int dtype, int B, int N, int C) {
+    Shape s;
+    s.vec = vec_of(dtype, C);
+    const int lanes = (C + s.vec - 1) / s.vec;
+    s.tc = 1;
+    while (s.tc < lanes && s.tc < 256) s.tc *= 2;
+    s.cols = (lanes + s.tc - 1) / s.tc;
+    const int tr = 256 / s.tc;
+    // token chunks: four workgroups per CU for the sums (each a record per channel), sixteen for the elementwise passes, at least eight / four tokens per thread
+    auto split = [&](int64_t want, int least, int& chunks, int& rows) {
+        const int64_t most = (N + (int64_t)tr * least - 1) / ((int64_t)tr * least), others = (int64_t)B * s.cols;
+        int64_t c = (want + others - 1) / others;
+        c = c < most ? c : most;
+        if (c < 1) c = 1;
+        rows = (int)((N + c - 1) / c);
+        chunks = (N + rows - 1) / rows;
+    };
+    split(1024, 8, s.chunks, s.rows);
+    split(4096, 4, s.achunks, s.arows);
+    return s;
+}
+
+const char* bad(int dtype, int B, int N, int C, int G, int act, const void* x, std::initializer_list<const void*> ptrs) {
+    if (dtype != IMP_DTYPE_F32 && dtype != IMP_DTYPE_F16 && dtype != IMP_DTYPE_BF16) return "unknown dtype";
+    if (B < 1 || N < 1 || C < 1 || B > 65535) return "batch must be between 1 and 65535, tokens and channels at least 1";
+    if (G < 1 || C % G) return "channels must be a multiple of groups";
+    if (C > (1 << 20) || N > (1 << 30)) return "too many channels or tokens";
+    if (act < IMP_ACT_RELU || act > IMP_ACT_NONE) return "unknown activation";
+    if (!x) return "null argument";
+    for (const void* q : ptrs) if ((uintptr_t)q & 15) return "tensors must be aligned to 16 bytes";
+    return nullptr;
+}
+uint64_t fwd_bytes(const Shape& s, int B, int C) { return (uint64_t)B * C * s.chunks * 16; }
+uint64_t bwd_bytes(const Shape& s, int B, int C, int G) { return fwd_bytes(s, B, C) + (uint64_t)B * C * 16 + (uint64_t)B * G * 8; }
+
+template <typename F> void by_type(int dtype, int vec, F f) {
+    if (dtype == IMP_DTYPE_F32) { if (vec > 1) f((float*)nullptr, std::integral_constant<int, 4>()); else f((float*)nullptr, std::integral_constant<int, 1>()); }
+    else if (dtype == IMP_DTYPE_F16) { if (vec > 1) f((_Float16*)nullptr, std::integral_constant<int, 8>()); else f((_Float16*)nullptr, std::integral_constant<int, 1>()); }
+    else { if (vec > 1) f((__bf16*)nullptr, std::integral_constant<int, 8>()); else f((__bf16*)nullptr, std::integral_constant<int, 1>()); }
+}
+int ready(int device) {
+    hipError_t e = hipSetDevice(device);
+    return e == hipSuccess ? 0 : imp_fail(IMP_E_HIP, hipGetErrorString(e));
+}
+int done() {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? IMP_OK : imp_fail(IMP_E_HIP, hipGetErrorString(e));
+}
+
+}  // namespace
+
+extern "C" {
+
+int imp_group_norm_act_workspace(int dtype, int batch, int n, int channels, int groups, int backward, uint64_t* bytes) {
+    if (const char* why = bad(dtype, batch, n, channels, groups, 0, bytes, {})) return imp_fail(IMP_E_ARG, why);
+    const Shape s = shape_of(dtype, batch, n, channels);
+    *bytes = backward ? bwd_bytes(s, batch, channels, groups) : fwd_bytes(s, batch, channels);
+    return IMP_OK;
+}
+
+int imp_group_norm_act_forward(int dtype, int batch, int n, int channels, int groups, const void* x, const float* weight, const float* bias, const int32_t* lens,
+                               float eps, int act, void* y, float* stats, void* workspace, uint64_t workspace_bytes, int device, void* stream) {
+    if (const char* why = bad(dtype, batch, n, channels, groups, act, x, {x, y, stats, workspace})) return imp_fail(IMP_E_ARG, why);
+    if (!y || !stats || !(eps > 0.f)) return imp_fail(IMP_E_ARG, "imp_group_norm_act_forward: null argument, or eps not positive");
+    const Shape s = shape_of(dtype, batch, n, channels);
+    if (!workspace || workspace_bytes < fwd_bytes(s, batch, channels)) return imp_fail(IMP_E_NOMEM, "imp_group_norm_act_forward: workspace too small");
+    if (int rc = ready(device)) return rc;
+    NormOp p = {};
+    p.x = x; p.y = y; p.w = weight; p.b = bias; p.lens = lens; p.stats = (float4*)stats; p.part = (double2*)workspace;
+    p.B = batch; p.N = n; p.C = channels; p.G = groups; p.cg = channels / groups; p.act = act; p.eps = eps;
+    p.tc = s.tc; p.chunks = s.chunks; p.rows = s.rows;
+    const hipStream_t st = (hipStream_t)stream;
+    by_type(dtype, s.vec, [&](auto* t, auto v) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        constexpr int V = decltype(v)::value;
+        norm_sums_kernel<T, V><<<dim3(s.chunks, s.cols, batch), 256, 0, st>>>(p);
+        norm_stats_kernel<T><<<(unsigned)(((int64_t)batch * groups + 3) / 4), 256, 0, st>>>(p);
+        NormOp a = p;
+        a.chunks = s.achunks; a.rows = s.arows;
+        norm_apply_kernel<T, V><<<dim3(s.achunks, s.cols, batch), 256, 0, st>>>(a);
+    });
+    return done();
+}
+
+int imp_group_norm_act_backward(int dtype, int batch, int n, int channels, int groups, const void* x, const float* weight, const float* bias, const int32_t* lens,
+                                int act, const float* stats, const void* dy, void* dx, float* dweight, float* dbias, void* workspace, uint64_t workspace_bytes,
+                                int device, void* stream) {
+    if (const char* why = bad(dtype, batch, n, channels, groups, act, x, {x, dy, dx, stats, workspace})) return imp_fail(IMP_E_ARG, why);
+    if (!stats || !dy || !dx) return imp_fail(IMP_E_ARG, "imp_group_norm_act_backward: null argument");
+    const Shape s = shape_of(dtype, batch, n, channels);
+    if (!workspace || workspace_bytes < bwd_bytes(s, batch, channels, groups)) return imp_fail(IMP_E_NOMEM, "imp_group_norm_act_backward: workspace too small");
+    if (int rc = ready(device)) return rc;
+    NormOp p = {};
+    p.x = x; p.dy = dy; p.dx = dx; p.w = weight; p.b = bias; p.lens = lens; p.stats = (float4*)const_cast<float*>(stats); p.dw = dweight; p.db = dbias;
+    p.part = (double2*)workspace;
+    p.chan = p.part + (int64_t)batch * channels * s.chunks;
+    p.mom = (float2*)(p.chan + (int64_t)batch * channels);
+    p.B = batch; p.N = n; p.C = channels; p.G = groups; p.cg = channels / groups; p.act = act;
+    p.tc = s.tc; p.chunks = s.chunks; p.rows = s.rows;
+    const hipStream_t st = (hipStream_t)stream;
+    by_type(dtype, s.vec, [&](auto* t, auto v) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        constexpr int V = decltype(v)::value;
+        norm_grad_sums_kernel<T, V><<<dim3(s.chunks, s.cols, batch), 256, 0, st>>>(p);
+        norm_grad_means_kernel<<<(unsigned)(((int64_t)batch * groups + 3) / 4), 256, 0, st>>>(p);
+        if (dweight || dbias) norm_affine_kernel<<<(channels + 255) / 256, 256, 0, st>>>(p);
+        NormOp a = p;
+        a.chunks = s.achunks; a.rows = s.arows;
+        norm_grad_kernel<T, V><<<dim3(s.achunks, s.cols, batch), 256, 0, st>>>(a);
+    });
+    return done();
+}
+
+}  // extern "C"

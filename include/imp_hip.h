@@ -481,6 +481,64 @@ int imp_sp_dense(imp_sp_ctx* ctx, float* scores, float* nms_scores, float* descr
  * output channels), 9 = convDb (1x1).  in [B][H][W][Cin] -> out [B][Ho][Wo][Cout], pool != 0 fuses MaxPool2d(2, 2) (Ho = H / 2). */
 int imp_sp_op_conv(imp_sp_ctx* ctx, int layer, const float* in, int B, int H, int W, float* out, int relu, int pool, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------------------
+ * Operators with gradients, for training and scoring next to the matcher.  Context-free: every call names its `device`, runs on `stream`, allocates nothing (scratch memory
+ * comes from the caller: ask the *_workspace function; a call may overlap another only on its own workspace) and never synchronises, so that it can be captured into a
+ * graph.  Results do not depend on timing: no atomics, every sum in an order that the sizes alone decide.  Arguments that the host can see are checked (IMP_E_ARG);
+ * counts and targets are device data: counts are clamped to the tensor, targets as described. */
+#define IMP_DTYPE_F32 0
+#define IMP_DTYPE_F16 1
+#define IMP_DTYPE_BF16 2
+
+/* Multi-head attention with gradients (csrc/attention_grad.hip; the operation of nets/layers.py:121-131 with any number of heads, shared key heads and types):
+ *   S = scale q.k   P = softmax of S over the kept keys   out = P v   lse = log sum exp S
+ * q [batch][nq][heads][head_dim], k, v [batch][nk][kv_heads][head_dim], all of `dtype`, channels contiguous, other strides in elements (batch, token, head; multiples of
+ * 16 bytes, so a packed q | k | v projection is taken as it lies); query head h reads key head h / (heads / kv_heads).  head_dim a multiple of 8 up to 128.
+ * key_mask: optional uint8 [batch][nk], 0 = the key does not exist; q_lens / k_lens: optional int32 [batch] counts of a ragged batch (clamped to 0 .. nq / nk).  What does not
+ * exist is never read into a result (it may hold NaN).  A query without a key, and a query past its count: out 0, lse -inf, no gradient. */
+typedef struct imp_attn_desc {
+    int32_t dtype, batch, nq, nk, heads, kv_heads, head_dim;
+    float scale;
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    const uint8_t* key_mask;
+    const int32_t* q_lens;
+    const int32_t* k_lens;
+} imp_attn_desc;
+int imp_attn_workspace(const imp_attn_desc* d, int backward, uint64_t* bytes);
+/* out [batch][nq][heads][head_dim] contiguous, lse [batch][heads][nq] float32 (optional: needed by the backward) */
+int imp_attn_forward(const imp_attn_desc* d, const void* q, const void* k, const void* v, void* out, float* lse, void* workspace, uint64_t workspace_bytes,
+                     int device, void* stream);
+/* gradients from dout (contiguous like out) and the forward's out and lse; dq like out, dk, dv [batch][nk][kv_heads][head_dim] contiguous: dq, or dk and dv, may be NULL */
+int imp_attn_backward(const imp_attn_desc* d, const void* q, const void* k, const void* v, const void* out, const float* lse, const void* dout, void* dq, void* dk,
+                      void* dv, void* workspace, uint64_t workspace_bytes, int device, void* stream);
+
+/* Group norm + activation on token-major data (csrc/norm_act.hip; groups == channels: the InstanceNorm + activation of nets/layers.py:59-77): x, y [batch][n][channels] of
+ * `dtype`, weight / bias float32 [channels] (optional), lens int32 [batch] (optional; clamped to 0 .. n; tokens past it are not read, y and dx are 0 there), act IMP_ACT_*,
+ * stats float32 [batch][groups][4] (mean and rstd, two floats each): written by the forward, read by the backward. */
+#define IMP_ACT_SILU 3      /* these operators only */
+#define IMP_ACT_NONE 4
+int imp_group_norm_act_workspace(int dtype, int batch, int n, int channels, int groups, int backward, uint64_t* bytes);
+int imp_group_norm_act_forward(int dtype, int batch, int n, int channels, int groups, const void* x, const float* weight, const float* bias, const int32_t* lens,
+                               float eps, int act, void* y, float* stats, void* workspace, uint64_t workspace_bytes, int device, void* stream);
+/* dx like x; dweight / dbias float32 [channels] (optional) */
+int imp_group_norm_act_backward(int dtype, int batch, int n, int channels, int groups, const void* x, const float* weight, const float* bias, const int32_t* lens,
+                                int act, const float* stats, const void* dy, void* dx, float* dweight, float* dbias, void* workspace, uint64_t workspace_bytes,
+                                int device, void* stream);
+
+/* Log probabilities of given matches (csrc/log_probs.hip; the row softmax of nets/layers.py:20-24 as a loss and as a confidence): logits [rows][cols] of `dtype`, row stride
+ * `ld` elements; bin_score: optional DEVICE float32, the dustbin: one more column `cols` of that value in every row (cols may then be 0).  targets int64 [rows]: a column; -1 =
+ * unmatched (the dustbin where there is one, else no target); -2 = no target; anything else gives NaN.  logp float32 [rows] = log softmax at the target (0 without a target),
+ * entropy float32 [rows] of the whole row, stats float32 [rows][2] for the backward, top_logp float32 / top_ids int64 [rows][top] the `top` <= 16 largest columns, largest
+ * first, ties to the lower index (the dustbin is column `cols`; -inf / -1 where there are no more).  A logit of -inf is masked: no probability, never an alternative; a row of
+ * nothing else: logp -inf, entropy 0, no gradient.  A row with a NaN or +inf: NaN. */
+int imp_log_probs_workspace(int64_t rows, int cols, int top, int backward, uint64_t* bytes);
+int imp_log_probs_forward(int dtype, int64_t rows, int cols, int64_t ld, const void* logits, const float* bin_score, const int64_t* targets, int top, float* logp,
+                          float* entropy, float* stats, float* top_logp, int64_t* top_ids, void* workspace, uint64_t workspace_bytes, int device, void* stream);
+/* gradient from those of logp and entropy (float32 [rows], either may be NULL): dlogits [rows][cols] contiguous and / or dbin float32 [1] */
+int imp_log_probs_backward(int dtype, int64_t rows, int cols, int64_t ld, const void* logits, const float* bin_score, const int64_t* targets, const float* entropy,
+                           const float* stats, const float* dlogp, const float* dentropy, void* dlogits, float* dbin, void* workspace, uint64_t workspace_bytes,
+                           int device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
