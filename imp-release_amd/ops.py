@@ -11,6 +11,7 @@ are no autograd functions themselves).  Nothing waits for the GPU and nothing is
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from typing import Optional
 
@@ -18,7 +19,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import ACT_IDS, DTYPE_IDS, ImpAttnDesc, ImpError, _ptr
+from ._lib import ACT_IDS, DTYPE_IDS, ImpAttnDesc, ImpError
 
 OP_ACT_IDS = {**ACT_IDS, 'silu': 3, 'none': 4}
 
@@ -55,74 +56,98 @@ def _scratch(nbytes, device):
 
 def _where(t):
     """(device index, its current stream)"""
-    return t.device.index, C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+    i = t.device.index
+    return i, torch._C._cuda_getCurrentRawStream(i)
 
 
-def _aligned(t):
-    return t.data_ptr() % 16 == 0
+def _dense(t, dtype):
+    """a gradient as the kernels take it"""
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 # --------------------------------------------------------------------------------------------------------------------------- attention
+@functools.lru_cache(maxsize=1024)
+def _regular(shape, stride, size):
+    unit = 16 // size
+    return (shape[3] == 1 or stride[3] == 1) and all(shape[i] == 1 or (stride[i] % unit == 0 and stride[i] > 0) for i in range(3))
+
+
 def _rows(t):
     """t [batch, tokens, heads, channels] as the kernels take it: channels contiguous, everything else in steps of 16 bytes (a copy if it is not)"""
-    unit = 16 // t.element_size()
-    ok = (t.shape[3] == 1 or t.stride(3) == 1) and _aligned(t) and all(t.shape[i] == 1 or (t.stride(i) % unit == 0 and t.stride(i) > 0) for i in range(3))
-    return t if ok else t.contiguous()
+    if t.data_ptr() % 16 == 0 and _regular(t.shape, t.stride(), t.element_size()):
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _strides(t):
-    return (C.c_int64 * 3)(*[0 if t.shape[i] == 1 else t.stride(i) for i in range(3)])
-
-
-def _desc(q, k, v, mask, q_lens, k_lens, scale):
+@functools.lru_cache(maxsize=1024)
+def _attn_plan(dtype, q_shape, k_shape, q_stride, k_stride, v_stride, scale):
+    """(the description of a problem of these sizes, without masks; scratch bytes of the forward; of the backward)"""
     d = ImpAttnDesc()
-    d.dtype, d.batch, d.nq, d.nk, d.heads, d.kv_heads, d.head_dim = DTYPE_IDS[q.dtype], q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3]
-    d.scale = scale
-    d.q_stride, d.k_stride, d.v_stride = _strides(q), _strides(k), _strides(v)
-    d.key_mask, d.q_lens, d.k_lens = (None if t is None else t.data_ptr() for t in (mask, q_lens, k_lens))
-    return d
+    d.dtype, d.batch, d.nq, d.nk, d.heads, d.kv_heads, d.head_dim, d.scale = dtype, q_shape[0], q_shape[1], k_shape[1], q_shape[2], k_shape[2], q_shape[3], scale
+    for field, shape, stride in ((d.q_stride, q_shape, q_stride), (d.k_stride, k_shape, k_stride), (d.v_stride, k_shape, v_stride)):
+        for i in range(3):
+            field[i] = 0 if shape[i] == 1 else stride[i]
+    need = []
+    for backward in (0, 1):
+        n = C.c_uint64()
+        _check(_lib.lib().imp_attn_workspace(C.byref(d), backward, C.byref(n)))
+        need.append(n.value)
+    return d, need[0], need[1]
+
+
+def _attn_desc(q, k, v, mask, q_lens, k_lens, scale):
+    d, fwd, bwd = _attn_plan(DTYPE_IDS[q.dtype], q.shape, k.shape, q.stride(), k.stride(), v.stride(), scale)
+    if mask is not None or q_lens is not None or k_lens is not None:
+        d = ImpAttnDesc.from_buffer_copy(d)
+        d.key_mask, d.q_lens, d.k_lens = (None if t is None else t.data_ptr() for t in (mask, q_lens, k_lens))
+    return d, fwd, bwd
 
 
 def _attn_forward(q, k, v, mask, q_lens, k_lens, scale, want_lse):
-    L = _lib.lib()
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    d = _desc(q, k, v, mask, q_lens, k_lens, scale)
-    need = C.c_uint64()
-    _check(L.imp_attn_workspace(C.byref(d), 0, C.byref(need)))
+    d, need, _ = _attn_desc(q, k, v, mask, q_lens, k_lens, scale)
     out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], device=q.device, dtype=torch.float32) if want_lse else None
-    ws = _scratch(need.value, q.device)
-    _check(L.imp_attn_forward(C.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(ws), need, *_where(q)))
+    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), device=q.device, dtype=torch.float32) if want_lse else None
+    ws = _scratch(need, q.device)
+    _check(_lib.lib().imp_attn_forward(d, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if want_lse else None,
+                                       ws.data_ptr() if need else None, need, *_where(q)))
     return out, lse
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, q_lens, k_lens, scale):
+        q, k, v = _rows(q), _rows(k), _rows(v)
         out, lse = _attn_forward(q, k, v, mask, q_lens, k_lens, scale, True)
         ctx.save_for_backward(q, k, v, out, lse, mask, q_lens, k_lens)
         ctx.scale = scale
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
         return out, lse
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, _):
+        if dout is None:
+            return None, None, None, None, None, None, None
         q, k, v, out, lse, mask, q_lens, k_lens = ctx.saved_tensors
-        L = _lib.lib()
-        q, k, v = _rows(q), _rows(k), _rows(v)
-        dout = dout.to(out.dtype).contiguous()
-        dout = dout if _aligned(dout) else dout.clone()
-        d = _desc(q, k, v, mask, q_lens, k_lens, ctx.scale)
-        need = C.c_uint64()
-        _check(L.imp_attn_workspace(C.byref(d), 1, C.byref(need)))
-        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype) if ctx.needs_input_grad[0] else None
-        kv = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        dk = torch.empty(k.shape, device=k.device, dtype=k.dtype) if kv else None
-        dv = torch.empty(v.shape, device=v.device, dtype=v.dtype) if kv else None
-        ws = _scratch(need.value, q.device)
-        _check(L.imp_attn_backward(C.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), need, *_where(q)))
-        return dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None, None
+        dout = _dense(dout, out.dtype)
+        d, _, need = _attn_desc(q, k, v, mask, q_lens, k_lens, ctx.scale)
+        want_q, want_k, want_v = ctx.needs_input_grad[:3]
+        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype) if want_q else None
+        dk = dv = None
+        if want_k or want_v:
+            dk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+            dv = torch.empty(v.shape, device=v.device, dtype=v.dtype)
+        ws = _scratch(need, q.device)
+        _check(_lib.lib().imp_attn_backward(d, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+                                            dq.data_ptr() if want_q else None, None if dk is None else dk.data_ptr(), None if dv is None else dv.data_ptr(),
+                                            ws.data_ptr(), need, *_where(q)))
+        return dq, dk if want_k else None, dv if want_v else None, None, None, None, None
 
 
 def attention(q, k, v, key_mask: Optional[torch.Tensor] = None, q_lens=None, k_lens=None, scale: Optional[float] = None, return_lse: bool = False):
@@ -159,21 +184,31 @@ def attention(q, k, v, key_mask: Optional[torch.Tensor] = None, q_lens=None, k_l
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _Attention.apply(q, k, v, key_mask, q_lens, k_lens, scale)
     else:
-        out, lse = _attn_forward(q, k, v, key_mask, q_lens, k_lens, scale, return_lse)
+        out, lse = _attn_forward(_rows(q), _rows(k), _rows(v), key_mask, q_lens, k_lens, scale, return_lse)
     return (out, lse) if return_lse else out
 
 
 # -------------------------------------------------------------------------------------------------------------------------- group norm
-def _norm_forward(x, weight, bias, lens, groups, eps, act):
-    L = _lib.lib()
-    b, n, c = x.shape
+@functools.lru_cache(maxsize=1024)
+def _norm_scratch(dtype, b, n, c, groups, backward):
     need = C.c_uint64()
-    _check(L.imp_group_norm_act_workspace(DTYPE_IDS[x.dtype], b, n, c, groups, 0, C.byref(need)))
+    _check(_lib.lib().imp_group_norm_act_workspace(dtype, b, n, c, groups, backward, C.byref(need)))
+    return need.value
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _norm_forward(x, weight, bias, lens, groups, eps, act):
+    b, n, c = x.shape
+    dt = DTYPE_IDS[x.dtype]
+    need = _norm_scratch(dt, b, n, c, groups, 0)
     y = torch.empty_like(x)
-    stats = torch.empty(b, groups, 4, device=x.device, dtype=torch.float32)
-    ws = _scratch(need.value, x.device)
-    _check(L.imp_group_norm_act_forward(DTYPE_IDS[x.dtype], b, n, c, groups, _ptr(x), _ptr(weight), _ptr(bias), _ptr(lens), eps, act, _ptr(y), _ptr(stats), _ptr(ws),
-                                        need, *_where(x)))
+    stats = torch.empty((b, groups, 4), device=x.device, dtype=torch.float32)
+    ws = _scratch(need, x.device)
+    _check(_lib.lib().imp_group_norm_act_forward(dt, b, n, c, groups, x.data_ptr(), _at(weight), _at(bias), _at(lens), eps, act, y.data_ptr(), stats.data_ptr(),
+                                                 _at(ws), need, *_where(x)))
     return y, stats
 
 
@@ -189,18 +224,16 @@ class _GroupNormAct(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, weight, bias, lens, stats = ctx.saved_tensors
-        L = _lib.lib()
         b, n, c = x.shape
-        dy = dy.to(x.dtype).contiguous()
-        dy = dy if _aligned(dy) else dy.clone()
-        need = C.c_uint64()
-        _check(L.imp_group_norm_act_workspace(DTYPE_IDS[x.dtype], b, n, c, ctx.groups, 1, C.byref(need)))
+        dt = DTYPE_IDS[x.dtype]
+        dy = _dense(dy, x.dtype)
+        need = _norm_scratch(dt, b, n, c, ctx.groups, 1)
         dx = torch.empty_like(x)
         dw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
         db = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[2] else None
-        ws = _scratch(need.value, x.device)
-        _check(L.imp_group_norm_act_backward(DTYPE_IDS[x.dtype], b, n, c, ctx.groups, _ptr(x), _ptr(weight), _ptr(bias), _ptr(lens), ctx.act, _ptr(stats), _ptr(dy),
-                                             _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), need, *_where(x)))
+        ws = _scratch(need, x.device)
+        _check(_lib.lib().imp_group_norm_act_backward(dt, b, n, c, ctx.groups, x.data_ptr(), _at(weight), _at(bias), _at(lens), ctx.act, stats.data_ptr(),
+                                                      dy.data_ptr(), dx.data_ptr(), _at(dw), _at(db), _at(ws), need, *_where(x)))
         return dx if ctx.needs_input_grad[0] else None, dw, db, None, None, None, None
 
 
@@ -230,7 +263,7 @@ def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-3, ac
     if x.numel() == 0:
         return x + sum(t.sum() * 0 for t in (weight, bias) if t is not None)
     flat = x.reshape(b, -1, c).contiguous()
-    flat = flat if _aligned(flat) else flat.clone()
+    flat = flat if flat.data_ptr() % 16 == 0 else flat.clone()
     weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         y = _GroupNormAct.apply(flat, weight, bias, lens, groups, eps, OP_ACT_IDS[act])
@@ -240,23 +273,29 @@ def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-3, ac
 
 
 # ------------------------------------------------------------------------------------------------------------------- log probabilities
-def _logp_forward(x, targets, bin_score, top):
-    L = _lib.lib()
-    rows, cols = x.shape
-    dev = x.device
+@functools.lru_cache(maxsize=1024)
+def _logp_scratch(rows, cols, top, backward):
     need = C.c_uint64()
-    _check(L.imp_log_probs_workspace(rows, cols, top, 0, C.byref(need)))
-    logp, entropy = torch.empty(rows, device=dev), torch.empty(rows, device=dev)
-    stats = torch.empty(rows, 2, device=dev)
-    top_logp, top_ids = torch.empty(rows, top, device=dev), torch.empty(rows, top, device=dev, dtype=torch.int64)
-    ws = _scratch(need.value, dev)
-    _check(L.imp_log_probs_forward(DTYPE_IDS[x.dtype], rows, cols, _ld(x), _ptr(x), _ptr(bin_score), _ptr(targets), top, _ptr(logp), _ptr(entropy), _ptr(stats),
-                                   _ptr(top_logp) if top else None, _ptr(top_ids) if top else None, _ptr(ws), need, *_where(x)))
-    return logp, entropy, stats, top_logp, top_ids
+    _check(_lib.lib().imp_log_probs_workspace(rows, cols, top, backward, C.byref(need)))
+    return need.value
 
 
 def _ld(x):
     return x.shape[1] if x.shape[0] == 1 else x.stride(0)
+
+
+def _logp_forward(x, targets, bin_score, top):
+    rows, cols = x.shape
+    dev = x.device
+    need = _logp_scratch(rows, cols, top, 0)
+    logp, entropy = torch.empty(rows, device=dev, dtype=torch.float32), torch.empty(rows, device=dev, dtype=torch.float32)
+    stats = torch.empty((rows, 2), device=dev, dtype=torch.float32)
+    top_logp, top_ids = torch.empty((rows, top), device=dev, dtype=torch.float32), torch.empty((rows, top), device=dev, dtype=torch.int64)
+    ws = _scratch(need, dev)
+    _check(_lib.lib().imp_log_probs_forward(DTYPE_IDS[x.dtype], rows, cols, _ld(x), x.data_ptr(), _at(bin_score), targets.data_ptr(), top, logp.data_ptr(),
+                                            entropy.data_ptr(), stats.data_ptr(), top_logp.data_ptr() if top else None, top_ids.data_ptr() if top else None, _at(ws),
+                                            need, *_where(x)))
+    return logp, entropy, stats, top_logp, top_ids
 
 
 class _LogProbs(torch.autograd.Function):
@@ -272,19 +311,17 @@ class _LogProbs(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dlogp, dentropy, _, __):
         x, bin_score, targets, entropy, stats = ctx.saved_tensors
-        if dlogp is None and dentropy is None:
+        want_x, want_bin = ctx.needs_input_grad[0], bin_score is not None and ctx.needs_input_grad[1]
+        if (dlogp is None and dentropy is None) or not (want_x or want_bin):
             return None, None, None, None
-        L = _lib.lib()
         rows, cols = x.shape
-        dlogp, dentropy = (None if t is None else t.float().contiguous() for t in (dlogp, dentropy))
-        dx = torch.empty(rows, cols, device=x.device, dtype=x.dtype) if ctx.needs_input_grad[0] else None
-        dbin = torch.empty_like(bin_score) if bin_score is not None and ctx.needs_input_grad[1] else None
-        need = C.c_uint64()
-        _check(L.imp_log_probs_workspace(rows, cols, 0, 1, C.byref(need)))
-        ws = _scratch(need.value, x.device) if dbin is not None else None
-        if dx is not None or dbin is not None:
-            _check(L.imp_log_probs_backward(DTYPE_IDS[x.dtype], rows, cols, _ld(x), _ptr(x), _ptr(bin_score), _ptr(targets), _ptr(entropy), _ptr(stats), _ptr(dlogp),
-                                            _ptr(dentropy), _ptr(dx), _ptr(dbin), _ptr(ws), need if ws is not None else 0, *_where(x)))
+        dlogp, dentropy = (None if t is None else _dense(t, torch.float32) for t in (dlogp, dentropy))
+        dx = torch.empty((rows, cols), device=x.device, dtype=x.dtype) if want_x else None
+        dbin = torch.empty_like(bin_score) if want_bin else None
+        need = _logp_scratch(rows, cols, 0, 1) if want_bin else 0
+        ws = _scratch(need, x.device)
+        _check(_lib.lib().imp_log_probs_backward(DTYPE_IDS[x.dtype], rows, cols, _ld(x), x.data_ptr(), _at(bin_score), targets.data_ptr(), entropy.data_ptr(),
+                                                 stats.data_ptr(), _at(dlogp), _at(dentropy), _at(dx), _at(dbin), _at(ws), need, *_where(x)))
         return dx, dbin, None, None
 
 
