@@ -16,9 +16,13 @@
 // r = q G + g of one problem, so dK / dV sum over them in registers and one query of many heads still fills a tile.
 // Few rows: the walk is cut in shares (partials in the caller's workspace, joined in a fixed order by a second launch).
 //
-// Arithmetic: bf16 inputs one bf16 MFMA per product, P and dS rounded to bf16 (half a step of 2^-8, the inputs' own precision); fp16 forward one f16 MFMA; fp16
-// backward two bf16 planes per operand (hi + lo: all 11 bits, and dS far below the fp16 range keeps them) and three products; fp32 three bf16 planes
-// (24 bits, the full fp32 exponent range: no operand limit) and six products - what is dropped is below 2^-26.  Accumulators, softmax statistics and D fp32.
+// Arithmetic (accumulators, softmax statistics and D in fp32; what the operands of the products are rounded to):
+//   bf16  one bf16 MFMA per product; P and dS rounded to bf16, half a step of 2^-8: the inputs' own precision
+//   fp16  one f16 MFMA; P carries a factor 2^14 (weights of long rows stay normal numbers) and dS a power of two per owned row, raised or lowered as the walk meets larger
+//         values (LaneScale), so that gradients far below the fp16 range keep their bits
+//   fp32, many rows: split halves as in the inference kernels (x = hi + lo in f16, 22 bits, three MFMAs), each tensor scaled per key head by a power of two that a first
+//         small launch takes from its largest finite value - no operand limit, and what is small against the head's largest value keeps 2^-39 of that
+//   fp32, few rows: three bf16 planes (24 bits, the whole fp32 range) and six MFMAs - twice the matrix work where it does not bound, without the extra launch
 #include "../../include/imp_hip.h"
 #include "imp_kernels.h"
 
@@ -35,6 +39,7 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int OWN = 128;                 // owned rows per workgroup
+constexpr int SPLIT_ROWS = 256;          // fp32: rows and keys from which the split halves' extra launch pays
 
 struct AttnOp {
     const void *q, *k, *v, *out, *dout;  // out: read by the backward
@@ -46,6 +51,8 @@ struct AttnOp {
     int B, nq, nk, H, Hkv, G, dh;
     float scale;
     int shares;
+    float* amax;                         // [4][B * Hkv][chunks]: largest finite |q|, |k|, |v|, |dout| of a part of the rows (fp32 split halves)
+    int chunks;
 };
 
 template <typename E> struct Vec8;
@@ -54,6 +61,19 @@ template <> struct Vec8<_Float16> { using type = f16x8; };
 
 __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// operand type, planes, tensors scaled per head, dS scaled per owned row, log2 of the factor P carries, rows per tile of the walk
+template <typename T_, typename E_, int NP_, bool SCALED_, bool LANE_, int SHIFT_, int R_> struct Arith {
+    using T = T_;
+    using E = E_;
+    using V = typename Vec8<E_>::type;
+    static constexpr int NP = NP_, SHIFT = SHIFT_, R = R_;
+    static constexpr bool SCALED = SCALED_, LANE = LANE_;
+};
+using ArithBf16 = Arith<__bf16, __bf16, 1, false, false, 0, 64>;
+using ArithF16 = Arith<_Float16, _Float16, 1, false, true, 14, 64>;
+using ArithSplit = Arith<float, _Float16, 2, true, true, 14, 32>;
+using ArithPlanes = Arith<float, __bf16, 3, false, false, 0, 32>;
 
 // c += a b over the planes, the small products first
 template <int NP, typename V>
@@ -121,12 +141,16 @@ template <> struct Chunk<__bf16> : Chunk16<__bf16> {};
 template <> struct Chunk<_Float16> : Chunk16<_Float16> {};
 
 template <typename T, int NP, typename E>
-__device__ __forceinline__ void to_planes(const Chunk<T>& c, typename Vec8<E>::type (&p)[NP]) {
+__device__ __forceinline__ void to_planes(const Chunk<T>& c, float factor, typename Vec8<E>::type (&p)[NP]) {
     if constexpr (NP == 1 && sizeof(T) == 2) {
         p[0] = __builtin_bit_cast(typename Vec8<E>::type, c.a);
     } else {
         float x[8];
         c.get(x);
+        if constexpr (NP == 2) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] *= factor;
+        }
         split8<NP, E>(x, p);
     }
 }
@@ -156,8 +180,6 @@ __device__ __forceinline__ int64_t stat_row(const AttnOp& p, int b, int hk, int 
     return ((int64_t)b * p.H + hk * p.G + g) * p.nq + q;
 }
 
-template <typename E> using lds_tile_t = E*;
-
 // A operand of the first product: row = lane % 32 of the 32-row sub-tile, 8 columns of k-step s
 template <typename E, int NP, int LD, int PLANE>
 __device__ __forceinline__ void read_rows(const E* tile, int sub, int s, int lane, typename Vec8<E>::type (&f)[NP]) {
@@ -180,14 +202,14 @@ __device__ __forceinline__ void read_cols(const E* tile, int sub, int s, int dt,
 
 // the owned row of this lane as B-operand fragments (zeros when the row is dead or past the head's channels)
 template <typename T, typename E, int NP, int DHP>
-__device__ __forceinline__ void load_owned(const T* row, bool live, int dh, int half, typename Vec8<E>::type (&f)[DHP / 16][NP]) {
+__device__ __forceinline__ void load_owned(const T* row, bool live, int dh, int half, float factor, typename Vec8<E>::type (&f)[DHP / 16][NP]) {
 #pragma unroll
     for (int s = 0; s < DHP / 16; ++s) {
         Chunk<T> c;
         const int col = 16 * s + 8 * half;
         if (live && col < dh) c.load(row + col);
         else c.zero();
-        to_planes<T, NP, E>(c, f[s]);
+        to_planes<T, NP, E>(c, factor, f[s]);
     }
 }
 
@@ -210,16 +232,16 @@ struct Stage {
             }
         }
     }
-    __device__ void store(int tid, E* X, E* Y) const {
+    __device__ void store(int tid, E* X, E* Y, float fx, float fy) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = tid + 256 * i, row = c / CPR, col = (c % CPR) * 8;
             if (R * CPR % 256 == 0 || row < R) {
                 typename Vec8<E>::type p[NP];
-                to_planes<T, NP, E>(x[i], p);
+                to_planes<T, NP, E>(x[i], fx, p);
 #pragma unroll
                 for (int j = 0; j < NP; ++j) *(typename Vec8<E>::type*)(X + j * PLANE + row * LD + col) = p[j];
-                to_planes<T, NP, E>(y[i], p);
+                to_planes<T, NP, E>(y[i], fy, p);
 #pragma unroll
                 for (int j = 0; j < NP; ++j) *(typename Vec8<E>::type*)(Y + j * PLANE + row * LD + col) = p[j];
             }
@@ -243,10 +265,76 @@ __device__ __forceinline__ void pack(const f32x16& v, int s, typename Vec8<E>::t
     split8<NP, E>(x, p);
 }
 
+__device__ __forceinline__ int clamp_exp(int e) { return min(max(e, -120), 120); }
+// the power of two that brings the largest of a tensor's values (of this key head) to [2^13, 2^14)
+__device__ __forceinline__ float head_factor(const AttnOp& p, int tensor, int head, int lane) {
+    const float* a = p.amax + ((int64_t)tensor * p.B * p.Hkv + head) * p.chunks;
+    float m = lane < p.chunks ? a[lane] : 0.f;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    return m == 0.f ? 1.f : __builtin_ldexpf(1.f, clamp_exp(14 - __builtin_amdgcn_frexp_expf(m)));
+}
+__device__ __forceinline__ float other_half_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
+
+// the power of two dS of an owned row is multiplied by before it is rounded: its largest value so far is kept below 2^15
+struct LaneScale {
+    float f = 0.f;                       // 0: nothing but zeros so far
+    // the factor for 16 more values; acc: the sums in the present unit
+    template <int DT> __device__ void step(const f32x16& v, f32x16 (&acc)[DT]) {
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[i]));
+        m = other_half_max(m);
+        const bool grow = m * f > 32768.f || (f == 0.f && m > 0.f);
+        if (__ballot(grow)) {
+            const float nf = grow ? __builtin_ldexpf(1.f, clamp_exp(10 - __builtin_amdgcn_frexp_expf(m))) : f;
+            const float ratio = f == 0.f || nf == f ? 1.f : nf / f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[d] *= ratio;
+            f = nf;
+        }
+    }
+    __device__ float inverse() const { return f == 0.f ? 0.f : 1.f / f; }
+};
+
+// largest finite |value| of a part of the rows that exist, per key head; blockIdx.z: 0 q, 1 k, 2 v, 3 dout
+__global__ __launch_bounds__(256) void attn_amax_kernel(AttnOp p) {
+    __shared__ float sm[4];
+    const int head = blockIdx.y, b = head / p.Hkv, hk = head % p.Hkv, which = blockIdx.z, per = p.dh / 8;
+    const bool keys = which == 1 || which == 2;
+    const int rows = keys ? clamp_len(p.k_lens, b, p.nk) : clamp_len(p.q_lens, b, p.nq) * p.G;
+    const int r0 = (int)((int64_t)rows * blockIdx.x / p.chunks), r1 = (int)((int64_t)rows * (blockIdx.x + 1) / p.chunks);
+    const uint8_t* mask = keys && p.mask ? p.mask + (int64_t)b * p.nk : nullptr;
+    float m = 0.f;
+    const int group = 256 / per, tr = threadIdx.x / per, col = (threadIdx.x % per) * 8;
+    if (tr < group)
+        for (int r = r0 + tr; r < r1; r += group) {
+            if (mask && !mask[r]) continue;
+            const float* row = which == 0 ? (const float*)p.q + q_row(p, p.qs, b, hk, r)
+                             : which == 1 ? (const float*)p.k + b * p.ks[0] + r * p.ks[1] + hk * p.ks[2]
+                             : which == 2 ? (const float*)p.v + b * p.vs[0] + r * p.vs[1] + hk * p.vs[2]
+                                          : (const float*)p.dout + dense_row(p, b, hk, r) * p.dh;
+            Chunk<float> c;
+            c.load(row + col);
+            float x[8];
+            c.get(x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { const float v = fabsf(x[i]); m = fmaxf(m, v < INFINITY ? v : 0.f); }
+        }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) p.amax[((int64_t)which * p.B * p.Hkv + head) * p.chunks + blockIdx.x] = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+}
+
 // ---------------------------------------------------------------------------------------------------------------------- forward
-template <typename T, typename E, int NP, int DHP, int R>
+template <typename A, int DHP>
 __global__ __launch_bounds__(256, 1) void attn_fwd_kernel(AttnOp p) {
-    using V = typename Vec8<E>::type;
+    using T = typename A::T;
+    using E = typename A::E;
+    using V = typename A::V;
+    constexpr int NP = A::NP, R = A::R;
     using St = Stage<T, E, NP, DHP, R>;
     constexpr int LD = St::LD, PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32;
     __shared__ __attribute__((aligned(16))) E Ks[NP * PLANE], Vs[NP * PLANE];
@@ -260,12 +348,14 @@ __global__ __launch_bounds__(256, 1) void attn_fwd_kernel(AttnOp p) {
     int t0 = 0, t1 = own0 < live_rows ? tiles : 0;
     if (p.shares > 1 && t1) { t0 = (int)((int64_t)tiles * share / p.shares); t1 = (int)((int64_t)tiles * (share + 1) / p.shares); }
 
+    float fq = 1.f, fk = 1.f, fv = 1.f;
+    if constexpr (A::SCALED) { fq = head_factor(p, 0, blockIdx.y, lane); fk = head_factor(p, 1, blockIdx.y, lane); fv = head_factor(p, 2, blockIdx.y, lane); }
     V qf[KS][NP];
-    load_owned<T, E, NP, DHP>((const T*)p.q + (live ? q_row(p, p.qs, b, hk, r) : 0), live, p.dh, half, qf);
+    load_owned<T, E, NP, DHP>((const T*)p.q + (live ? q_row(p, p.qs, b, hk, r) : 0), live, p.dh, half, fq, qf);
     const T* kbase = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
     const T* vbase = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
     const uint8_t* mask = p.mask ? p.mask + (int64_t)b * p.nk : nullptr;
-    const float c = p.scale * LOG2E;
+    const float c = p.scale * LOG2E * ((1.f / fq) * (1.f / fk));
 
     f32x16 o[DT];
 #pragma unroll
@@ -284,7 +374,7 @@ __global__ __launch_bounds__(256, 1) void attn_fwd_kernel(AttnOp p) {
     if (t0 < t1) fetch(t0);
     for (int t = t0; t < t1; ++t) {
         __syncthreads();
-        st.store(tid, Ks, Vs);
+        st.store(tid, Ks, Vs, fk, fv);
         if (tid < R) { const int key = t * R + tid; kb[tid] = key < klen && (!mask || mask[key]) ? 0.f : -INFINITY; }
         __syncthreads();
         if (t + 1 < t1) fetch(t + 1);
@@ -311,8 +401,8 @@ __global__ __launch_bounds__(256, 1) void attn_fwd_kernel(AttnOp p) {
                 }
             }
         }
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - mu);
+        mx = other_half_max(mx);
+        const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - mu), ref = mu - A::SHIFT;
         m = mn;
         if (__ballot(alpha != 1.f)) {
             l *= alpha;
@@ -323,7 +413,7 @@ __global__ __launch_bounds__(256, 1) void attn_fwd_kernel(AttnOp p) {
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[n][i] = __builtin_amdgcn_exp2f(s[n][i] - mu);
+                s[n][i] = __builtin_amdgcn_exp2f(s[n][i] - ref);
                 l += s[n][i];
             }
 #pragma unroll
@@ -346,7 +436,7 @@ __global__ __launch_bounds__(256, 1) void attn_fwd_kernel(AttnOp p) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] = zero16();
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l, lse = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+    const float inv = l == 0.f ? 0.f : 1.f / l * (1.f / fv), lse = l == 0.f ? -INFINITY : (m + (__builtin_amdgcn_logf(l) - A::SHIFT)) * LN2;
     const int64_t row = dense_row(p, b, hk, r), rows = (int64_t)p.B * p.nq * p.H;
     if (p.shares > 1) {
         float* out = p.part + (share * rows + row) * p.dh;
@@ -431,9 +521,12 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(AttnOp p) {
 // the exponent reference of a row: lse in log2 units, +inf (P = 0) for rows that do not exist or have no key
 __device__ __forceinline__ float row_ref(float lse) { return lse == -INFINITY ? INFINITY : lse * LOG2E; }
 
-template <typename T, typename E, int NP, int DHP, int R>
+template <typename A, int DHP>
 __global__ __launch_bounds__(256, 1) void attn_dq_kernel(AttnOp p) {
-    using V = typename Vec8<E>::type;
+    using T = typename A::T;
+    using E = typename A::E;
+    using V = typename A::V;
+    constexpr int NP = A::NP, R = A::R;
     using St = Stage<T, E, NP, DHP, R>;
     constexpr int LD = St::LD, PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32;
     __shared__ __attribute__((aligned(16))) E Ks[NP * PLANE], Vs[NP * PLANE];
@@ -454,13 +547,18 @@ __global__ __launch_bounds__(256, 1) void attn_dq_kernel(AttnOp p) {
     }
     const bool live = ref != INFINITY;
     if (!live) delta = 0.f;
+    float fq = 1.f, fk = 1.f, fv = 1.f, fo = 1.f;
+    if constexpr (A::SCALED) {
+        fq = head_factor(p, 0, blockIdx.y, lane); fk = head_factor(p, 1, blockIdx.y, lane); fv = head_factor(p, 2, blockIdx.y, lane); fo = head_factor(p, 3, blockIdx.y, lane);
+    }
     V qf[KS][NP], of[KS][NP];
-    load_owned<T, E, NP, DHP>((const T*)p.q + (live ? q_row(p, p.qs, b, hk, r) : 0), live, p.dh, half, qf);
-    load_owned<T, E, NP, DHP>((const T*)p.dout + (live ? dense_row(p, b, hk, r) * p.dh : 0), live, p.dh, half, of);
+    load_owned<T, E, NP, DHP>((const T*)p.q + (live ? q_row(p, p.qs, b, hk, r) : 0), live, p.dh, half, fq, qf);
+    load_owned<T, E, NP, DHP>((const T*)p.dout + (live ? dense_row(p, b, hk, r) * p.dh : 0), live, p.dh, half, fo, of);
     const T* kbase = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
     const T* vbase = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
     const uint8_t* mask = p.mask ? p.mask + (int64_t)b * p.nk : nullptr;
-    const float c = p.scale * LOG2E;
+    const float c = p.scale * LOG2E * ((1.f / fq) * (1.f / fk)), cd = (1.f / fo) * (1.f / fv);
+    LaneScale ls;
     f32x16 dq[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) dq[d] = zero16();
@@ -477,7 +575,7 @@ __global__ __launch_bounds__(256, 1) void attn_dq_kernel(AttnOp p) {
     if (t0 < t1) fetch(t0);
     for (int t = t0; t < t1; ++t) {
         __syncthreads();
-        st.store(tid, Ks, Vs);
+        st.store(tid, Ks, Vs, fk, fv);
         if (tid < R) { const int key = t * R + tid; kb[tid] = key < klen && (!mask || mask[key]) ? 0.f : -INFINITY; }
         __syncthreads();
         if (t + 1 < t1) fetch(t + 1);
@@ -499,8 +597,12 @@ __global__ __launch_bounds__(256, 1) void attn_dq_kernel(AttnOp p) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], c, -ref) + bias[i]);
-                    s[4 * g + i] = pr * (dp[4 * g + i] - delta);
+                    s[4 * g + i] = pr * __builtin_fmaf(dp[4 * g + i], cd, -delta);
                 }
+            }
+            if constexpr (A::LANE) {
+                ls.step(s, dq);
+                s *= ls.f;
             }
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -521,22 +623,26 @@ __global__ __launch_bounds__(256, 1) void attn_dq_kernel(AttnOp p) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) dq[d] = zero16();
     }
+    const float unit = p.scale * (1.f / fk) * (A::LANE ? ls.inverse() : 1.f);
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int col = 32 * d + 8 * g + 4 * half;
             if (col < p.dh) {
-                const float x0 = dq[d][4 * g] * p.scale, x1 = dq[d][4 * g + 1] * p.scale, x2 = dq[d][4 * g + 2] * p.scale, x3 = dq[d][4 * g + 3] * p.scale;
+                const float x0 = dq[d][4 * g] * unit, x1 = dq[d][4 * g + 1] * unit, x2 = dq[d][4 * g + 2] * unit, x3 = dq[d][4 * g + 3] * unit;
                 if (p.shares > 1) store4(p.part + (share * rows + row) * p.dh + col, x0, x1, x2, x3);
                 else store4((T*)p.dq + row * p.dh + col, x0, x1, x2, x3);
             }
         }
 }
 
-template <typename T, typename E, int NP, int DHP, int R>
+template <typename A, int DHP>
 __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnOp p) {
-    using V = typename Vec8<E>::type;
+    using T = typename A::T;
+    using E = typename A::E;
+    using V = typename A::V;
+    constexpr int NP = A::NP, R = A::R;
     using St = Stage<T, E, NP, DHP, R>;
     constexpr int LD = St::LD, PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32;
     __shared__ __attribute__((aligned(16))) E Qs[NP * PLANE], Os[NP * PLANE];
@@ -550,10 +656,15 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnOp p) {
     int t0 = 0, t1 = own0 < klen ? tiles : 0;
     if (p.shares > 1 && t1) { t0 = (int)((int64_t)tiles * share / p.shares); t1 = (int)((int64_t)tiles * (share + 1) / p.shares); }
 
+    float fq = 1.f, fk = 1.f, fv = 1.f, fo = 1.f;
+    if constexpr (A::SCALED) {
+        fq = head_factor(p, 0, blockIdx.y, lane); fk = head_factor(p, 1, blockIdx.y, lane); fv = head_factor(p, 2, blockIdx.y, lane); fo = head_factor(p, 3, blockIdx.y, lane);
+    }
     V kf[KS][NP], vf[KS][NP];
-    load_owned<T, E, NP, DHP>((const T*)p.k + (live ? b * p.ks[0] + key * p.ks[1] + hk * p.ks[2] : 0), live, p.dh, half, kf);
-    load_owned<T, E, NP, DHP>((const T*)p.v + (live ? b * p.vs[0] + key * p.vs[1] + hk * p.vs[2] : 0), live, p.dh, half, vf);
-    const float c = p.scale * LOG2E, off = live ? 0.f : -INFINITY;
+    load_owned<T, E, NP, DHP>((const T*)p.k + (live ? b * p.ks[0] + key * p.ks[1] + hk * p.ks[2] : 0), live, p.dh, half, fk, kf);
+    load_owned<T, E, NP, DHP>((const T*)p.v + (live ? b * p.vs[0] + key * p.vs[1] + hk * p.vs[2] : 0), live, p.dh, half, fv, vf);
+    const float c = p.scale * LOG2E * ((1.f / fq) * (1.f / fk)), cd = (1.f / fo) * (1.f / fv), off = live ? (float)A::SHIFT : -INFINITY;
+    LaneScale ls;
     f32x16 dk[DT], dv[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
@@ -571,7 +682,7 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnOp p) {
     if (t0 < t1) fetch(t0);
     for (int t = t0; t < t1; ++t) {
         __syncthreads();
-        st.store(tid, Qs, Os);
+        st.store(tid, Qs, Os, fq, fo);
         if (tid < R) {
             const int r = t * R + tid;
             float ref = INFINITY, dl = 0.f;
@@ -605,8 +716,12 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnOp p) {
                 for (int i = 0; i < 4; ++i) {
                     const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], c, -ref[i]) + off);
                     s[4 * g + i] = pr;
-                    dp[4 * g + i] = pr * (dp[4 * g + i] - dl[i]);
+                    dp[4 * g + i] = pr * __builtin_fmaf(dp[4 * g + i], cd, -dl[i]);
                 }
+            }
+            if constexpr (A::LANE) {
+                ls.step(dp, dk);
+                dp *= ls.f;
             }
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -625,6 +740,7 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnOp p) {
         }
     }
     if (key >= p.nk) return;
+    const float unp = A::SHIFT ? 1.f / (float)(1 << A::SHIFT) : 1.f, unit = p.scale * (1.f / fq) * unp * (A::LANE ? ls.inverse() : 1.f), vunit = (1.f / fo) * unp;
     const int64_t row = ((int64_t)b * p.nk + key) * p.Hkv + hk, rows = (int64_t)p.B * p.nk * p.Hkv;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -632,8 +748,8 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnOp p) {
         for (int g = 0; g < 4; ++g) {
             const int col = 32 * d + 8 * g + 4 * half;
             if (col < p.dh) {
-                const float x0 = dk[d][4 * g] * p.scale, x1 = dk[d][4 * g + 1] * p.scale, x2 = dk[d][4 * g + 2] * p.scale, x3 = dk[d][4 * g + 3] * p.scale;
-                const float y0 = dv[d][4 * g], y1 = dv[d][4 * g + 1], y2 = dv[d][4 * g + 2], y3 = dv[d][4 * g + 3];
+                const float x0 = dk[d][4 * g] * unit, x1 = dk[d][4 * g + 1] * unit, x2 = dk[d][4 * g + 2] * unit, x3 = dk[d][4 * g + 3] * unit;
+                const float y0 = dv[d][4 * g] * vunit, y1 = dv[d][4 * g + 1] * vunit, y2 = dv[d][4 * g + 2] * vunit, y3 = dv[d][4 * g + 3] * vunit;
                 if (p.shares > 1) {
                     store4(p.part + (2 * share * rows + row) * p.dh + col, x0, x1, x2, x3);
                     store4(p.part + ((2 * share + 1) * rows + row) * p.dh + col, y0, y1, y2, y3);
@@ -663,7 +779,7 @@ int shares_for(int64_t blocks, int64_t walked) {
     return s < 1 ? 1 : (s > 64 ? 64 : (int)s);
 }
 
-struct Plan { int fwd, dq, dkv; int64_t q_rows, k_rows; size_t fwd_bytes, bwd_bytes; };
+struct Plan { int fwd, dq, dkv, chunks; bool split; int64_t q_rows, k_rows; size_t amax_bytes, fwd_bytes, bwd_bytes; };
 Plan plan(const imp_attn_desc& d) {
     Plan p;
     const int64_t heads = (int64_t)d.batch * d.kv_heads, rows = (int64_t)d.nq * (d.heads / d.kv_heads);
@@ -673,9 +789,13 @@ Plan plan(const imp_attn_desc& d) {
     p.dkv = shares_for(kbk, rows);
     p.q_rows = (int64_t)d.batch * d.nq * d.heads;
     p.k_rows = (int64_t)d.batch * d.nk * d.kv_heads;
-    p.fwd_bytes = p.fwd > 1 ? (size_t)p.fwd * p.q_rows * (d.head_dim + 1) * 4 : 0;
+    p.split = d.dtype == IMP_DTYPE_F32 && rows >= SPLIT_ROWS && d.nk >= SPLIT_ROWS;
+    const int64_t c = 256 / heads;
+    p.chunks = (int)(c < 4 ? 4 : c > 64 ? 64 : c);
+    p.amax_bytes = p.split ? (size_t)4 * heads * p.chunks * 4 : 0;
+    p.fwd_bytes = p.amax_bytes + (p.fwd > 1 ? (size_t)p.fwd * p.q_rows * (d.head_dim + 1) * 4 : 0);
     const size_t a = p.dq > 1 ? (size_t)p.dq * p.q_rows * d.head_dim * 4 : 0, b = p.dkv > 1 ? (size_t)p.dkv * 2 * p.k_rows * d.head_dim * 4 : 0;
-    p.bwd_bytes = ((size_t)p.q_rows * 4 + 15) / 16 * 16 + (a > b ? a : b);
+    p.bwd_bytes = p.amax_bytes + ((size_t)p.q_rows * 4 + 15) / 16 * 16 + (a > b ? a : b);
     return p;
 }
 
@@ -709,25 +829,23 @@ AttnOp op_of(const imp_attn_desc& d) {
 }
 
 // which: 0 forward, 1 dQ, 2 dK / dV
-template <typename T, typename E, int NP, int DHP, int R>
-void launch(int which, const AttnOp& p, hipStream_t st) {
+template <typename A, int DHP> void launch(int which, const AttnOp& p, hipStream_t st) {
     const int64_t own = which == 2 ? p.nk : (int64_t)p.nq * p.G;
     const dim3 grid((unsigned)((own + OWN - 1) / OWN), (unsigned)(p.B * p.Hkv), (unsigned)p.shares);
-    if (which == 0) attn_fwd_kernel<T, E, NP, DHP, R><<<grid, 256, 0, st>>>(p);
-    else if (which == 1) attn_dq_kernel<T, E, NP, DHP, R><<<grid, 256, 0, st>>>(p);
-    else attn_dkv_kernel<T, E, NP, DHP, R><<<grid, 256, 0, st>>>(p);
+    if (which == 0) attn_fwd_kernel<A, DHP><<<grid, 256, 0, st>>>(p);
+    else if (which == 1) attn_dq_kernel<A, DHP><<<grid, 256, 0, st>>>(p);
+    else attn_dkv_kernel<A, DHP><<<grid, 256, 0, st>>>(p);
 }
-template <typename T, typename E, int NP, int R>
-void launch_dh(int which, const AttnOp& p, hipStream_t st) {
-    if (p.dh <= 32) launch<T, E, NP, 32, R>(which, p, st);
-    else if (p.dh <= 64) launch<T, E, NP, 64, R>(which, p, st);
-    else launch<T, E, NP, 128, R>(which, p, st);
+template <typename A> void launch_dh(int which, const AttnOp& p, hipStream_t st) {
+    if (p.dh <= 32) launch<A, 32>(which, p, st);
+    else if (p.dh <= 64) launch<A, 64>(which, p, st);
+    else launch<A, 128>(which, p, st);
 }
-void launch_any(int dtype, int which, const AttnOp& p, hipStream_t st) {
-    if (dtype == IMP_DTYPE_F32) launch_dh<float, __bf16, 3, 32>(which, p, st);
-    else if (dtype == IMP_DTYPE_BF16) launch_dh<__bf16, __bf16, 1, 64>(which, p, st);
-    else if (which == 0) launch_dh<_Float16, _Float16, 1, 64>(which, p, st);
-    else launch_dh<_Float16, __bf16, 2, 32>(which, p, st);
+void launch_any(int dtype, bool split, int which, const AttnOp& p, hipStream_t st) {
+    if (dtype == IMP_DTYPE_BF16) launch_dh<ArithBf16>(which, p, st);
+    else if (dtype == IMP_DTYPE_F16) launch_dh<ArithF16>(which, p, st);
+    else if (split) launch_dh<ArithSplit>(which, p, st);
+    else launch_dh<ArithPlanes>(which, p, st);
 }
 
 int on_device(int device) {
@@ -764,10 +882,13 @@ int imp_attn_forward(const imp_attn_desc* d, const void* q, const void* k, const
     AttnOp p = op_of(*d);
     p.q = q; p.k = k; p.v = v; p.o = out; p.lse = lse;
     p.shares = pl.fwd;
-    p.part = (float*)workspace;
+    p.amax = (float*)workspace;
+    p.chunks = pl.chunks;
+    p.part = (float*)((char*)workspace + pl.amax_bytes);
     p.part_lse = p.part + (int64_t)pl.fwd * pl.q_rows * d->head_dim;
     const hipStream_t st = (hipStream_t)stream;
-    launch_any(d->dtype, 0, p, st);
+    if (pl.split) attn_amax_kernel<<<dim3(pl.chunks, d->batch * d->kv_heads, 3), 256, 0, st>>>(p);
+    launch_any(d->dtype, pl.split, 0, p, st);
     if (pl.fwd > 1) {
         const unsigned grid = (unsigned)((pl.q_rows + 3) / 4);
         if (d->dtype == IMP_DTYPE_F32) attn_join_kernel<float><<<grid, 256, 0, st>>>(p);
@@ -787,8 +908,10 @@ int imp_attn_backward(const imp_attn_desc* d, const void* q, const void* k, cons
     if (int rc = on_device(device)) return rc;
     AttnOp p = op_of(*d);
     p.q = q; p.k = k; p.v = v; p.out = out; p.lse = const_cast<float*>(lse); p.dout = dout; p.dq = dq; p.dk = dk; p.dv = dv;
-    p.delta = (float*)workspace;
-    p.part = (float*)((char*)workspace + ((size_t)pl.q_rows * 4 + 15) / 16 * 16);
+    p.amax = (float*)workspace;
+    p.chunks = pl.chunks;
+    p.delta = (float*)((char*)workspace + pl.amax_bytes);
+    p.part = (float*)((char*)p.delta + ((size_t)pl.q_rows * 4 + 15) / 16 * 16);
     const hipStream_t st = (hipStream_t)stream;
     const int dt = d->dtype;
     auto each = [&](auto f) {
@@ -796,6 +919,7 @@ int imp_attn_backward(const imp_attn_desc* d, const void* q, const void* k, cons
         else if (dt == IMP_DTYPE_BF16) f((__bf16*)nullptr);
         else f((_Float16*)nullptr);
     };
+    if (pl.split) attn_amax_kernel<<<dim3(pl.chunks, d->batch * d->kv_heads, 4), 256, 0, st>>>(p);
     each([&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         attn_delta_kernel<T><<<(unsigned)((pl.q_rows + 15) / 16), 256, 0, st>>>(p);
@@ -809,12 +933,12 @@ int imp_attn_backward(const imp_attn_desc* d, const void* q, const void* k, cons
     };
     if (dk) {
         p.shares = pl.dkv;
-        launch_any(dt, 2, p, st);
+        launch_any(dt, pl.split, 2, p, st);
         if (p.shares > 1) { join(pl.k_rows, 2, 0, dk); join(pl.k_rows, 2, 1, dv); }
     }
     if (dq) {
         p.shares = pl.dq;
-        launch_any(dt, 1, p, st);
+        launch_any(dt, pl.split, 1, p, st);
         if (p.shares > 1) join(pl.q_rows, 1, 0, dq);
     }
     return launched("imp_attn_backward");
