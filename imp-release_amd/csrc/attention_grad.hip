@@ -18,7 +18,7 @@
 //
 // Arithmetic (accumulators, softmax statistics and D in fp32; what the operands of the products are rounded to):
 //   bf16  one bf16 MFMA per product; P and dS rounded to bf16, half a step of 2^-8: the inputs' own precision
-//   fp16  one f16 MFMA; P carries a factor 2^14 (weights of long rows stay normal numbers) and dS a power of two per owned row, raised or lowered as the walk meets larger
+//   fp16  one f16 MFMA; P carries a factor 2^10 (weights of long rows stay normal numbers) and dS a power of two per owned row, raised or lowered as the walk meets larger
 //         values (LaneScale), so that gradients far below the fp16 range keep their bits
 //   fp32, many rows: split halves as in the inference kernels (x = hi + lo in f16, 22 bits, three MFMAs), each tensor scaled per key head by a power of two that a first
 //         small launch takes from its largest finite value - no operand limit, and what is small against the head's largest value keeps 2^-39 of that
@@ -71,8 +71,9 @@ template <typename T_, typename E_, int NP_, bool SCALED_, bool LANE_, int SHIFT
     static constexpr bool SCALED = SCALED_, LANE = LANE_;
 };
 using ArithBf16 = Arith<__bf16, __bf16, 1, false, false, 0, 64>;
-using ArithF16 = Arith<_Float16, _Float16, 1, false, true, 14, 64>;
-using ArithSplit = Arith<float, _Float16, 2, true, true, 14, 32>;
+using ArithF16 = Arith<_Float16, _Float16, 1, false, true, 10, 64>;
+using ArithSplit = Arith<float, _Float16, 2, true, true, 10, 32>;
+constexpr float LAZY = 5.f;              // the softmax reference of a row follows its maximum when that is 2^LAZY above it: P stays below 2^(SHIFT + LAZY)
 using ArithPlanes = Arith<float, __bf16, 3, false, false, 0, 32>;
 
 // c += a b over the planes, the small products first
@@ -90,24 +91,21 @@ __device__ __forceinline__ f32x16 mfma_planes(const V (&a)[NP], const V (&b)[NP]
     return mfma(a[0], b[0], c);
 }
 
-// the same with the small products in an accumulator of their own (added once at the end): a sum over the channels is then rounded once per k-step at its
-// full size, not once per product - what dS = P (dP - D) keeps after the cancellation is decided here
-template <int NP, typename V>
-__device__ __forceinline__ void mfma_apart(const V (&a)[NP], const V (&b)[NP], f32x16& c, f32x16& small) {
-    if constexpr (NP == 3) {
-        small = mfma(a[1], b[1], small);
-        small = mfma(a[0], b[2], small);
-        small = mfma(a[2], b[0], small);
-    }
-    if constexpr (NP >= 2) {
-        small = mfma(a[0], b[1], small);
-        small = mfma(a[1], b[0], small);
-    }
-    c = mfma(a[0], b[0], c);
-}
-
 template <int NP, typename E>
 __device__ __forceinline__ void split8(const float (&x)[8], typename Vec8<E>::type (&p)[NP]) {
+    if constexpr (NP == 2 && __is_same(E, _Float16)) {           // the values come from vector instructions, never straight from a matrix one (imp_split2 is assembly)
+        u32x4 hi, lo;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            unsigned h, l;
+            imp_split2(x[2 * i], x[2 * i + 1], h, l);
+            hi[i] = h;
+            lo[i] = l;
+        }
+        p[0] = __builtin_bit_cast(f16x8, hi);
+        p[1] = __builtin_bit_cast(f16x8, lo);
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         float r = x[i];
@@ -126,12 +124,14 @@ template <> struct Chunk<float> {
     f32x4 a, b;
     __device__ void load(const float* p) { a = *(const f32x4*)p; b = *(const f32x4*)(p + 4); }
     __device__ void zero() { a = f32x4{0, 0, 0, 0}; b = a; }
+    __device__ void negate() { a = -a; b = -b; }
     __device__ void get(float (&x)[8]) const { for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[i + 4] = b[i]; } }
 };
 template <typename T> struct Chunk16 {
     u32x4 a;
     __device__ void load(const T* p) { a = *(const u32x4*)p; }
     __device__ void zero() { a = u32x4{0, 0, 0, 0}; }
+    __device__ void negate() { a ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u}; }
     __device__ void get(float (&x)[8]) const {
         const auto v = __builtin_bit_cast(typename Vec8<T>::type, a);
         for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
@@ -202,13 +202,14 @@ __device__ __forceinline__ void read_cols(const E* tile, int sub, int s, int dt,
 
 // the owned row of this lane as B-operand fragments (zeros when the row is dead or past the head's channels)
 template <typename T, typename E, int NP, int DHP>
-__device__ __forceinline__ void load_owned(const T* row, bool live, int dh, int half, float factor, typename Vec8<E>::type (&f)[DHP / 16][NP]) {
+__device__ __forceinline__ void load_owned(const T* row, bool live, int dh, int half, float factor, typename Vec8<E>::type (&f)[DHP / 16][NP], bool negative = false) {
 #pragma unroll
     for (int s = 0; s < DHP / 16; ++s) {
         Chunk<T> c;
         const int col = 16 * s + 8 * half;
         if (live && col < dh) c.load(row + col);
         else c.zero();
+        if (negative) c.negate();
         to_planes<T, NP, E>(c, factor, f[s]);
     }
 }
@@ -249,11 +250,51 @@ struct Stage {
     }
 };
 
+__device__ __forceinline__ f32x16 zero16();
+// the first product of a 32 x 32 sub-tile: rows of `tile` times the owned rows.  Over all k-steps the small products come first and hi . hi last: the sum is rounded once
+// per k-step at its full size, not once per product - what dS = P (dP - D) keeps after the cancellation is decided here
+template <typename A, int KS, int LD, int PLANE>
+__device__ __forceinline__ f32x16 first_product(const typename A::E* tile, int sub, int lane, const typename A::V (&own)[KS][A::NP]) {
+    using V = typename A::V;
+    f32x16 c = zero16();
+    V hi[KS];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+        V f[A::NP];
+        read_rows<typename A::E, A::NP, LD, PLANE>(tile, sub, k, lane, f);
+        if constexpr (A::NP == 3) {
+            c = mfma(f[1], own[k][1], c);
+            c = mfma(f[0], own[k][2], c);
+            c = mfma(f[2], own[k][0], c);
+        }
+        if constexpr (A::NP >= 2) {
+            c = mfma(f[0], own[k][1], c);
+            c = mfma(f[1], own[k][0], c);
+            hi[k] = f[0];
+        } else c = mfma(f[0], own[k][0], c);
+    }
+    if constexpr (A::NP >= 2) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) c = mfma(hi[k], own[k][0], c);
+    }
+    return c;
+}
+
 __device__ __forceinline__ f32x16 zero16() {
     f32x16 z;
 #pragma unroll
     for (int i = 0; i < 16; ++i) z[i] = 0.f;
     return z;
+}
+
+// adds 0 or -inf per walked row (the rows of a first product's result)
+__device__ __forceinline__ void add_rows(f32x16& s, const float* bias, int half) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const f32x4 v = *(const f32x4*)(bias + 8 * g + 4 * half);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[4 * g + i] += v[i];
+    }
 }
 
 // registers 8 s .. 8 s + 7 of a first product's result as the planes of a B operand
@@ -274,7 +315,15 @@ __device__ __forceinline__ float head_factor(const AttnOp& p, int tensor, int he
     for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
     return m == 0.f ? 1.f : __builtin_ldexpf(1.f, clamp_exp(14 - __builtin_amdgcn_frexp_expf(m)));
 }
-__device__ __forceinline__ float other_half_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
+// the larger of a lane's and the other half's value (v: the result of a vector instruction; the swap may follow one only after two wait states)
+__device__ __forceinline__ float other_half_max(float v) {
+    float w = v;
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(v), "+v"(w));
+    return fmaxf(v, w);
+}
+
+// scores in log2 units: |scale| log2 e in the operands' unit (the sign is the owned operand's; 0 becomes next to nothing, so that -inf stays what it is)
+__device__ __forceinline__ float score_unit(float scale, float fa, float fb) { return fmaxf(fabsf(scale) * LOG2E * ((1.f / fa) * (1.f / fb)), 1e-37f); }
 
 // the power of two dS of an owned row is multiplied by before it is rounded: its largest value so far is kept below 2^15
 struct LaneScale {
@@ -351,11 +400,11 @@ __global__ __launch_bounds__(256, 1) void attn_fwd_kernel(AttnOp p) {
     float fq = 1.f, fk = 1.f, fv = 1.f;
     if constexpr (A::SCALED) { fq = head_factor(p, 0, blockIdx.y, lane); fk = head_factor(p, 1, blockIdx.y, lane); fv = head_factor(p, 2, blockIdx.y, lane); }
     V qf[KS][NP];
-    load_owned<T, E, NP, DHP>((const T*)p.q + (live ? q_row(p, p.qs, b, hk, r) : 0), live, p.dh, half, fq, qf);
+    load_owned<T, E, NP, DHP>((const T*)p.q + (live ? q_row(p, p.qs, b, hk, r) : 0), live, p.dh, half, fq, qf, p.scale < 0.f);
     const T* kbase = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
     const T* vbase = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
     const uint8_t* mask = p.mask ? p.mask + (int64_t)b * p.nk : nullptr;
-    const float c = p.scale * LOG2E * ((1.f / fq) * (1.f / fk));
+    const float c = score_unit(p.scale, fq, fk);
 
     f32x16 o[DT];
 #pragma unroll
@@ -382,38 +431,26 @@ __global__ __launch_bounds__(256, 1) void attn_fwd_kernel(AttnOp p) {
         float mx = -INFINITY;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            f32x16 s1 = zero16();
-            s[n] = zero16();
+            s[n] = first_product<A, KS, LD, PLANE>(Ks, n, lane, qf);
+            if (mask || (t + 1) * R > klen) add_rows(s[n], kb + 32 * n, half);
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                V f[NP];
-                read_rows<E, NP, LD, PLANE>(Ks, n, k, lane, f);
-                mfma_apart<NP, V>(f, qf[k], s[n], s1);
-            }
-            if constexpr (NP > 1) s[n] += s1;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x4 bias = *(const f32x4*)(kb + 32 * n + 8 * g + 4 * half);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[n][4 * g + i] = __builtin_fmaf(s[n][4 * g + i], c, bias[i]);
-                    mx = fmaxf(mx, s[n][4 * g + i]);
-                }
-            }
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
         }
-        mx = other_half_max(mx);
-        const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - mu), ref = mu - A::SHIFT;
-        m = mn;
-        if (__ballot(alpha != 1.f)) {
+        mx = other_half_max(mx) * c;
+        const bool up = mx > m + LAZY;
+        if (__ballot(up)) {
+            const float mn = up ? mx : m, alpha = up ? __builtin_amdgcn_exp2f(m - mn) : 1.f;          // (up: mn is finite or +inf)
+            m = mn;
             l *= alpha;
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d] *= alpha;
         }
+        const float ref = m == -INFINITY ? 0.f : A::SHIFT - m;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[n][i] = __builtin_amdgcn_exp2f(s[n][i] - ref);
+                s[n][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], c, ref));
                 l += s[n][i];
             }
 #pragma unroll
@@ -552,12 +589,12 @@ __global__ __launch_bounds__(256, 1) void attn_dq_kernel(AttnOp p) {
         fq = head_factor(p, 0, blockIdx.y, lane); fk = head_factor(p, 1, blockIdx.y, lane); fv = head_factor(p, 2, blockIdx.y, lane); fo = head_factor(p, 3, blockIdx.y, lane);
     }
     V qf[KS][NP], of[KS][NP];
-    load_owned<T, E, NP, DHP>((const T*)p.q + (live ? q_row(p, p.qs, b, hk, r) : 0), live, p.dh, half, fq, qf);
+    load_owned<T, E, NP, DHP>((const T*)p.q + (live ? q_row(p, p.qs, b, hk, r) : 0), live, p.dh, half, fq, qf, p.scale < 0.f);
     load_owned<T, E, NP, DHP>((const T*)p.dout + (live ? dense_row(p, b, hk, r) * p.dh : 0), live, p.dh, half, fo, of);
     const T* kbase = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
     const T* vbase = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
     const uint8_t* mask = p.mask ? p.mask + (int64_t)b * p.nk : nullptr;
-    const float c = p.scale * LOG2E * ((1.f / fq) * (1.f / fk)), cd = (1.f / fo) * (1.f / fv);
+    const float c = score_unit(p.scale, fq, fk), cd = (1.f / fo) * (1.f / fv);
     LaneScale ls;
     f32x16 dq[DT];
 #pragma unroll
@@ -581,25 +618,11 @@ __global__ __launch_bounds__(256, 1) void attn_dq_kernel(AttnOp p) {
         if (t + 1 < t1) fetch(t + 1);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            f32x16 s = zero16(), dp = zero16(), s1 = zero16(), dp1 = zero16();
+            f32x16 s = first_product<A, KS, LD, PLANE>(Ks, n, lane, qf);
+            const f32x16 dp = first_product<A, KS, LD, PLANE>(Vs, n, lane, of);
+            if (mask || (t + 1) * R > klen) add_rows(s, kb + 32 * n, half);
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                V f[NP];
-                read_rows<E, NP, LD, PLANE>(Ks, n, k, lane, f);
-                mfma_apart<NP, V>(f, qf[k], s, s1);
-                read_rows<E, NP, LD, PLANE>(Vs, n, k, lane, f);
-                mfma_apart<NP, V>(f, of[k], dp, dp1);
-            }
-            if constexpr (NP > 1) { s += s1; dp += dp1; }
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x4 bias = *(const f32x4*)(kb + 32 * n + 8 * g + 4 * half);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], c, -ref) + bias[i]);
-                    s[4 * g + i] = pr * __builtin_fmaf(dp[4 * g + i], cd, -delta);
-                }
-            }
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ref)) * __builtin_fmaf(dp[i], cd, -delta);
             if constexpr (A::LANE) {
                 ls.step(s, dq);
                 s *= ls.f;
@@ -661,9 +684,9 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnOp p) {
         fq = head_factor(p, 0, blockIdx.y, lane); fk = head_factor(p, 1, blockIdx.y, lane); fv = head_factor(p, 2, blockIdx.y, lane); fo = head_factor(p, 3, blockIdx.y, lane);
     }
     V kf[KS][NP], vf[KS][NP];
-    load_owned<T, E, NP, DHP>((const T*)p.k + (live ? b * p.ks[0] + key * p.ks[1] + hk * p.ks[2] : 0), live, p.dh, half, fk, kf);
+    load_owned<T, E, NP, DHP>((const T*)p.k + (live ? b * p.ks[0] + key * p.ks[1] + hk * p.ks[2] : 0), live, p.dh, half, fk, kf, p.scale < 0.f);
     load_owned<T, E, NP, DHP>((const T*)p.v + (live ? b * p.vs[0] + key * p.vs[1] + hk * p.vs[2] : 0), live, p.dh, half, fv, vf);
-    const float c = p.scale * LOG2E * ((1.f / fq) * (1.f / fk)), cd = (1.f / fo) * (1.f / fv), off = live ? (float)A::SHIFT : -INFINITY;
+    const float c = score_unit(p.scale, fq, fk), cd = (1.f / fo) * (1.f / fv);
     LaneScale ls;
     f32x16 dk[DT], dv[DT];
 #pragma unroll
@@ -691,30 +714,22 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnOp p) {
                 ref = row_ref(p.lse[at]);
                 if (ref != INFINITY) dl = p.delta[at];
             }
-            refs[tid] = ref;
+            refs[tid] = ref - A::SHIFT;
             deltas[tid] = dl;
         }
         __syncthreads();
         if (t + 1 < t1) fetch(t + 1);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            f32x16 s = zero16(), dp = zero16(), s1 = zero16(), dp1 = zero16();
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                V f[NP];
-                read_rows<E, NP, LD, PLANE>(Qs, n, k, lane, f);
-                mfma_apart<NP, V>(f, kf[k], s, s1);
-                read_rows<E, NP, LD, PLANE>(Os, n, k, lane, f);
-                mfma_apart<NP, V>(f, vf[k], dp, dp1);
-            }
-            if constexpr (NP > 1) { s += s1; dp += dp1; }
+            f32x16 s = first_product<A, KS, LD, PLANE>(Qs, n, lane, kf);
+            f32x16 dp = first_product<A, KS, LD, PLANE>(Os, n, lane, vf);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const f32x4 ref = *(const f32x4*)(refs + 32 * n + 8 * g + 4 * half);
                 const f32x4 dl = *(const f32x4*)(deltas + 32 * n + 8 * g + 4 * half);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], c, -ref[i]) + off);
+                    const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], c, -ref[i]));
                     s[4 * g + i] = pr;
                     dp[4 * g + i] = pr * __builtin_fmaf(dp[4 * g + i], cd, -dl[i]);
                 }
@@ -740,6 +755,11 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnOp p) {
         }
     }
     if (key >= p.nk) return;
+    if (!live) {                         // a masked key: whatever its lane summed up
+#pragma unroll
+        for (int d = 0; d < DT; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
+        ls.f = 0.f;
+    }
     const float unp = A::SHIFT ? 1.f / (float)(1 << A::SHIFT) : 1.f, unit = p.scale * (1.f / fq) * unp * (A::LANE ? ls.inverse() : 1.f), vunit = (1.f / fo) * unp;
     const int64_t row = ((int64_t)b * p.nk + key) * p.Hkv + hk, rows = (int64_t)p.B * p.nk * p.Hkv;
 #pragma unroll
