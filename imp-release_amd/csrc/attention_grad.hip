@@ -180,22 +180,33 @@ __device__ __forceinline__ int64_t stat_row(const AttnOp& p, int b, int hk, int 
     return ((int64_t)b * p.H + hk * p.G + g) * p.nq + q;
 }
 
+// A tile lies in LDS row by row without padding, its 16-byte chunks exchanged within the row: chunk c of row r at place c ^ turn(r).  Both reads then touch every bank
+// once per pass: 16 neighbouring rows at one chunk (first product), and 4 rows x 64 bytes (transpose read of the second).
+template <int DHP> __device__ __forceinline__ int turn(int r) {
+    if constexpr (DHP == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+    else if constexpr (DHP == 64) return ((r & 2) << 1) | ((r >> 2) & 3);
+    else return (r >> 2) & 3;
+}
 // A operand of the first product: row = lane % 32 of the 32-row sub-tile, 8 columns of k-step s
-template <typename E, int NP, int LD, int PLANE>
+template <typename E, int NP, int DHP, int PLANE>
 __device__ __forceinline__ void read_rows(const E* tile, int sub, int s, int lane, typename Vec8<E>::type (&f)[NP]) {
-    const E* a = tile + (sub * 32 + (lane & 31)) * LD + 16 * s + 8 * (lane >> 5);
+    const int r = lane & 31;
+    const E* a = tile + sub * 32 * DHP + r * DHP + ((((lane >> 5) ^ turn<DHP>(r)) ^ (2 * s)) * 8);
 #pragma unroll
     for (int j = 0; j < NP; ++j) f[j] = *(const typename Vec8<E>::type*)(a + j * PLANE);
 }
 // A operand of the second product: the tile transposed, channel = 32 dt + lane % 32, slot e of half h = row 16 s + 8 (e / 4) + 4 h + e % 4
-template <typename E, int NP, int LD, int PLANE>
+template <typename E, int NP, int DHP, int PLANE>
 __device__ __forceinline__ void read_cols(const E* tile, int sub, int s, int dt, int lane, typename Vec8<E>::type (&f)[NP]) {
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    const E* a = tile + (sub * 32 + 16 * s + 4 * (lane >> 5) + ((lane & 15) >> 2)) * LD + 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const int r = 4 * (lane >> 5) + ((lane & 15) >> 2), c = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ turn<DHP>(r);
+    const E* base = tile + (sub * 32 + 16 * s) * DHP + 4 * (lane & 1);
+    const E* a0 = base + r * DHP + (c ^ (4 * dt)) * 8;
+    const E* a1 = base + (r + 8) * DHP + (c ^ (4 * dt) ^ 2) * 8;             // turn(r + 8) = turn(r) ^ 2
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + j * PLANE));
-        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + j * PLANE + 8 * LD));
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a0 + j * PLANE));
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a1 + j * PLANE));
         f[j] = __builtin_bit_cast(typename Vec8<E>::type, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 }
@@ -217,7 +228,7 @@ __device__ __forceinline__ void load_owned(const T* row, bool live, int dh, int 
 // One tile of the walked side: 256 threads fetch R rows x DHP columns of two matrices into registers, and store them as planes
 template <typename T, typename E, int NP, int DHP, int R>
 struct Stage {
-    static constexpr int CPR = DHP / 8, N = (R * CPR + 255) / 256, LD = DHP + 8, PLANE = R * LD;
+    static constexpr int CPR = DHP / 8, N = (R * CPR + 255) / 256, PLANE = R * DHP;
     Chunk<T> x[N], y[N];
     // addr(i, row, live) -> pointers of both matrices' rows
     template <typename F> __device__ void fetch(int tid, int dh, F addr) {
@@ -236,15 +247,15 @@ struct Stage {
     __device__ void store(int tid, E* X, E* Y, float fx, float fy) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int c = tid + 256 * i, row = c / CPR, col = (c % CPR) * 8;
+            const int c = tid + 256 * i, row = c / CPR, at = row * DHP + ((c % CPR) ^ turn<DHP>(row)) * 8;
             if (R * CPR % 256 == 0 || row < R) {
                 typename Vec8<E>::type p[NP];
                 to_planes<T, NP, E>(x[i], fx, p);
 #pragma unroll
-                for (int j = 0; j < NP; ++j) *(typename Vec8<E>::type*)(X + j * PLANE + row * LD + col) = p[j];
+                for (int j = 0; j < NP; ++j) *(typename Vec8<E>::type*)(X + j * PLANE + at) = p[j];
                 to_planes<T, NP, E>(y[i], fy, p);
 #pragma unroll
-                for (int j = 0; j < NP; ++j) *(typename Vec8<E>::type*)(Y + j * PLANE + row * LD + col) = p[j];
+                for (int j = 0; j < NP; ++j) *(typename Vec8<E>::type*)(Y + j * PLANE + at) = p[j];
             }
         }
     }
@@ -253,7 +264,7 @@ struct Stage {
 __device__ __forceinline__ f32x16 zero16();
 // the first product of a 32 x 32 sub-tile: rows of `tile` times the owned rows.  Over all k-steps the small products come first and hi . hi last: the sum is rounded once
 // per k-step at its full size, not once per product - what dS = P (dP - D) keeps after the cancellation is decided here
-template <typename A, int KS, int LD, int PLANE>
+template <typename A, int KS, int DHP, int PLANE>
 __device__ __forceinline__ f32x16 first_product(const typename A::E* tile, int sub, int lane, const typename A::V (&own)[KS][A::NP]) {
     using V = typename A::V;
     f32x16 c = zero16();
@@ -261,7 +272,7 @@ __device__ __forceinline__ f32x16 first_product(const typename A::E* tile, int s
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
         V f[A::NP];
-        read_rows<typename A::E, A::NP, LD, PLANE>(tile, sub, k, lane, f);
+        read_rows<typename A::E, A::NP, DHP, PLANE>(tile, sub, k, lane, f);
         if constexpr (A::NP == 3) {
             c = mfma(f[1], own[k][1], c);
             c = mfma(f[0], own[k][2], c);
@@ -379,13 +390,13 @@ __global__ __launch_bounds__(256) void attn_amax_kernel(AttnOp p) {
 
 // ---------------------------------------------------------------------------------------------------------------------- forward
 template <typename A, int DHP>
-__global__ __launch_bounds__(256, 1) void attn_fwd_kernel(AttnOp p) {
+__global__ __launch_bounds__(256, A::NP == 3 && DHP == 128 ? 1 : 2) void attn_fwd_kernel(AttnOp p) {
     using T = typename A::T;
     using E = typename A::E;
     using V = typename A::V;
     constexpr int NP = A::NP, R = A::R;
     using St = Stage<T, E, NP, DHP, R>;
-    constexpr int LD = St::LD, PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32;
+    constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32;
     __shared__ __attribute__((aligned(16))) E Ks[NP * PLANE], Vs[NP * PLANE];
     __shared__ __attribute__((aligned(16))) float kb[R];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
@@ -431,7 +442,7 @@ __global__ __launch_bounds__(256, 1) void attn_fwd_kernel(AttnOp p) {
         float mx = -INFINITY;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            s[n] = first_product<A, KS, LD, PLANE>(Ks, n, lane, qf);
+            s[n] = first_product<A, KS, DHP, PLANE>(Ks, n, lane, qf);
             if (mask || (t + 1) * R > klen) add_rows(s[n], kb + 32 * n, half);
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
@@ -460,7 +471,7 @@ __global__ __launch_bounds__(256, 1) void attn_fwd_kernel(AttnOp p) {
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
                     V f[NP];
-                    read_cols<E, NP, LD, PLANE>(Vs, n, k, d, lane, f);
+                    read_cols<E, NP, DHP, PLANE>(Vs, n, k, d, lane, f);
                     o[d] = mfma_planes<NP, V>(f, pf, o[d]);
                 }
             }
@@ -559,13 +570,13 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(AttnOp p) {
 __device__ __forceinline__ float row_ref(float lse) { return lse == -INFINITY ? INFINITY : lse * LOG2E; }
 
 template <typename A, int DHP>
-__global__ __launch_bounds__(256, 1) void attn_dq_kernel(AttnOp p) {
+__global__ __launch_bounds__(256, A::NP > 1 && DHP == 128 ? 1 : 2) void attn_dq_kernel(AttnOp p) {
     using T = typename A::T;
     using E = typename A::E;
     using V = typename A::V;
     constexpr int NP = A::NP, R = A::R;
     using St = Stage<T, E, NP, DHP, R>;
-    constexpr int LD = St::LD, PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32;
+    constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32;
     __shared__ __attribute__((aligned(16))) E Ks[NP * PLANE], Vs[NP * PLANE];
     __shared__ __attribute__((aligned(16))) float kb[R];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
@@ -618,8 +629,8 @@ __global__ __launch_bounds__(256, 1) void attn_dq_kernel(AttnOp p) {
         if (t + 1 < t1) fetch(t + 1);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            f32x16 s = first_product<A, KS, LD, PLANE>(Ks, n, lane, qf);
-            const f32x16 dp = first_product<A, KS, LD, PLANE>(Vs, n, lane, of);
+            f32x16 s = first_product<A, KS, DHP, PLANE>(Ks, n, lane, qf);
+            const f32x16 dp = first_product<A, KS, DHP, PLANE>(Vs, n, lane, of);
             if (mask || (t + 1) * R > klen) add_rows(s, kb + 32 * n, half);
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ref)) * __builtin_fmaf(dp[i], cd, -delta);
@@ -634,7 +645,7 @@ __global__ __launch_bounds__(256, 1) void attn_dq_kernel(AttnOp p) {
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
                     V f[NP];
-                    read_cols<E, NP, LD, PLANE>(Ks, n, k, d, lane, f);
+                    read_cols<E, NP, DHP, PLANE>(Ks, n, k, d, lane, f);
                     dq[d] = mfma_planes<NP, V>(f, df, dq[d]);
                 }
             }
@@ -661,13 +672,13 @@ __global__ __launch_bounds__(256, 1) void attn_dq_kernel(AttnOp p) {
 }
 
 template <typename A, int DHP>
-__global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnOp p) {
+__global__ __launch_bounds__(256, DHP == 128 || (A::NP == 3 && DHP == 64) ? 1 : 2) void attn_dkv_kernel(AttnOp p) {
     using T = typename A::T;
     using E = typename A::E;
     using V = typename A::V;
     constexpr int NP = A::NP, R = A::R;
     using St = Stage<T, E, NP, DHP, R>;
-    constexpr int LD = St::LD, PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32;
+    constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32;
     __shared__ __attribute__((aligned(16))) E Qs[NP * PLANE], Os[NP * PLANE];
     __shared__ __attribute__((aligned(16))) float refs[R], deltas[R];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
@@ -721,8 +732,8 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnOp p) {
         if (t + 1 < t1) fetch(t + 1);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            f32x16 s = first_product<A, KS, LD, PLANE>(Qs, n, lane, kf);
-            f32x16 dp = first_product<A, KS, LD, PLANE>(Os, n, lane, vf);
+            f32x16 s = first_product<A, KS, DHP, PLANE>(Qs, n, lane, kf);
+            f32x16 dp = first_product<A, KS, DHP, PLANE>(Os, n, lane, vf);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const f32x4 ref = *(const f32x4*)(refs + 32 * n + 8 * g + 4 * half);
@@ -746,9 +757,9 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnOp p) {
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
                     V f[NP];
-                    read_cols<E, NP, LD, PLANE>(Os, n, k, d, lane, f);
+                    read_cols<E, NP, DHP, PLANE>(Os, n, k, d, lane, f);
                     dv[d] = mfma_planes<NP, V>(f, pf, dv[d]);
-                    read_cols<E, NP, LD, PLANE>(Qs, n, k, d, lane, f);
+                    read_cols<E, NP, DHP, PLANE>(Qs, n, k, d, lane, f);
                     dk[d] = mfma_planes<NP, V>(f, df, dk[d]);
                 }
             }
