@@ -49,6 +49,7 @@ struct AttnOp {
     const int32_t *q_lens, *k_lens;
     int64_t qs[3], ks[3], vs[3];         // batch, token, head strides in elements
     int B, nq, nk, H, Hkv, G, dh;
+    int gshift;                          // log2 G, or -1
     float scale;
     int shares;
     float* amax;                         // [4][B * Hkv][chunks]: largest finite |q|, |k|, |v|, |dout| of a part of the rows (fp32 split halves)
@@ -167,16 +168,17 @@ template <typename T> __device__ __forceinline__ void store4(T* p, float a, floa
 __device__ __forceinline__ int clamp_len(const int32_t* lens, int b, int n) { return lens ? min(max(lens[b], 0), n) : n; }
 
 // row r = q G + g of key head hk (query side)
+__device__ __forceinline__ int query_of(const AttnOp& p, int r) { return p.gshift >= 0 ? r >> p.gshift : r / p.G; }
 __device__ __forceinline__ int64_t q_row(const AttnOp& p, const int64_t (&st)[3], int b, int hk, int r) {
-    const int q = r / p.G, g = r - q * p.G;
+    const int q = query_of(p, r), g = r - q * p.G;
     return b * st[0] + q * st[1] + (int64_t)(hk * p.G + g) * st[2];
 }
 __device__ __forceinline__ int64_t dense_row(const AttnOp& p, int b, int hk, int r) {        // row index in [B][nq][H]
-    const int q = r / p.G, g = r - q * p.G;
+    const int q = query_of(p, r), g = r - q * p.G;
     return ((int64_t)b * p.nq + q) * p.H + hk * p.G + g;
 }
 __device__ __forceinline__ int64_t stat_row(const AttnOp& p, int b, int hk, int r) {         // index in [B][H][nq]
-    const int q = r / p.G, g = r - q * p.G;
+    const int q = query_of(p, r), g = r - q * p.G;
     return ((int64_t)b * p.H + hk * p.G + g) * p.nq + q;
 }
 
@@ -225,30 +227,35 @@ __device__ __forceinline__ void load_owned(const T* row, bool live, int dh, int 
     }
 }
 
-// One tile of the walked side: 256 threads fetch R rows x DHP columns of two matrices into registers, and store them as planes
+// One tile of the walked side: 256 threads fetch R rows x DHP columns of two matrices into registers, and store them as planes.  Nothing is waited for between: whether a
+// row exists at all (a mask byte, or its lse) is fetched beside it, and what does not exist becomes zeros on the way to LDS
 template <typename T, typename E, int NP, int DHP, int R>
 struct Stage {
     static constexpr int CPR = DHP / 8, N = (R * CPR + 255) / 256, PLANE = R * DHP;
     Chunk<T> x[N], y[N];
-    // addr(i, row, live) -> pointers of both matrices' rows
-    template <typename F> __device__ void fetch(int tid, int dh, F addr) {
+    int flag[N];
+    // addr(row, px, py): whether the row lies inside the tensors, and its pointers; mark(row): its flag
+    template <typename F, typename M> __device__ void fetch(int tid, int dh, F addr, M mark) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = tid + 256 * i, row = c / CPR, col = (c % CPR) * 8;
             x[i].zero();
             y[i].zero();
+            flag[i] = 0;
             const T *px, *py;
             if ((R * CPR % 256 == 0 || row < R) && col < dh && addr(row, px, py)) {
                 x[i].load(px + col);
                 y[i].load(py + col);
+                flag[i] = mark(row);
             }
         }
     }
-    __device__ void store(int tid, E* X, E* Y, float fx, float fy) const {
+    template <typename L> __device__ void store(int tid, E* X, E* Y, float fx, float fy, L lives) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = tid + 256 * i, row = c / CPR, at = row * DHP + ((c % CPR) ^ turn<DHP>(row)) * 8;
             if (R * CPR % 256 == 0 || row < R) {
+                if (!lives(flag[i])) { x[i].zero(); y[i].zero(); }
                 typename Vec8<E>::type p[NP];
                 to_planes<T, NP, E>(x[i], fx, p);
 #pragma unroll
@@ -422,20 +429,22 @@ __global__ __launch_bounds__(256, A::NP == 3 && DHP == 128 ? 1 : 2) void attn_fw
     for (int d = 0; d < DT; ++d) o[d] = zero16();
     float m = -INFINITY, l = 0.f;
     St st;
+    int keep = 0;
     auto fetch = [&](int t) {
         st.fetch(tid, p.dh, [&](int row, const T*& px, const T*& py) {
             const int key = t * R + row;
-            if (key >= klen || (mask && !mask[key])) return false;
             px = kbase + key * p.ks[1];
             py = vbase + key * p.vs[1];
-            return true;
-        });
+            return key < klen;
+        }, [&](int row) { return mask ? (int)mask[t * R + row] : 1; });
+        if (tid < R) { const int key = t * R + tid; keep = key < klen ? (mask ? (int)mask[key] : 1) : 0; }
     };
+    auto exists = [](int flag) { return flag != 0; };
     if (t0 < t1) fetch(t0);
     for (int t = t0; t < t1; ++t) {
         __syncthreads();
-        st.store(tid, Ks, Vs, fk, fv);
-        if (tid < R) { const int key = t * R + tid; kb[tid] = key < klen && (!mask || mask[key]) ? 0.f : -INFINITY; }
+        st.store(tid, Ks, Vs, fk, fv, exists);
+        if (tid < R) kb[tid] = keep ? 0.f : -INFINITY;
         __syncthreads();
         if (t + 1 < t1) fetch(t + 1);
         f32x16 s[NT];
@@ -611,20 +620,22 @@ __global__ __launch_bounds__(256, A::NP > 1 && DHP == 128 ? 1 : 2) void attn_dq_
 #pragma unroll
     for (int d = 0; d < DT; ++d) dq[d] = zero16();
     St st;
+    int keep = 0;
     auto fetch = [&](int t) {
         st.fetch(tid, p.dh, [&](int row, const T*& px, const T*& py) {
             const int key = t * R + row;
-            if (key >= klen || (mask && !mask[key])) return false;
             px = kbase + key * p.ks[1];
             py = vbase + key * p.vs[1];
-            return true;
-        });
+            return key < klen;
+        }, [&](int row) { return mask ? (int)mask[t * R + row] : 1; });
+        if (tid < R) { const int key = t * R + tid; keep = key < klen ? (mask ? (int)mask[key] : 1) : 0; }
     };
+    auto exists = [](int flag) { return flag != 0; };
     if (t0 < t1) fetch(t0);
     for (int t = t0; t < t1; ++t) {
         __syncthreads();
-        st.store(tid, Ks, Vs, fk, fv);
-        if (tid < R) { const int key = t * R + tid; kb[tid] = key < klen && (!mask || mask[key]) ? 0.f : -INFINITY; }
+        st.store(tid, Ks, Vs, fk, fv, exists);
+        if (tid < R) kb[tid] = keep ? 0.f : -INFINITY;
         __syncthreads();
         if (t + 1 < t1) fetch(t + 1);
 #pragma unroll
@@ -703,30 +714,33 @@ __global__ __launch_bounds__(256, DHP == 128 || (A::NP == 3 && DHP == 64) ? 1 : 
 #pragma unroll
     for (int d = 0; d < DT; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
     St st;
-    auto row_live = [&](int r) { return r < live_rows && p.lse[stat_row(p, b, hk, r)] != -INFINITY; };
+    float ref = -INFINITY, delta = 0.f;
     auto fetch = [&](int t) {
         st.fetch(tid, p.dh, [&](int row, const T*& px, const T*& py) {
             const int r = t * R + row;
-            if (!row_live(r)) return false;
             px = (const T*)p.q + q_row(p, p.qs, b, hk, r);
             py = (const T*)p.dout + dense_row(p, b, hk, r) * p.dh;
-            return true;
-        });
+            return r < live_rows;
+        }, [&](int row) { return __builtin_bit_cast(int, p.lse[stat_row(p, b, hk, t * R + row)]); });
+        if (tid < R) {
+            const int r = t * R + tid;
+            ref = -INFINITY;
+            if (r < live_rows) {
+                const int64_t at = stat_row(p, b, hk, r);
+                ref = p.lse[at];
+                delta = p.delta[at];
+            }
+        }
     };
+    // chunks past the tensors are zeros already, whatever their flag
+    auto exists = [](int flag) { return __builtin_bit_cast(float, flag) != -INFINITY; };
     if (t0 < t1) fetch(t0);
     for (int t = t0; t < t1; ++t) {
         __syncthreads();
-        st.store(tid, Qs, Os, fq, fo);
+        st.store(tid, Qs, Os, fq, fo, exists);
         if (tid < R) {
-            const int r = t * R + tid;
-            float ref = INFINITY, dl = 0.f;
-            if (r < live_rows) {
-                const int64_t at = stat_row(p, b, hk, r);
-                ref = row_ref(p.lse[at]);
-                if (ref != INFINITY) dl = p.delta[at];
-            }
-            refs[tid] = ref - A::SHIFT;
-            deltas[tid] = dl;
+            refs[tid] = row_ref(ref) - A::SHIFT;
+            deltas[tid] = ref == -INFINITY ? 0.f : delta;
         }
         __syncthreads();
         if (t + 1 < t1) fetch(t + 1);
@@ -855,6 +869,7 @@ AttnOp op_of(const imp_attn_desc& d) {
     p.mask = d.key_mask; p.q_lens = d.q_lens; p.k_lens = d.k_lens;
     for (int i = 0; i < 3; ++i) { p.qs[i] = d.q_stride[i]; p.ks[i] = d.k_stride[i]; p.vs[i] = d.v_stride[i]; }
     p.B = d.batch; p.nq = d.nq; p.nk = d.nk; p.H = d.heads; p.Hkv = d.kv_heads; p.G = d.heads / d.kv_heads; p.dh = d.head_dim;
+    p.gshift = p.G & (p.G - 1) ? -1 : __builtin_ctz(p.G);
     p.scale = d.scale;
     return p;
 }
