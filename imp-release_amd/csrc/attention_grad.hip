@@ -351,7 +351,9 @@ struct LaneScale {
         float m = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[i]));
-        m = other_half_max(m);
+        step_max(other_half_max(m), acc);
+    }
+    template <int DT> __device__ void step_max(float m, f32x16 (&acc)[DT]) {
         const bool grow = m * f > 32768.f || (f == 0.f && m > 0.f);
         if (__ballot(grow)) {
             const float nf = grow ? __builtin_ldexpf(1.f, clamp_exp(10 - __builtin_amdgcn_frexp_expf(m))) : f;
@@ -682,6 +684,30 @@ __global__ __launch_bounds__(256, A::NP > 1 && DHP == 128 ? 1 : 2) void attn_dq_
         }
 }
 
+// channels from c0 of one key's dk and dv, or of its share of them
+template <typename T, int DT>
+__device__ __forceinline__ void store_dkv(const AttnOp& p, int b, int hk, int key, int share, int c0, int half, const f32x16 (&dk)[DT], const f32x16 (&dv)[DT], float unit,
+                                          float vunit) {
+    const int64_t row = ((int64_t)b * p.nk + key) * p.Hkv + hk, rows = (int64_t)p.B * p.nk * p.Hkv;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int col = c0 + 32 * d + 8 * g + 4 * half;
+            if (col < p.dh) {
+                const float x0 = dk[d][4 * g] * unit, x1 = dk[d][4 * g + 1] * unit, x2 = dk[d][4 * g + 2] * unit, x3 = dk[d][4 * g + 3] * unit;
+                const float y0 = dv[d][4 * g] * vunit, y1 = dv[d][4 * g + 1] * vunit, y2 = dv[d][4 * g + 2] * vunit, y3 = dv[d][4 * g + 3] * vunit;
+                if (p.shares > 1) {
+                    store4(p.part + (2 * share * rows + row) * p.dh + col, x0, x1, x2, x3);
+                    store4(p.part + ((2 * share + 1) * rows + row) * p.dh + col, y0, y1, y2, y3);
+                } else {
+                    store4((T*)p.dk + row * p.dh + col, x0, x1, x2, x3);
+                    store4((T*)p.dv + row * p.dh + col, y0, y1, y2, y3);
+                }
+            }
+        }
+}
+
 template <typename A, int DHP>
 __global__ __launch_bounds__(256, DHP == 128 || (A::NP == 3 && DHP == 64) ? 1 : 2) void attn_dkv_kernel(AttnOp p) {
     using T = typename A::T;
@@ -785,25 +811,131 @@ __global__ __launch_bounds__(256, DHP == 128 || (A::NP == 3 && DHP == 64) ? 1 : 
         for (int d = 0; d < DT; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
         ls.f = 0.f;
     }
-    const float unp = A::SHIFT ? 1.f / (float)(1 << A::SHIFT) : 1.f, unit = p.scale * (1.f / fq) * unp * (A::LANE ? ls.inverse() : 1.f), vunit = (1.f / fo) * unp;
-    const int64_t row = ((int64_t)b * p.nk + key) * p.Hkv + hk, rows = (int64_t)p.B * p.nk * p.Hkv;
+    const float unp = A::SHIFT ? 1.f / (float)(1 << A::SHIFT) : 1.f;
+    store_dkv<T, DT>(p, b, hk, key, share, 0, half, dk, dv, p.scale * (1.f / fq) * unp * (A::LANE ? ls.inverse() : 1.f), (1.f / fo) * unp);
+}
+
+// dK / dV for 128 channels in 16-bit types: 128 fp32 accumulators and 64 registers of operands leave a wave of the kernel above alone on its SIMD.  Here two waves share 32 keys:
+// wave h computes the scores of the h-th 32 rows of a tile, hands P and dS on through LDS (in the operand layout they are used in), and sums its half of the channels over
+// both.  No product is computed twice; 64 accumulators, two waves per SIMD.
+template <typename A>
+__global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
+    using T = typename A::T;
+    using E = typename A::E;
+    using V = typename A::V;
+    static_assert(A::NP == 1 && A::R == 64);
+    constexpr int NP = 1, R = 64, DHP = 128;
+    using St = Stage<T, E, NP, DHP, R>;
+    constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = 2;
+    __shared__ __attribute__((aligned(16))) E Qs[PLANE], Os[PLANE];
+    __shared__ __attribute__((aligned(16))) float refs[R], deltas[R];
+    __shared__ __attribute__((aligned(16))) V hand[4][4][64];
+    __shared__ float largest[4][32];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6, h = wave & 1;
+    const int b = blockIdx.y / p.Hkv, hk = blockIdx.y % p.Hkv, share = blockIdx.z;
+    const int klen = clamp_len(p.k_lens, b, p.nk), live_rows = clamp_len(p.q_lens, b, p.nq) * p.G;
+    const int own0 = blockIdx.x * (OWN / 2), key = own0 + 32 * (wave >> 1) + (lane & 31);
+    const bool live = key < klen && (!p.mask || p.mask[(int64_t)b * p.nk + key]);
+    const int tiles = (live_rows + R - 1) / R;
+    int t0 = 0, t1 = own0 < klen ? tiles : 0;
+    if (p.shares > 1 && t1) { t0 = (int)((int64_t)tiles * share / p.shares); t1 = (int)((int64_t)tiles * (share + 1) / p.shares); }
+
+    V kf[KS][NP], vf[KS][NP];
+    load_owned<T, E, NP, DHP>((const T*)p.k + (live ? b * p.ks[0] + key * p.ks[1] + hk * p.ks[2] : 0), live, p.dh, half, 1.f, kf, p.scale < 0.f);
+    load_owned<T, E, NP, DHP>((const T*)p.v + (live ? b * p.vs[0] + key * p.vs[1] + hk * p.vs[2] : 0), live, p.dh, half, 1.f, vf);
+    const float c = score_unit(p.scale, 1.f, 1.f);
+    LaneScale ls;
+    f32x16 dk[DT], dv[DT];
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int col = 32 * d + 8 * g + 4 * half;
-            if (col < p.dh) {
-                const float x0 = dk[d][4 * g] * unit, x1 = dk[d][4 * g + 1] * unit, x2 = dk[d][4 * g + 2] * unit, x3 = dk[d][4 * g + 3] * unit;
-                const float y0 = dv[d][4 * g] * vunit, y1 = dv[d][4 * g + 1] * vunit, y2 = dv[d][4 * g + 2] * vunit, y3 = dv[d][4 * g + 3] * vunit;
-                if (p.shares > 1) {
-                    store4(p.part + (2 * share * rows + row) * p.dh + col, x0, x1, x2, x3);
-                    store4(p.part + ((2 * share + 1) * rows + row) * p.dh + col, y0, y1, y2, y3);
-                } else {
-                    store4((T*)p.dk + row * p.dh + col, x0, x1, x2, x3);
-                    store4((T*)p.dv + row * p.dh + col, y0, y1, y2, y3);
-                }
+    for (int d = 0; d < DT; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
+    St st;
+    float ref = -INFINITY, delta = 0.f;
+    auto fetch = [&](int t) {
+        st.fetch(tid, p.dh, [&](int row, const T*& px, const T*& py) {
+            const int r = t * R + row;
+            px = (const T*)p.q + q_row(p, p.qs, b, hk, r);
+            py = (const T*)p.dout + dense_row(p, b, hk, r) * p.dh;
+            return r < live_rows;
+        }, [&](int row) { return __builtin_bit_cast(int, p.lse[stat_row(p, b, hk, t * R + row)]); });
+        if (tid < R) {
+            const int r = t * R + tid;
+            ref = -INFINITY;
+            if (r < live_rows) {
+                const int64_t at = stat_row(p, b, hk, r);
+                ref = p.lse[at];
+                delta = p.delta[at];
             }
         }
+    };
+    auto exists = [](int flag) { return __builtin_bit_cast(float, flag) != -INFINITY; };
+    auto sums = [&](int n, int k, V pk, V dsk) __attribute__((always_inline)) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            V f[NP];
+            read_cols<E, NP, DHP, PLANE>(Os, n, k, 2 * h + d, lane, f);
+            dv[d] = mfma(f[0], pk, dv[d]);
+            read_cols<E, NP, DHP, PLANE>(Qs, n, k, 2 * h + d, lane, f);
+            dk[d] = mfma(f[0], dsk, dk[d]);
+        }
+    };
+    if (t0 < t1) fetch(t0);
+    for (int t = t0; t < t1; ++t) {
+        __syncthreads();
+        st.store(tid, Qs, Os, 1.f, 1.f, exists);
+        if (tid < R) {
+            refs[tid] = row_ref(ref) - A::SHIFT;
+            deltas[tid] = ref == -INFINITY ? 0.f : delta;
+        }
+        __syncthreads();
+        if (t + 1 < t1) fetch(t + 1);
+        f32x16 s = first_product<A, KS, DHP, PLANE>(Qs, h, lane, kf);
+        f32x16 dp = first_product<A, KS, DHP, PLANE>(Os, h, lane, vf);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 rv = *(const f32x4*)(refs + 32 * h + 8 * g + 4 * half);
+            const f32x4 dl = *(const f32x4*)(deltas + 32 * h + 8 * g + 4 * half);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], c, -rv[i]));
+                s[4 * g + i] = pr;
+                dp[4 * g + i] = pr * (dp[4 * g + i] - dl[i]);
+            }
+        }
+        if constexpr (A::LANE) {         // both waves of the keys take the same factor
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(dp[i]));
+            m = other_half_max(m);
+            if (!half) largest[wave][lane] = m;
+            __syncthreads();
+            ls.step_max(fmaxf(m, largest[wave ^ 1][lane & 31]), dk);
+            dp *= ls.f;
+        }
+        V pf[2], df[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            V one[1];
+            pack<NP, E>(s, k, one);
+            pf[k] = one[0];
+            pack<NP, E>(dp, k, one);
+            df[k] = one[0];
+            hand[wave][2 * k][lane] = pf[k];
+            hand[wave][2 * k + 1][lane] = df[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) sums(h, k, pf[k], df[k]);
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 2; ++k) sums(h ^ 1, k, hand[wave ^ 1][2 * k][lane], hand[wave ^ 1][2 * k + 1][lane]);
+    }
+    if (key >= p.nk) return;
+    if (!live) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
+        ls.f = 0.f;
+    }
+    const float unp = A::SHIFT ? 1.f / (float)(1 << A::SHIFT) : 1.f;
+    store_dkv<T, DT>(p, b, hk, key, share, 64 * h, half, dk, dv, p.scale * unp * (A::LANE ? ls.inverse() : 1.f), unp);
 }
 
 // out[i] = sum over the shares, in their order (4 elements per thread; n % 4 == 0)
@@ -828,7 +960,9 @@ struct Plan { int fwd, dq, dkv, chunks; bool split; int64_t q_rows, k_rows; size
 Plan plan(const imp_attn_desc& d) {
     Plan p;
     const int64_t heads = (int64_t)d.batch * d.kv_heads, rows = (int64_t)d.nq * (d.heads / d.kv_heads);
-    const int64_t qb = (rows + OWN - 1) / OWN * heads, kbk = ((int64_t)d.nk + OWN - 1) / OWN * heads;
+    const int64_t qb = (rows + OWN - 1) / OWN * heads;
+    const int own_keys = d.dtype != IMP_DTYPE_F32 && d.head_dim > 64 ? OWN / 2 : OWN;          // the paired kernel's 64
+    const int64_t kbk = ((int64_t)d.nk + own_keys - 1) / own_keys * heads;
     p.fwd = shares_for(qb, d.nk);
     p.dq = p.fwd;
     p.dkv = shares_for(kbk, rows);
@@ -880,6 +1014,7 @@ template <typename A, int DHP> void launch(int which, const AttnOp& p, hipStream
     const dim3 grid((unsigned)((own + OWN - 1) / OWN), (unsigned)(p.B * p.Hkv), (unsigned)p.shares);
     if (which == 0) attn_fwd_kernel<A, DHP><<<grid, 256, 0, st>>>(p);
     else if (which == 1) attn_dq_kernel<A, DHP><<<grid, 256, 0, st>>>(p);
+    else if constexpr (A::NP == 1 && DHP == 128) attn_dkv_pair_kernel<A><<<dim3((unsigned)((own + OWN / 2 - 1) / (OWN / 2)), grid.y, grid.z), 256, 0, st>>>(p);
     else attn_dkv_kernel<A, DHP><<<grid, 256, 0, st>>>(p);
 }
 template <typename A> void launch_dh(int which, const AttnOp& p, hipStream_t st) {
