@@ -124,6 +124,10 @@ template <typename T> struct Chunk;
 template <> struct Chunk<float> {
     f32x4 a, b;
     __device__ void load(const float* p) { a = *(const f32x4*)p; b = *(const f32x4*)(p + 4); }
+    __device__ void load(__amdgpu_buffer_rsrc_t r, unsigned off) {
+        a = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+        b = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off + 16, 0, 0));
+    }
     __device__ void zero() { a = f32x4{0, 0, 0, 0}; b = a; }
     __device__ void negate() { a = -a; b = -b; }
     __device__ void get(float (&x)[8]) const { for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[i + 4] = b[i]; } }
@@ -131,6 +135,7 @@ template <> struct Chunk<float> {
 template <typename T> struct Chunk16 {
     u32x4 a;
     __device__ void load(const T* p) { a = *(const u32x4*)p; }
+    __device__ void load(__amdgpu_buffer_rsrc_t r, unsigned off) { a = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0); }
     __device__ void zero() { a = u32x4{0, 0, 0, 0}; }
     __device__ void negate() { a ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u}; }
     __device__ void get(float (&x)[8]) const {
@@ -227,35 +232,50 @@ __device__ __forceinline__ void load_owned(const T* row, bool live, int dh, int 
     }
 }
 
-// One tile of the walked side: 256 threads fetch R rows x DHP columns of two matrices into registers, and store them as planes.  Nothing is waited for between: whether a
-// row exists at all (a mask byte, or its lse) is fetched beside it, and what does not exist becomes zeros on the way to LDS
+constexpr unsigned OUTSIDE = 0x80000000u;    // an offset past the end of a buffer descriptor: the load returns zeros
+// One tile of the walked side: 256 threads fetch R rows x DHP columns of two matrices into registers, and store them as planes.  A thread's places within a tile are 32-bit
+// offsets; a buffer descriptor moves with the tile, and rows and channels that do not exist are offsets past its end.  Nothing is waited for between.  Rows inside the tensors
+// that do not count (masked keys, queries without a key) become zeros on the way to LDS.
 template <typename T, typename E, int NP, int DHP, int R>
 struct Stage {
     static constexpr int CPR = DHP / 8, N = (R * CPR + 255) / 256, PLANE = R * DHP;
     Chunk<T> x[N], y[N];
-    int flag[N];
-    // addr(row, px, py): whether the row lies inside the tensors, and its pointers; mark(row): its flag
-    template <typename F, typename M> __device__ void fetch(int tid, int dh, F addr, M mark) {
+    unsigned xo[N], yo[N];
+    // offs(row, x, y): element offsets of a tile's row in both matrices
+    template <typename F> __device__ void places(int tid, int dh, F offs) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = tid + 256 * i, row = c / CPR, col = (c % CPR) * 8;
-            x[i].zero();
-            y[i].zero();
-            flag[i] = 0;
-            const T *px, *py;
-            if ((R * CPR % 256 == 0 || row < R) && col < dh && addr(row, px, py)) {
-                x[i].load(px + col);
-                y[i].load(py + col);
-                flag[i] = mark(row);
-            }
+            int64_t ox, oy;
+            offs(row, ox, oy);
+            const bool in = row < R && col < dh;
+            xo[i] = in ? (unsigned)((ox + col) * (int64_t)sizeof(T)) : OUTSIDE;
+            yo[i] = in ? (unsigned)((oy + col) * (int64_t)sizeof(T)) : OUTSIDE;
         }
     }
-    template <typename L> __device__ void store(int tid, E* X, E* Y, float fx, float fy, L lives) {
+    // the tile at px, py, of which `left` rows exist
+    __device__ void fetch(int tid, const T* px, const T* py, int left) {
+        const auto rx = __builtin_amdgcn_make_buffer_rsrc((void*)px, 0, 0x7fffff00, 0x27000), ry = __builtin_amdgcn_make_buffer_rsrc((void*)py, 0, 0x7fffff00, 0x27000);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bool in = (tid + 256 * i) / CPR < left;
+            x[i].load(rx, in ? xo[i] : OUTSIDE);
+            y[i].load(ry, in ? yo[i] : OUTSIDE);
+        }
+    }
+    // alive: which of the tile's rows count (LDS), or null
+    __device__ void store(int tid, E* X, E* Y, float fx, float fy, const int* alive) {
+        if (alive) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int row = (tid + 256 * i) / CPR;
+                if (row < R && !alive[row]) { x[i].zero(); y[i].zero(); }
+            }
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = tid + 256 * i, row = c / CPR, at = row * DHP + ((c % CPR) ^ turn<DHP>(row)) * 8;
             if (R * CPR % 256 == 0 || row < R) {
-                if (!lives(flag[i])) { x[i].zero(); y[i].zero(); }
                 typename Vec8<E>::type p[NP];
                 to_planes<T, NP, E>(x[i], fx, p);
 #pragma unroll
@@ -408,6 +428,7 @@ __global__ __launch_bounds__(256, A::NP == 3 && DHP == 128 ? 1 : 2) void attn_fw
     constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32;
     __shared__ __attribute__((aligned(16))) E Ks[NP * PLANE], Vs[NP * PLANE];
     __shared__ __attribute__((aligned(16))) float kb[R];
+    __shared__ int alive[R];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
     const int b = blockIdx.y / p.Hkv, hk = blockIdx.y % p.Hkv, share = blockIdx.z;
     const int nrows = p.nq * p.G, klen = clamp_len(p.k_lens, b, p.nk), live_rows = clamp_len(p.q_lens, b, p.nq) * p.G;
@@ -431,22 +452,19 @@ __global__ __launch_bounds__(256, A::NP == 3 && DHP == 128 ? 1 : 2) void attn_fw
     for (int d = 0; d < DT; ++d) o[d] = zero16();
     float m = -INFINITY, l = 0.f;
     St st;
+    st.places(tid, p.dh, [&](int row, int64_t& ox, int64_t& oy) { ox = row * p.ks[1]; oy = row * p.vs[1]; });
     int keep = 0;
     auto fetch = [&](int t) {
-        st.fetch(tid, p.dh, [&](int row, const T*& px, const T*& py) {
-            const int key = t * R + row;
-            px = kbase + key * p.ks[1];
-            py = vbase + key * p.vs[1];
-            return key < klen;
-        }, [&](int row) { return mask ? (int)mask[t * R + row] : 1; });
-        if (tid < R) { const int key = t * R + tid; keep = key < klen ? (mask ? (int)mask[key] : 1) : 0; }
+        const int left = klen - t * R;
+        st.fetch(tid, kbase + t * R * p.ks[1], vbase + t * R * p.vs[1], left);
+        if (tid < R) keep = tid < left ? (mask ? (int)mask[t * R + tid] : 1) : 0;
     };
-    auto exists = [](int flag) { return flag != 0; };
     if (t0 < t1) fetch(t0);
     for (int t = t0; t < t1; ++t) {
         __syncthreads();
-        st.store(tid, Ks, Vs, fk, fv, exists);
-        if (tid < R) kb[tid] = keep ? 0.f : -INFINITY;
+        if (tid < R) { alive[tid] = keep; kb[tid] = keep ? 0.f : -INFINITY; }
+        if (mask) __syncthreads();
+        st.store(tid, Ks, Vs, fk, fv, mask ? alive : nullptr);
         __syncthreads();
         if (t + 1 < t1) fetch(t + 1);
         f32x16 s[NT];
@@ -590,6 +608,7 @@ __global__ __launch_bounds__(256, A::NP > 1 && DHP == 128 ? 1 : 2) void attn_dq_
     constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32;
     __shared__ __attribute__((aligned(16))) E Ks[NP * PLANE], Vs[NP * PLANE];
     __shared__ __attribute__((aligned(16))) float kb[R];
+    __shared__ int alive[R];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
     const int b = blockIdx.y / p.Hkv, hk = blockIdx.y % p.Hkv, share = blockIdx.z;
     const int nrows = p.nq * p.G, klen = clamp_len(p.k_lens, b, p.nk), live_rows = clamp_len(p.q_lens, b, p.nq) * p.G;
@@ -622,22 +641,19 @@ __global__ __launch_bounds__(256, A::NP > 1 && DHP == 128 ? 1 : 2) void attn_dq_
 #pragma unroll
     for (int d = 0; d < DT; ++d) dq[d] = zero16();
     St st;
+    st.places(tid, p.dh, [&](int row, int64_t& ox, int64_t& oy) { ox = row * p.ks[1]; oy = row * p.vs[1]; });
     int keep = 0;
     auto fetch = [&](int t) {
-        st.fetch(tid, p.dh, [&](int row, const T*& px, const T*& py) {
-            const int key = t * R + row;
-            px = kbase + key * p.ks[1];
-            py = vbase + key * p.vs[1];
-            return key < klen;
-        }, [&](int row) { return mask ? (int)mask[t * R + row] : 1; });
-        if (tid < R) { const int key = t * R + tid; keep = key < klen ? (mask ? (int)mask[key] : 1) : 0; }
+        const int left = klen - t * R;
+        st.fetch(tid, kbase + t * R * p.ks[1], vbase + t * R * p.vs[1], left);
+        if (tid < R) keep = tid < left ? (mask ? (int)mask[t * R + tid] : 1) : 0;
     };
-    auto exists = [](int flag) { return flag != 0; };
     if (t0 < t1) fetch(t0);
     for (int t = t0; t < t1; ++t) {
         __syncthreads();
-        st.store(tid, Ks, Vs, fk, fv, exists);
-        if (tid < R) kb[tid] = keep ? 0.f : -INFINITY;
+        if (tid < R) { alive[tid] = keep; kb[tid] = keep ? 0.f : -INFINITY; }
+        if (mask) __syncthreads();
+        st.store(tid, Ks, Vs, fk, fv, mask ? alive : nullptr);
         __syncthreads();
         if (t + 1 < t1) fetch(t + 1);
 #pragma unroll
@@ -718,6 +734,7 @@ __global__ __launch_bounds__(256, DHP == 128 || (A::NP == 3 && DHP == 64) ? 1 : 
     constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32;
     __shared__ __attribute__((aligned(16))) E Qs[NP * PLANE], Os[NP * PLANE];
     __shared__ __attribute__((aligned(16))) float refs[R], deltas[R];
+    __shared__ int alive[R];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
     const int b = blockIdx.y / p.Hkv, hk = blockIdx.y % p.Hkv, share = blockIdx.z;
     const int klen = clamp_len(p.k_lens, b, p.nk), live_rows = clamp_len(p.q_lens, b, p.nq) * p.G;
@@ -741,13 +758,22 @@ __global__ __launch_bounds__(256, DHP == 128 || (A::NP == 3 && DHP == 64) ? 1 : 
     for (int d = 0; d < DT; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
     St st;
     float ref = -INFINITY, delta = 0.f;
+    const bool check = p.mask || p.k_lens;       // otherwise every row has a key
+    const T *qbase = (const T*)p.q + b * p.qs[0] + (int64_t)hk * p.G * p.qs[2], *obase = (const T*)p.dout + ((int64_t)b * p.nq * p.H + hk * p.G) * p.dh;
+    // a tile's rows relative to query q0: the same for every tile where G divides R, else looked up per tile
+    auto places = [&](int r0, int q0) {
+        st.places(tid, p.dh, [&](int row, int64_t& ox, int64_t& oy) {
+            const int q = query_of(p, r0 + row), g = r0 + row - q * p.G;
+            ox = (q - q0) * p.qs[1] + g * p.qs[2];
+            oy = (int64_t)((q - q0) * p.H + g) * p.dh;
+        });
+    };
+    const bool regular = p.gshift >= 0 && p.G <= R;
+    places(0, 0);
     auto fetch = [&](int t) {
-        st.fetch(tid, p.dh, [&](int row, const T*& px, const T*& py) {
-            const int r = t * R + row;
-            px = (const T*)p.q + q_row(p, p.qs, b, hk, r);
-            py = (const T*)p.dout + dense_row(p, b, hk, r) * p.dh;
-            return r < live_rows;
-        }, [&](int row) { return __builtin_bit_cast(int, p.lse[stat_row(p, b, hk, t * R + row)]); });
+        const int left = live_rows - t * R, q0 = query_of(p, t * R);
+        if (!regular) places(t * R, q0);
+        st.fetch(tid, qbase + q0 * p.qs[1], obase + (int64_t)q0 * p.H * p.dh, left);
         if (tid < R) {
             const int r = t * R + tid;
             ref = -INFINITY;
@@ -758,16 +784,16 @@ __global__ __launch_bounds__(256, DHP == 128 || (A::NP == 3 && DHP == 64) ? 1 : 
             }
         }
     };
-    // chunks past the tensors are zeros already, whatever their flag
-    auto exists = [](int flag) { return __builtin_bit_cast(float, flag) != -INFINITY; };
     if (t0 < t1) fetch(t0);
     for (int t = t0; t < t1; ++t) {
         __syncthreads();
-        st.store(tid, Qs, Os, fq, fo, exists);
         if (tid < R) {
+            alive[tid] = ref != -INFINITY;
             refs[tid] = row_ref(ref) - A::SHIFT;
             deltas[tid] = ref == -INFINITY ? 0.f : delta;
         }
+        if (check) __syncthreads();
+        st.store(tid, Qs, Os, fq, fo, check ? alive : nullptr);
         __syncthreads();
         if (t + 1 < t1) fetch(t + 1);
 #pragma unroll
@@ -829,6 +855,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
     constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = 2;
     __shared__ __attribute__((aligned(16))) E Qs[PLANE], Os[PLANE];
     __shared__ __attribute__((aligned(16))) float refs[R], deltas[R];
+    __shared__ int alive[R];
     __shared__ __attribute__((aligned(16))) V hand[4][4][64];
     __shared__ float largest[4][32];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6, h = wave & 1;
@@ -850,13 +877,22 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
     for (int d = 0; d < DT; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
     St st;
     float ref = -INFINITY, delta = 0.f;
+    const bool check = p.mask || p.k_lens;       // otherwise every row has a key
+    const T *qbase = (const T*)p.q + b * p.qs[0] + (int64_t)hk * p.G * p.qs[2], *obase = (const T*)p.dout + ((int64_t)b * p.nq * p.H + hk * p.G) * p.dh;
+    // a tile's rows relative to query q0: the same for every tile where G divides R, else looked up per tile
+    auto places = [&](int r0, int q0) {
+        st.places(tid, p.dh, [&](int row, int64_t& ox, int64_t& oy) {
+            const int q = query_of(p, r0 + row), g = r0 + row - q * p.G;
+            ox = (q - q0) * p.qs[1] + g * p.qs[2];
+            oy = (int64_t)((q - q0) * p.H + g) * p.dh;
+        });
+    };
+    const bool regular = p.gshift >= 0 && p.G <= R;
+    places(0, 0);
     auto fetch = [&](int t) {
-        st.fetch(tid, p.dh, [&](int row, const T*& px, const T*& py) {
-            const int r = t * R + row;
-            px = (const T*)p.q + q_row(p, p.qs, b, hk, r);
-            py = (const T*)p.dout + dense_row(p, b, hk, r) * p.dh;
-            return r < live_rows;
-        }, [&](int row) { return __builtin_bit_cast(int, p.lse[stat_row(p, b, hk, t * R + row)]); });
+        const int left = live_rows - t * R, q0 = query_of(p, t * R);
+        if (!regular) places(t * R, q0);
+        st.fetch(tid, qbase + q0 * p.qs[1], obase + (int64_t)q0 * p.H * p.dh, left);
         if (tid < R) {
             const int r = t * R + tid;
             ref = -INFINITY;
@@ -867,7 +903,6 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
             }
         }
     };
-    auto exists = [](int flag) { return __builtin_bit_cast(float, flag) != -INFINITY; };
     auto sums = [&](int n, int k, V pk, V dsk) __attribute__((always_inline)) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
@@ -881,11 +916,13 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
     if (t0 < t1) fetch(t0);
     for (int t = t0; t < t1; ++t) {
         __syncthreads();
-        st.store(tid, Qs, Os, 1.f, 1.f, exists);
         if (tid < R) {
+            alive[tid] = ref != -INFINITY;
             refs[tid] = row_ref(ref) - A::SHIFT;
             deltas[tid] = ref == -INFINITY ? 0.f : delta;
         }
+        if (check) __syncthreads();
+        st.store(tid, Qs, Os, 1.f, 1.f, check ? alive : nullptr);
         __syncthreads();
         if (t + 1 < t1) fetch(t + 1);
         f32x16 s = first_product<A, KS, DHP, PLANE>(Qs, h, lane, kf);
@@ -991,6 +1028,11 @@ const char* bad_desc(const imp_attn_desc* d) {
     for (int i = 0; i < 3; ++i)
         if (d->q_stride[i] % unit || d->k_stride[i] % unit || d->v_stride[i] % unit || d->q_stride[i] < 0 || d->k_stride[i] < 0 || d->v_stride[i] < 0)
             return "strides must be multiples of 16 bytes";
+    // the 32-bit offsets within a tile of 64 rows
+    const int64_t most = ((int64_t)1 << 30) / (d->dtype == IMP_DTYPE_F32 ? 4 : 2);
+    if (d->q_stride[1] > most / 64 || d->k_stride[1] > most / 64 || d->v_stride[1] > most / 64 || d->q_stride[2] > most / (d->heads / d->kv_heads) ||
+        (int64_t)d->heads * d->head_dim > most / 64)
+        return "strides too large: 64 tokens, and the query heads of a key head, must lie within 2^30 bytes";
     return nullptr;
 }
 bool unaligned(std::initializer_list<const void*> ptrs) {

@@ -72,12 +72,16 @@ def _dense(t, dtype):
 # --------------------------------------------------------------------------------------------------------------------------- attention
 @functools.lru_cache(maxsize=1024)
 def _regular(shape, stride, size):
-    unit = 16 // size
-    return (shape[3] == 1 or stride[3] == 1) and all(shape[i] == 1 or (stride[i] % unit == 0 and stride[i] > 0) for i in range(3))
+    unit, most = 16 // size, (1 << 30) // size
+    if shape[3] != 1 and stride[3] != 1:
+        return False
+    if (shape[1] > 1 and stride[1] > most // 64) or (shape[2] > 1 and stride[2] > most // shape[2]):
+        return False
+    return all(shape[i] == 1 or (stride[i] % unit == 0 and stride[i] > 0) for i in range(3))
 
 
 def _rows(t):
-    """t [batch, tokens, heads, channels] as the kernels take it: channels contiguous, everything else in steps of 16 bytes (a copy if it is not)"""
+    """t [batch, tokens, heads, channels] as the kernels take it: channels contiguous, everything else in steps of 16 bytes that stay within their reach (a copy if not)"""
     if t.data_ptr() % 16 == 0 and _regular(t.shape, t.stride(), t.element_size()):
         return t
     t = t.contiguous()
