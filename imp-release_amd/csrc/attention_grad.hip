@@ -13,7 +13,7 @@
 // registers in exactly the order the second one takes its B operand (row 16 s + 8 (e / 4) + 4 half + e % 4 <-> register 8 s + e), and its A operand comes from
 // the SAME row-major LDS tile through the transpose read.  dQ recomputes S and dP (7 products backward instead of 5) so that no gradient is accumulated with
 // atomics: every sum has a fixed order and results repeat bit for bit.  Shared key heads: the G query heads of a key head are interleaved as rows
-// r = q G + g of one problem, so dK / dV sum over them in registers and one query of many heads still fills a tile.
+// r = q G + g of one problem where queries are owned (one query of many heads still fills a wave), and walked one after the other for dK / dV, which sum over them in registers.
 // Few rows: the walk is cut in shares (partials in the caller's workspace, joined in a fixed order by a second launch).
 //
 // Arithmetic (accumulators, softmax statistics and D in fp32; what the operands of the products are rounded to):
@@ -124,19 +124,24 @@ template <typename T> struct Chunk;
 template <> struct Chunk<float> {
     f32x4 a, b;
     __device__ void load(const float* p) { a = *(const f32x4*)p; b = *(const f32x4*)(p + 4); }
-    __device__ void load(__amdgpu_buffer_rsrc_t r, unsigned off) {
-        a = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
-        b = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off + 16, 0, 0));
+    __device__ void load(__amdgpu_buffer_rsrc_t r, unsigned off, unsigned soff) {
+        a = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, soff, 0));
+        b = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off + 16, soff, 0));
     }
     __device__ void zero() { a = f32x4{0, 0, 0, 0}; b = a; }
     __device__ void negate() { a = -a; b = -b; }
+    __device__ void keep(unsigned m) {       // all bits or none
+        a = __builtin_bit_cast(f32x4, __builtin_bit_cast(u32x4, a) & m);
+        b = __builtin_bit_cast(f32x4, __builtin_bit_cast(u32x4, b) & m);
+    }
     __device__ void get(float (&x)[8]) const { for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[i + 4] = b[i]; } }
 };
 template <typename T> struct Chunk16 {
     u32x4 a;
     __device__ void load(const T* p) { a = *(const u32x4*)p; }
-    __device__ void load(__amdgpu_buffer_rsrc_t r, unsigned off) { a = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0); }
+    __device__ void load(__amdgpu_buffer_rsrc_t r, unsigned off, unsigned soff) { a = __builtin_amdgcn_raw_buffer_load_b128(r, off, soff, 0); }
     __device__ void zero() { a = u32x4{0, 0, 0, 0}; }
+    __device__ void keep(unsigned m) { a &= m; }
     __device__ void negate() { a ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u}; }
     __device__ void get(float (&x)[8]) const {
         const auto v = __builtin_bit_cast(typename Vec8<T>::type, a);
@@ -233,43 +238,40 @@ __device__ __forceinline__ void load_owned(const T* row, bool live, int dh, int 
 }
 
 constexpr unsigned OUTSIDE = 0x80000000u;    // an offset past the end of a buffer descriptor: the load returns zeros
-// One tile of the walked side: 256 threads fetch R rows x DHP columns of two matrices into registers, and store them as planes.  A thread's places within a tile are 32-bit
-// offsets; a buffer descriptor moves with the tile, and rows and channels that do not exist are offsets past its end.  Nothing is waited for between.  Rows inside the tensors
-// that do not count (masked keys, queries without a key) become zeros on the way to LDS.
+// One tile of the walked side: 256 threads fetch R rows x DHP columns of two matrices into registers, and store them as planes.  A thread's place within a tile is one 32-bit
+// offset per matrix; a buffer descriptor moves with the tile, and rows and channels that do not exist are offsets past its end.  Nothing is waited for between.  Rows inside
+// the tensors that do not count (masked keys, queries without a key) become zeros on the way to LDS.
 template <typename T, typename E, int NP, int DHP, int R>
 struct Stage {
-    static constexpr int CPR = DHP / 8, N = (R * CPR + 255) / 256, PLANE = R * DHP;
+    static constexpr int CPR = DHP / 8, N = (R * CPR + 255) / 256, PLANE = R * DHP, STEP = 256 / CPR;
     Chunk<T> x[N], y[N];
-    unsigned xo[N], yo[N];
-    // offs(row, x, y): element offsets of a tile's row in both matrices
-    template <typename F> __device__ void places(int tid, int dh, F offs) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = tid + 256 * i, row = c / CPR, col = (c % CPR) * 8;
-            int64_t ox, oy;
-            offs(row, ox, oy);
-            const bool in = row < R && col < dh;
-            xo[i] = in ? (unsigned)((ox + col) * (int64_t)sizeof(T)) : OUTSIDE;
-            yo[i] = in ? (unsigned)((oy + col) * (int64_t)sizeof(T)) : OUTSIDE;
-        }
+    unsigned xo, yo;                     // this thread's chunk of the first STEP rows
+    // row strides of both matrices in elements
+    __device__ void places(int tid, int dh, int64_t xs, int64_t ys) {
+        const int row = tid / CPR, col = tid % CPR * 8;
+        const bool in = row < R && col < dh;
+        xo = in ? (unsigned)((row * xs + col) * (int64_t)sizeof(T)) : OUTSIDE;
+        yo = in ? (unsigned)((row * ys + col) * (int64_t)sizeof(T)) : OUTSIDE;
     }
     // the tile at px, py, of which `left` rows exist
-    __device__ void fetch(int tid, const T* px, const T* py, int left) {
+    __device__ void fetch(int tid, const T* px, const T* py, int64_t xs, int64_t ys, int left) {
         const auto rx = __builtin_amdgcn_make_buffer_rsrc((void*)px, 0, 0x7fffff00, 0x27000), ry = __builtin_amdgcn_make_buffer_rsrc((void*)py, 0, 0x7fffff00, 0x27000);
+        const int row = tid / CPR;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const bool in = (tid + 256 * i) / CPR < left;
-            x[i].load(rx, in ? xo[i] : OUTSIDE);
-            y[i].load(ry, in ? yo[i] : OUTSIDE);
+            const bool in = row + STEP * i < left;
+            x[i].load(rx, in ? xo : OUTSIDE, (unsigned)(STEP * i * xs * (int64_t)sizeof(T)));
+            y[i].load(ry, in ? yo : OUTSIDE, (unsigned)(STEP * i * ys * (int64_t)sizeof(T)));
         }
     }
-    // alive: which of the tile's rows count (LDS), or null
-    __device__ void store(int tid, E* X, E* Y, float fx, float fy, const int* alive) {
-        if (alive) {
+    // alive: which of the tile's rows count (LDS; all bits or none)
+    template <bool CHECK> __device__ void store(int tid, E* X, E* Y, float fx, float fy, const unsigned* alive) {
+        if constexpr (CHECK) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const int row = (tid + 256 * i) / CPR;
-                if (row < R && !alive[row]) { x[i].zero(); y[i].zero(); }
+                const unsigned m = alive[min((tid + 256 * i) / CPR, R - 1)];
+                x[i].keep(m);
+                y[i].keep(m);
             }
         }
 #pragma unroll
@@ -288,34 +290,35 @@ struct Stage {
     }
 };
 
-__device__ __forceinline__ f32x16 zero16();
-// the first product of a 32 x 32 sub-tile: rows of `tile` times the owned rows.  Over all k-steps the small products come first and hi . hi last: the sum is rounded once
-// per k-step at its full size, not once per product - what dS = P (dP - D) keeps after the cancellation is decided here
-template <typename A, int KS, int DHP, int PLANE>
-__device__ __forceinline__ f32x16 first_product(const typename A::E* tile, int sub, int lane, const typename A::V (&own)[KS][A::NP]) {
-    using V = typename A::V;
-    f32x16 c = zero16();
-    V hi[KS];
+// The operands of the matrix instructions are read from LDS a group ahead of their use (about 130 cycles of latency; left to itself the compiler waits for every read right
+// after it): GROUP operands, 16 registers of one plane or of two, are under way while the previous group is multiplied.
+template <int NP, int KS> constexpr int group_of() { return NP == 1 ? (KS < 4 ? KS : 4) : NP == 2 ? 2 : 1; }
+template <typename A, int KS> struct Group { typename A::V f[group_of<A::NP, KS>()][A::NP]; };
+
+// k-steps [k0, k0 + GROUP) of a first product (32 walked rows x the owned ones).  Small products first: a score is rounded less often at its full size - what
+// dS = P (dP - D) keeps after the cancellation is decided here
+template <typename A, int KS>
+__device__ __forceinline__ void first_product(const Group<A, KS>& g, const typename A::V (&own)[KS][A::NP], int k0, f32x16& c) {
+    constexpr int N = group_of<A::NP, KS>();
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-        V f[A::NP];
-        read_rows<typename A::E, A::NP, DHP, PLANE>(tile, sub, k, lane, f);
+    for (int j = 0; j < N; ++j) {
         if constexpr (A::NP == 3) {
-            c = mfma(f[1], own[k][1], c);
-            c = mfma(f[0], own[k][2], c);
-            c = mfma(f[2], own[k][0], c);
+            c = mfma(g.f[j][1], own[k0 + j][1], c);
+            c = mfma(g.f[j][0], own[k0 + j][2], c);
+            c = mfma(g.f[j][2], own[k0 + j][0], c);
         }
         if constexpr (A::NP >= 2) {
-            c = mfma(f[0], own[k][1], c);
-            c = mfma(f[1], own[k][0], c);
-            hi[k] = f[0];
-        } else c = mfma(f[0], own[k][0], c);
+            c = mfma(g.f[j][0], own[k0 + j][1], c);
+            c = mfma(g.f[j][1], own[k0 + j][0], c);
+        }
     }
-    if constexpr (A::NP >= 2) {
 #pragma unroll
-        for (int k = 0; k < KS; ++k) c = mfma(hi[k], own[k][0], c);
-    }
-    return c;
+    for (int j = 0; j < N; ++j) c = mfma(g.f[j][0], own[k0 + j][0], c);
+}
+template <typename A, int KS, int DHP, int PLANE>
+__device__ __forceinline__ void read_group_rows(const typename A::E* tile, int sub, int k0, int lane, Group<A, KS>& g) {
+#pragma unroll
+    for (int j = 0; j < group_of<A::NP, KS>(); ++j) read_rows<typename A::E, A::NP, DHP, PLANE>(tile, sub, k0 + j, lane, g.f[j]);
 }
 
 __device__ __forceinline__ f32x16 zero16() {
@@ -418,17 +421,18 @@ __global__ __launch_bounds__(256) void attn_amax_kernel(AttnOp p) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------- forward
-template <typename A, int DHP>
+template <typename A, int DHP, bool CHECK>
 __global__ __launch_bounds__(256, A::NP == 3 && DHP == 128 ? 1 : 2) void attn_fwd_kernel(AttnOp p) {
     using T = typename A::T;
     using E = typename A::E;
     using V = typename A::V;
     constexpr int NP = A::NP, R = A::R;
     using St = Stage<T, E, NP, DHP, R>;
-    constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32;
+    constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32, GN = group_of<NP, KS>(), SG = KS / GN, PG = 2 * DT / GN;
+    constexpr bool PIPE = true;
     __shared__ __attribute__((aligned(16))) E Ks[NP * PLANE], Vs[NP * PLANE];
     __shared__ __attribute__((aligned(16))) float kb[R];
-    __shared__ int alive[R];
+    __shared__ unsigned alive[R];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
     const int b = blockIdx.y / p.Hkv, hk = blockIdx.y % p.Hkv, share = blockIdx.z;
     const int nrows = p.nq * p.G, klen = clamp_len(p.k_lens, b, p.nk), live_rows = clamp_len(p.q_lens, b, p.nq) * p.G;
@@ -444,7 +448,7 @@ __global__ __launch_bounds__(256, A::NP == 3 && DHP == 128 ? 1 : 2) void attn_fw
     load_owned<T, E, NP, DHP>((const T*)p.q + (live ? q_row(p, p.qs, b, hk, r) : 0), live, p.dh, half, fq, qf, p.scale < 0.f);
     const T* kbase = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
     const T* vbase = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
-    const uint8_t* mask = p.mask ? p.mask + (int64_t)b * p.nk : nullptr;
+    const uint8_t* mask = CHECK ? p.mask + (int64_t)b * p.nk : nullptr;
     const float c = score_unit(p.scale, fq, fk);
 
     f32x16 o[DT];
@@ -452,27 +456,46 @@ __global__ __launch_bounds__(256, A::NP == 3 && DHP == 128 ? 1 : 2) void attn_fw
     for (int d = 0; d < DT; ++d) o[d] = zero16();
     float m = -INFINITY, l = 0.f;
     St st;
-    st.places(tid, p.dh, [&](int row, int64_t& ox, int64_t& oy) { ox = row * p.ks[1]; oy = row * p.vs[1]; });
+    st.places(tid, p.dh, p.ks[1], p.vs[1]);
     int keep = 0;
     auto fetch = [&](int t) {
         const int left = klen - t * R;
-        st.fetch(tid, kbase + t * R * p.ks[1], vbase + t * R * p.vs[1], left);
+        st.fetch(tid, kbase + t * R * p.ks[1], vbase + t * R * p.vs[1], p.ks[1], p.vs[1], left);
         if (tid < R) keep = tid < left ? (mask ? (int)mask[t * R + tid] : 1) : 0;
     };
     if (t0 < t1) fetch(t0);
     for (int t = t0; t < t1; ++t) {
         __syncthreads();
-        if (tid < R) { alive[tid] = keep; kb[tid] = keep ? 0.f : -INFINITY; }
-        if (mask) __syncthreads();
-        st.store(tid, Ks, Vs, fk, fv, mask ? alive : nullptr);
+        if (tid < R) { alive[tid] = keep ? ~0u : 0u; kb[tid] = keep ? 0.f : -INFINITY; }
+        if constexpr (CHECK) __syncthreads();
+        st.template store<CHECK>(tid, Ks, Vs, fk, fv, alive);
         __syncthreads();
         if (t + 1 < t1) fetch(t + 1);
+        // the stream of operand groups: the scores' of all sub-tiles, then the sums'
+        Group<A, KS> buf[2];
+        auto read = [&](int i) __attribute__((always_inline)) {
+            Group<A, KS>& g = buf[i & 1];
+            if (i < NT * SG) read_group_rows<A, KS, DHP, PLANE>(Ks, i / SG, i % SG * GN, lane, g);
+            else if (i < NT * (SG + PG)) {
+                const int n = (i - NT * SG) / PG, e0 = (i - NT * SG) % PG * GN;
+#pragma unroll
+                for (int j = 0; j < GN; ++j) read_cols<E, NP, DHP, PLANE>(Vs, n, (e0 + j) / DT, (e0 + j) % DT, lane, g.f[j]);
+            }
+        };
         f32x16 s[NT];
         float mx = -INFINITY;
+        read(0);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            s[n] = first_product<A, KS, DHP, PLANE>(Ks, n, lane, qf);
-            if (mask || (t + 1) * R > klen) add_rows(s[n], kb + 32 * n, half);
+            s[n] = zero16();
+#pragma unroll
+            for (int i = 0; i < SG; ++i) {
+                read(n * SG + i + 1);
+                if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
+                first_product<A, KS>(buf[(n * SG + i) & 1], qf, i * GN, s[n]);
+                if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
+            }
+            if (CHECK || (t + 1) * R > klen) add_rows(s[n], kb + 32 * n, half);
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
         }
@@ -493,16 +516,17 @@ __global__ __launch_bounds__(256, A::NP == 3 && DHP == 128 ? 1 : 2) void attn_fw
                 s[n][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], c, ref));
                 l += s[n][i];
             }
+            V pf[2][NP];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                V pf[NP];
-                pack<NP, E>(s[n], k, pf);
+            for (int k = 0; k < 2; ++k) pack<NP, E>(s[n], k, pf[k]);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    V f[NP];
-                    read_cols<E, NP, DHP, PLANE>(Vs, n, k, d, lane, f);
-                    o[d] = mfma_planes<NP, V>(f, pf, o[d]);
-                }
+            for (int i = 0; i < PG; ++i) {
+                const int at = NT * SG + n * PG + i;
+                read(at + 1);
+                if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < GN; ++j) o[(i * GN + j) % DT] = mfma_planes<NP, V>(buf[at & 1].f[j], pf[(i * GN + j) / DT], o[(i * GN + j) % DT]);
+                if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
@@ -598,17 +622,18 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(AttnOp p) {
 // the exponent reference of a row: lse in log2 units, +inf (P = 0) for rows that do not exist or have no key
 __device__ __forceinline__ float row_ref(float lse) { return lse == -INFINITY ? INFINITY : lse * LOG2E; }
 
-template <typename A, int DHP>
+template <typename A, int DHP, bool CHECK>
 __global__ __launch_bounds__(256, A::NP > 1 && DHP == 128 ? 1 : 2) void attn_dq_kernel(AttnOp p) {
     using T = typename A::T;
     using E = typename A::E;
     using V = typename A::V;
     constexpr int NP = A::NP, R = A::R;
     using St = Stage<T, E, NP, DHP, R>;
-    constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32;
+    constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32, GN = group_of<NP, KS>(), SG = KS / GN, PG = 2 * DT / GN;
+    constexpr bool PIPE = !(DHP == 128 && NP == 1);      // no registers are left for it there
     __shared__ __attribute__((aligned(16))) E Ks[NP * PLANE], Vs[NP * PLANE];
     __shared__ __attribute__((aligned(16))) float kb[R];
-    __shared__ int alive[R];
+    __shared__ unsigned alive[R];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
     const int b = blockIdx.y / p.Hkv, hk = blockIdx.y % p.Hkv, share = blockIdx.z;
     const int nrows = p.nq * p.G, klen = clamp_len(p.k_lens, b, p.nk), live_rows = clamp_len(p.q_lens, b, p.nq) * p.G;
@@ -634,49 +659,71 @@ __global__ __launch_bounds__(256, A::NP > 1 && DHP == 128 ? 1 : 2) void attn_dq_
     load_owned<T, E, NP, DHP>((const T*)p.dout + (live ? dense_row(p, b, hk, r) * p.dh : 0), live, p.dh, half, fo, of);
     const T* kbase = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
     const T* vbase = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
-    const uint8_t* mask = p.mask ? p.mask + (int64_t)b * p.nk : nullptr;
+    const uint8_t* mask = CHECK ? p.mask + (int64_t)b * p.nk : nullptr;
     const float c = score_unit(p.scale, fq, fk), cd = (1.f / fo) * (1.f / fv);
     LaneScale ls;
     f32x16 dq[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) dq[d] = zero16();
     St st;
-    st.places(tid, p.dh, [&](int row, int64_t& ox, int64_t& oy) { ox = row * p.ks[1]; oy = row * p.vs[1]; });
+    st.places(tid, p.dh, p.ks[1], p.vs[1]);
     int keep = 0;
     auto fetch = [&](int t) {
         const int left = klen - t * R;
-        st.fetch(tid, kbase + t * R * p.ks[1], vbase + t * R * p.vs[1], left);
+        st.fetch(tid, kbase + t * R * p.ks[1], vbase + t * R * p.vs[1], p.ks[1], p.vs[1], left);
         if (tid < R) keep = tid < left ? (mask ? (int)mask[t * R + tid] : 1) : 0;
     };
     if (t0 < t1) fetch(t0);
     for (int t = t0; t < t1; ++t) {
         __syncthreads();
-        if (tid < R) { alive[tid] = keep; kb[tid] = keep ? 0.f : -INFINITY; }
-        if (mask) __syncthreads();
-        st.store(tid, Ks, Vs, fk, fv, mask ? alive : nullptr);
+        if (tid < R) { alive[tid] = keep ? ~0u : 0u; kb[tid] = keep ? 0.f : -INFINITY; }
+        if constexpr (CHECK) __syncthreads();
+        st.template store<CHECK>(tid, Ks, Vs, fk, fv, alive);
         __syncthreads();
         if (t + 1 < t1) fetch(t + 1);
+        // per sub-tile: operand groups of the scores, of dP, of the sums
+        constexpr int ALL = 2 * SG + PG;
+        Group<A, KS> buf[2];
+        auto read = [&](int n, int i) __attribute__((always_inline)) {
+            if (i == ALL) { ++n; i = 0; }
+            if (n == NT) return;
+            Group<A, KS>& g = buf[(n * ALL + i) & 1];
+            if (i < SG) read_group_rows<A, KS, DHP, PLANE>(Ks, n, i * GN, lane, g);
+            else if (i < 2 * SG) read_group_rows<A, KS, DHP, PLANE>(Vs, n, (i - SG) * GN, lane, g);
+            else {
+#pragma unroll
+                for (int j = 0; j < GN; ++j) { const int e = (i - 2 * SG) * GN + j; read_cols<E, NP, DHP, PLANE>(Ks, n, e / DT, e % DT, lane, g.f[j]); }
+            }
+        };
+        if (PIPE) read(0, 0);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            f32x16 s = first_product<A, KS, DHP, PLANE>(Ks, n, lane, qf);
-            const f32x16 dp = first_product<A, KS, DHP, PLANE>(Vs, n, lane, of);
-            if (mask || (t + 1) * R > klen) add_rows(s, kb + 32 * n, half);
+            f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+            for (int i = 0; i < 2 * SG; ++i) {
+                read(n, PIPE ? i + 1 : i);
+                if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
+                if (i < SG) first_product<A, KS>(buf[(n * ALL + i) & 1], qf, i * GN, s);
+                else first_product<A, KS>(buf[(n * ALL + i) & 1], of, (i - SG) * GN, dp);
+                if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
+            }
+            if (CHECK || (t + 1) * R > klen) add_rows(s, kb + 32 * n, half);
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ref)) * __builtin_fmaf(dp[i], cd, -delta);
             if constexpr (A::LANE) {
                 ls.step(s, dq);
                 s *= ls.f;
             }
+            V df[2][NP];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                V df[NP];
-                pack<NP, E>(s, k, df);
+            for (int k = 0; k < 2; ++k) pack<NP, E>(s, k, df[k]);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    V f[NP];
-                    read_cols<E, NP, DHP, PLANE>(Ks, n, k, d, lane, f);
-                    dq[d] = mfma_planes<NP, V>(f, df, dq[d]);
-                }
+            for (int i = 2 * SG; i < ALL; ++i) {
+                read(n, PIPE ? i + 1 : i);
+                if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < GN; ++j) { const int e = (i - 2 * SG) * GN + j; dq[e % DT] = mfma_planes<NP, V>(buf[(n * ALL + i) & 1].f[j], df[e / DT], dq[e % DT]); }
+                if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
@@ -724,23 +771,24 @@ __device__ __forceinline__ void store_dkv(const AttnOp& p, int b, int hk, int ke
         }
 }
 
-template <typename A, int DHP>
+template <typename A, int DHP, bool CHECK>
 __global__ __launch_bounds__(256, DHP == 128 || (A::NP == 3 && DHP == 64) ? 1 : 2) void attn_dkv_kernel(AttnOp p) {
     using T = typename A::T;
     using E = typename A::E;
     using V = typename A::V;
     constexpr int NP = A::NP, R = A::R;
     using St = Stage<T, E, NP, DHP, R>;
-    constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32;
+    constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32, GN = group_of<NP, KS>(), SG = KS / GN, PG = 2 * DT / GN;
+    constexpr bool PIPE = !(DHP == 64 && NP == 2);
     __shared__ __attribute__((aligned(16))) E Qs[NP * PLANE], Os[NP * PLANE];
     __shared__ __attribute__((aligned(16))) float refs[R], deltas[R];
-    __shared__ int alive[R];
+    __shared__ unsigned alive[R];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6;
     const int b = blockIdx.y / p.Hkv, hk = blockIdx.y % p.Hkv, share = blockIdx.z;
-    const int klen = clamp_len(p.k_lens, b, p.nk), live_rows = clamp_len(p.q_lens, b, p.nq) * p.G;
+    const int klen = clamp_len(p.k_lens, b, p.nk), qlen = clamp_len(p.q_lens, b, p.nq), per_head = (qlen + R - 1) / R;
     const int own0 = blockIdx.x * OWN, key = own0 + 32 * wave + (lane & 31);
     const bool live = key < klen && (!p.mask || p.mask[(int64_t)b * p.nk + key]);
-    const int tiles = (live_rows + R - 1) / R;
+    const int tiles = per_head * p.G;
     int t0 = 0, t1 = own0 < klen ? tiles : 0;
     if (p.shares > 1 && t1) { t0 = (int)((int64_t)tiles * share / p.shares); t1 = (int)((int64_t)tiles * (share + 1) / p.shares); }
 
@@ -758,55 +806,72 @@ __global__ __launch_bounds__(256, DHP == 128 || (A::NP == 3 && DHP == 64) ? 1 : 
     for (int d = 0; d < DT; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
     St st;
     float ref = -INFINITY, delta = 0.f;
-    const bool check = p.mask || p.k_lens;       // otherwise every row has a key
+    // the walk: query head by query head of the key head, R of its queries at a time
     const T *qbase = (const T*)p.q + b * p.qs[0] + (int64_t)hk * p.G * p.qs[2], *obase = (const T*)p.dout + ((int64_t)b * p.nq * p.H + hk * p.G) * p.dh;
-    // a tile's rows relative to query q0: the same for every tile where G divides R, else looked up per tile
-    auto places = [&](int r0, int q0) {
-        st.places(tid, p.dh, [&](int row, int64_t& ox, int64_t& oy) {
-            const int q = query_of(p, r0 + row), g = r0 + row - q * p.G;
-            ox = (q - q0) * p.qs[1] + g * p.qs[2];
-            oy = (int64_t)((q - q0) * p.H + g) * p.dh;
-        });
-    };
-    const bool regular = p.gshift >= 0 && p.G <= R;
-    places(0, 0);
-    auto fetch = [&](int t) {
-        const int left = live_rows - t * R, q0 = query_of(p, t * R);
-        if (!regular) places(t * R, q0);
-        st.fetch(tid, qbase + q0 * p.qs[1], obase + (int64_t)q0 * p.H * p.dh, left);
+    st.places(tid, p.dh, p.qs[1], (int64_t)p.H * p.dh);
+    int g = t0 / (per_head ? per_head : 1), q0 = (t0 - g * per_head) * R;
+    auto fetch = [&]() {
+        const int left = qlen - q0;
+        st.fetch(tid, qbase + g * p.qs[2] + q0 * p.qs[1], obase + ((int64_t)q0 * p.H + g) * p.dh, p.qs[1], (int64_t)p.H * p.dh, left);
         if (tid < R) {
-            const int r = t * R + tid;
             ref = -INFINITY;
-            if (r < live_rows) {
-                const int64_t at = stat_row(p, b, hk, r);
+            if (tid < left) {
+                const int64_t at = ((int64_t)b * p.H + hk * p.G + g) * p.nq + q0 + tid;
                 ref = p.lse[at];
                 delta = p.delta[at];
             }
         }
+        q0 += R;
+        if (q0 >= qlen) { q0 = 0; ++g; }
     };
-    if (t0 < t1) fetch(t0);
+    if (t0 < t1) fetch();
     for (int t = t0; t < t1; ++t) {
         __syncthreads();
         if (tid < R) {
-            alive[tid] = ref != -INFINITY;
+            alive[tid] = ref != -INFINITY ? ~0u : 0u;
             refs[tid] = row_ref(ref) - A::SHIFT;
             deltas[tid] = ref == -INFINITY ? 0.f : delta;
         }
-        if (check) __syncthreads();
-        st.store(tid, Qs, Os, fq, fo, check ? alive : nullptr);
+        if constexpr (CHECK) __syncthreads();
+        st.template store<CHECK>(tid, Qs, Os, fq, fo, alive);
         __syncthreads();
-        if (t + 1 < t1) fetch(t + 1);
+        if (t + 1 < t1) fetch();
+        // per sub-tile: operand groups of the scores, of dP, of both sums (dV's and dK's in turn)
+        constexpr int ALL = 2 * SG + 2 * PG;
+        Group<A, KS> buf[2];
+        auto read = [&](int n, int i) __attribute__((always_inline)) {
+            if (i == ALL) { ++n; i = 0; }
+            if (n == NT) return;
+            Group<A, KS>& g = buf[(n * ALL + i) & 1];
+            if (i < SG) read_group_rows<A, KS, DHP, PLANE>(Qs, n, i * GN, lane, g);
+            else if (i < 2 * SG) read_group_rows<A, KS, DHP, PLANE>(Os, n, (i - SG) * GN, lane, g);
+            else {
+#pragma unroll
+                for (int j = 0; j < GN; ++j) {
+                    const int e = (i - 2 * SG) * GN + j;
+                    read_cols<E, NP, DHP, PLANE>(e & 1 ? Qs : Os, n, e / (2 * DT), e / 2 % DT, lane, g.f[j]);
+                }
+            }
+        };
+        if (PIPE) read(0, 0);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            f32x16 s = first_product<A, KS, DHP, PLANE>(Qs, n, lane, kf);
-            f32x16 dp = first_product<A, KS, DHP, PLANE>(Os, n, lane, vf);
+            f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+            for (int i = 0; i < 2 * SG; ++i) {
+                read(n, PIPE ? i + 1 : i);
+                if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
+                if (i < SG) first_product<A, KS>(buf[(n * ALL + i) & 1], kf, i * GN, s);
+                else first_product<A, KS>(buf[(n * ALL + i) & 1], vf, (i - SG) * GN, dp);
+                if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const f32x4 ref = *(const f32x4*)(refs + 32 * n + 8 * g + 4 * half);
+                const f32x4 rv = *(const f32x4*)(refs + 32 * n + 8 * g + 4 * half);
                 const f32x4 dl = *(const f32x4*)(deltas + 32 * n + 8 * g + 4 * half);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], c, -ref[i]));
+                    const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], c, -rv[i]));
                     s[4 * g + i] = pr;
                     dp[4 * g + i] = pr * __builtin_fmaf(dp[4 * g + i], cd, -dl[i]);
                 }
@@ -815,19 +880,23 @@ __global__ __launch_bounds__(256, DHP == 128 || (A::NP == 3 && DHP == 64) ? 1 : 
                 ls.step(dp, dk);
                 dp *= ls.f;
             }
+            V pf[2][NP], df[2][NP];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                V pf[NP], df[NP];
-                pack<NP, E>(s, k, pf);
-                pack<NP, E>(dp, k, df);
+                pack<NP, E>(s, k, pf[k]);
+                pack<NP, E>(dp, k, df[k]);
+            }
 #pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    V f[NP];
-                    read_cols<E, NP, DHP, PLANE>(Os, n, k, d, lane, f);
-                    dv[d] = mfma_planes<NP, V>(f, pf, dv[d]);
-                    read_cols<E, NP, DHP, PLANE>(Qs, n, k, d, lane, f);
-                    dk[d] = mfma_planes<NP, V>(f, df, dk[d]);
+            for (int i = 2 * SG; i < ALL; ++i) {
+                read(n, PIPE ? i + 1 : i);
+                if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < GN; ++j) {
+                    const int e = (i - 2 * SG) * GN + j, k = e / (2 * DT), d = e / 2 % DT;
+                    if (e & 1) dk[d] = mfma_planes<NP, V>(buf[(n * ALL + i) & 1].f[j], df[k], dk[d]);
+                    else dv[d] = mfma_planes<NP, V>(buf[(n * ALL + i) & 1].f[j], pf[k], dv[d]);
                 }
+                if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
@@ -844,7 +913,7 @@ __global__ __launch_bounds__(256, DHP == 128 || (A::NP == 3 && DHP == 64) ? 1 : 
 // dK / dV for 128 channels in 16-bit types: 128 fp32 accumulators and 64 registers of operands leave a wave of the kernel above alone on its SIMD.  Here two waves share 32 keys:
 // wave h computes the scores of the h-th 32 rows of a tile, hands P and dS on through LDS (in the operand layout they are used in), and sums its half of the channels over
 // both.  No product is computed twice; 64 accumulators, two waves per SIMD.
-template <typename A>
+template <typename A, bool CHECK>
 __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
     using T = typename A::T;
     using E = typename A::E;
@@ -852,18 +921,19 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
     static_assert(A::NP == 1 && A::R == 64);
     constexpr int NP = 1, R = 64, DHP = 128;
     using St = Stage<T, E, NP, DHP, R>;
-    constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = 2;
+    constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = 2, GN = group_of<NP, KS>(), SG = KS / GN;
+    constexpr bool PIPE = false;
     __shared__ __attribute__((aligned(16))) E Qs[PLANE], Os[PLANE];
     __shared__ __attribute__((aligned(16))) float refs[R], deltas[R];
-    __shared__ int alive[R];
+    __shared__ unsigned alive[R];
     __shared__ __attribute__((aligned(16))) V hand[4][4][64];
     __shared__ float largest[4][32];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6, h = wave & 1;
     const int b = blockIdx.y / p.Hkv, hk = blockIdx.y % p.Hkv, share = blockIdx.z;
-    const int klen = clamp_len(p.k_lens, b, p.nk), live_rows = clamp_len(p.q_lens, b, p.nq) * p.G;
+    const int klen = clamp_len(p.k_lens, b, p.nk), qlen = clamp_len(p.q_lens, b, p.nq), per_head = (qlen + R - 1) / R;
     const int own0 = blockIdx.x * (OWN / 2), key = own0 + 32 * (wave >> 1) + (lane & 31);
     const bool live = key < klen && (!p.mask || p.mask[(int64_t)b * p.nk + key]);
-    const int tiles = (live_rows + R - 1) / R;
+    const int tiles = per_head * p.G;
     int t0 = 0, t1 = own0 < klen ? tiles : 0;
     if (p.shares > 1 && t1) { t0 = (int)((int64_t)tiles * share / p.shares); t1 = (int)((int64_t)tiles * (share + 1) / p.shares); }
 
@@ -877,56 +947,69 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
     for (int d = 0; d < DT; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
     St st;
     float ref = -INFINITY, delta = 0.f;
-    const bool check = p.mask || p.k_lens;       // otherwise every row has a key
+    // the walk: query head by query head of the key head, R of its queries at a time
     const T *qbase = (const T*)p.q + b * p.qs[0] + (int64_t)hk * p.G * p.qs[2], *obase = (const T*)p.dout + ((int64_t)b * p.nq * p.H + hk * p.G) * p.dh;
-    // a tile's rows relative to query q0: the same for every tile where G divides R, else looked up per tile
-    auto places = [&](int r0, int q0) {
-        st.places(tid, p.dh, [&](int row, int64_t& ox, int64_t& oy) {
-            const int q = query_of(p, r0 + row), g = r0 + row - q * p.G;
-            ox = (q - q0) * p.qs[1] + g * p.qs[2];
-            oy = (int64_t)((q - q0) * p.H + g) * p.dh;
-        });
-    };
-    const bool regular = p.gshift >= 0 && p.G <= R;
-    places(0, 0);
-    auto fetch = [&](int t) {
-        const int left = live_rows - t * R, q0 = query_of(p, t * R);
-        if (!regular) places(t * R, q0);
-        st.fetch(tid, qbase + q0 * p.qs[1], obase + (int64_t)q0 * p.H * p.dh, left);
+    st.places(tid, p.dh, p.qs[1], (int64_t)p.H * p.dh);
+    int g = t0 / (per_head ? per_head : 1), q0 = (t0 - g * per_head) * R;
+    auto fetch = [&]() {
+        const int left = qlen - q0;
+        st.fetch(tid, qbase + g * p.qs[2] + q0 * p.qs[1], obase + ((int64_t)q0 * p.H + g) * p.dh, p.qs[1], (int64_t)p.H * p.dh, left);
         if (tid < R) {
-            const int r = t * R + tid;
             ref = -INFINITY;
-            if (r < live_rows) {
-                const int64_t at = stat_row(p, b, hk, r);
+            if (tid < left) {
+                const int64_t at = ((int64_t)b * p.H + hk * p.G + g) * p.nq + q0 + tid;
                 ref = p.lse[at];
                 delta = p.delta[at];
             }
         }
+        q0 += R;
+        if (q0 >= qlen) { q0 = 0; ++g; }
     };
-    auto sums = [&](int n, int k, V pk, V dsk) __attribute__((always_inline)) {
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-            V f[NP];
-            read_cols<E, NP, DHP, PLANE>(Os, n, k, 2 * h + d, lane, f);
-            dv[d] = mfma(f[0], pk, dv[d]);
-            read_cols<E, NP, DHP, PLANE>(Qs, n, k, 2 * h + d, lane, f);
-            dk[d] = mfma(f[0], dsk, dk[d]);
-        }
-    };
-    if (t0 < t1) fetch(t0);
+    if (t0 < t1) fetch();
     for (int t = t0; t < t1; ++t) {
         __syncthreads();
         if (tid < R) {
-            alive[tid] = ref != -INFINITY;
+            alive[tid] = ref != -INFINITY ? ~0u : 0u;
             refs[tid] = row_ref(ref) - A::SHIFT;
             deltas[tid] = ref == -INFINITY ? 0.f : delta;
         }
-        if (check) __syncthreads();
-        st.store(tid, Qs, Os, 1.f, 1.f, check ? alive : nullptr);
+        if constexpr (CHECK) __syncthreads();
+        st.template store<CHECK>(tid, Qs, Os, 1.f, 1.f, alive);
         __syncthreads();
-        if (t + 1 < t1) fetch(t + 1);
-        f32x16 s = first_product<A, KS, DHP, PLANE>(Qs, h, lane, kf);
-        f32x16 dp = first_product<A, KS, DHP, PLANE>(Os, h, lane, vf);
+        if (t + 1 < t1) fetch();
+        // operand groups: scores, dP, then per half of the rows and k-step both sums
+        Group<A, KS> buf[2];
+        auto read = [&](int i) __attribute__((always_inline)) {
+            Group<A, KS>& g = buf[i & 1];
+            if (i < SG) read_group_rows<A, KS, DHP, PLANE>(Qs, h, i * GN, lane, g);
+            else if (i < 2 * SG) read_group_rows<A, KS, DHP, PLANE>(Os, h, (i - SG) * GN, lane, g);
+            else if (i < 2 * SG + 4) {
+                const int n = (i - 2 * SG) / 2 ? h ^ 1 : h, k = (i - 2 * SG) % 2;
+#pragma unroll
+                for (int j = 0; j < GN; ++j) read_cols<E, NP, DHP, PLANE>(j & 1 ? Qs : Os, n, k, 2 * h + j / 2, lane, g.f[j]);
+            }
+        };
+        auto sums = [&](int i, V pk, V dsk) __attribute__((always_inline)) {
+            static_assert(GN == 2 * DT);
+            read(PIPE ? i + 1 : i);
+            if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                dv[d] = mfma(buf[i & 1].f[2 * d][0], pk, dv[d]);
+                dk[d] = mfma(buf[i & 1].f[2 * d + 1][0], dsk, dk[d]);
+            }
+            if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
+        };
+        f32x16 s = zero16(), dp = zero16();
+        if (PIPE) read(0);
+#pragma unroll
+        for (int i = 0; i < 2 * SG; ++i) {
+            read(PIPE ? i + 1 : i);
+            if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
+            if (i < SG) first_product<A, KS>(buf[i & 1], kf, i * GN, s);
+            else first_product<A, KS>(buf[i & 1], vf, (i - SG) * GN, dp);
+            if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const f32x4 rv = *(const f32x4*)(refs + 32 * h + 8 * g + 4 * half);
@@ -960,10 +1043,15 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
             hand[wave][2 * k + 1][lane] = df[k];
         }
 #pragma unroll
-        for (int k = 0; k < 2; ++k) sums(h, k, pf[k], df[k]);
+        for (int k = 0; k < 2; ++k) sums(2 * SG + k, pf[k], df[k]);
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < 2; ++k) sums(h ^ 1, k, hand[wave ^ 1][2 * k][lane], hand[wave ^ 1][2 * k + 1][lane]);
+        for (int k = 0; k < 2; ++k) {
+            pf[k] = hand[wave ^ 1][2 * k][lane];
+            df[k] = hand[wave ^ 1][2 * k + 1][lane];
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) sums(2 * SG + 2 + k, pf[k], df[k]);
     }
     if (key >= p.nk) return;
     if (!live) {
@@ -1030,9 +1118,9 @@ const char* bad_desc(const imp_attn_desc* d) {
             return "strides must be multiples of 16 bytes";
     // the 32-bit offsets within a tile of 64 rows
     const int64_t most = ((int64_t)1 << 30) / (d->dtype == IMP_DTYPE_F32 ? 4 : 2);
-    if (d->q_stride[1] > most / 64 || d->k_stride[1] > most / 64 || d->v_stride[1] > most / 64 || d->q_stride[2] > most / (d->heads / d->kv_heads) ||
+    if (d->q_stride[1] > most / 64 || d->k_stride[1] > most / 64 || d->v_stride[1] > most / 64 ||
         (int64_t)d->heads * d->head_dim > most / 64)
-        return "strides too large: 64 tokens, and the query heads of a key head, must lie within 2^30 bytes";
+        return "strides too large: 64 tokens must lie within 2^30 bytes";
     return nullptr;
 }
 bool unaligned(std::initializer_list<const void*> ptrs) {
@@ -1051,13 +1139,18 @@ AttnOp op_of(const imp_attn_desc& d) {
 }
 
 // which: 0 forward, 1 dQ, 2 dK / dV
-template <typename A, int DHP> void launch(int which, const AttnOp& p, hipStream_t st) {
+template <typename A, int DHP, bool CHECK> void launch(int which, const AttnOp& p, hipStream_t st) {
     const int64_t own = which == 2 ? p.nk : (int64_t)p.nq * p.G;
     const dim3 grid((unsigned)((own + OWN - 1) / OWN), (unsigned)(p.B * p.Hkv), (unsigned)p.shares);
-    if (which == 0) attn_fwd_kernel<A, DHP><<<grid, 256, 0, st>>>(p);
-    else if (which == 1) attn_dq_kernel<A, DHP><<<grid, 256, 0, st>>>(p);
-    else if constexpr (A::NP == 1 && DHP == 128) attn_dkv_pair_kernel<A><<<dim3((unsigned)((own + OWN / 2 - 1) / (OWN / 2)), grid.y, grid.z), 256, 0, st>>>(p);
-    else attn_dkv_kernel<A, DHP><<<grid, 256, 0, st>>>(p);
+    if (which == 0) attn_fwd_kernel<A, DHP, CHECK><<<grid, 256, 0, st>>>(p);
+    else if (which == 1) attn_dq_kernel<A, DHP, CHECK><<<grid, 256, 0, st>>>(p);
+    else if constexpr (A::NP == 1 && DHP == 128) attn_dkv_pair_kernel<A, CHECK><<<dim3((unsigned)((own + OWN / 2 - 1) / (OWN / 2)), grid.y, grid.z), 256, 0, st>>>(p);
+    else attn_dkv_kernel<A, DHP, CHECK><<<grid, 256, 0, st>>>(p);
+}
+// CHECK: rows inside the tensors may not count - masked keys (forward, dQ); queries whose keys are all masked or past their count (dK / dV)
+template <typename A, int DHP> void launch(int which, const AttnOp& p, hipStream_t st) {
+    if (p.mask || (which == 2 && p.k_lens)) launch<A, DHP, true>(which, p, st);
+    else launch<A, DHP, false>(which, p, st);
 }
 template <typename A> void launch_dh(int which, const AttnOp& p, hipStream_t st) {
     if (p.dh <= 32) launch<A, 32>(which, p, st);

@@ -75,7 +75,7 @@ def _regular(shape, stride, size):
     unit, most = 16 // size, (1 << 30) // size
     if shape[3] != 1 and stride[3] != 1:
         return False
-    if (shape[1] > 1 and stride[1] > most // 64) or (shape[2] > 1 and stride[2] > most // shape[2]):
+    if shape[1] > 1 and stride[1] > most // 64:
         return False
     return all(shape[i] == 1 or (stride[i] % unit == 0 and stride[i] > 0) for i in range(3))
 

@@ -493,7 +493,7 @@ int imp_sp_op_conv(imp_sp_ctx* ctx, int layer, const float* in, int B, int H, in
 /* Multi-head attention with gradients (csrc/attention_grad.hip; the operation of nets/layers.py:121-131 with any number of heads, shared key heads and types):
  *   S = scale q.k   P = softmax of S over the kept keys   out = P v   lse = log sum exp S
  * q [batch][nq][heads][head_dim], k, v [batch][nk][kv_heads][head_dim], all of `dtype`, channels contiguous, other strides in elements (batch, token, head; multiples of
- * 16 bytes, so a packed q | k | v projection is taken as it lies; 64 tokens, and the query heads of one key head, within 2^30 bytes); query head h reads key head h / (heads / kv_heads).  head_dim a multiple of 8 up to 128.
+ * 16 bytes, so a packed q | k | v projection is taken as it lies; 64 tokens within 2^30 bytes); query head h reads key head h / (heads / kv_heads).  head_dim a multiple of 8 up to 128.
  * key_mask: optional uint8 [batch][nk], 0 = the key does not exist; q_lens / k_lens: optional int32 [batch] counts of a ragged batch (clamped to 0 .. nq / nk).  What does not
  * exist is never read into a result (it may hold NaN).  A query without a key, and a query past its count: out 0, lse -inf, no gradient. */
 typedef struct imp_attn_desc {
