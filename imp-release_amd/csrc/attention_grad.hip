@@ -199,22 +199,31 @@ template <int DHP> __device__ __forceinline__ int turn(int r) {
     else if constexpr (DHP == 64) return ((r & 2) << 1) | ((r >> 2) & 3);
     else return (r >> 2) & 3;
 }
+// a lane's element offsets in a tile: of its row (first product, k-step 0) and of its column block (transpose read, channels 0 .. 31); the others differ by an XOR
+template <int DHP> struct Lanes {
+    int row, col;
+    __device__ explicit Lanes(int lane) {
+        const int r = lane & 31, half = lane >> 5, q = 4 * half + ((lane & 15) >> 2);
+        row = r * DHP + (half ^ turn<DHP>(r)) * 8;
+        col = q * DHP + ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ turn<DHP>(q)) * 8 + 4 * (lane & 1);
+    }
+    // where registers are scarce: the XORs are done again at every use, not kept
+    __device__ void again() { asm volatile("" : "+v"(row), "+v"(col)); }
+};
 // A operand of the first product: row = lane % 32 of the 32-row sub-tile, 8 columns of k-step s
 template <typename E, int NP, int DHP, int PLANE>
-__device__ __forceinline__ void read_rows(const E* tile, int sub, int s, int lane, typename Vec8<E>::type (&f)[NP]) {
-    const int r = lane & 31;
-    const E* a = tile + sub * 32 * DHP + r * DHP + ((((lane >> 5) ^ turn<DHP>(r)) ^ (2 * s)) * 8);
+__device__ __forceinline__ void read_rows(const E* tile, int sub, int s, const Lanes<DHP>& at, typename Vec8<E>::type (&f)[NP]) {
+    const E* a = tile + sub * 32 * DHP + (at.row ^ (16 * s));
 #pragma unroll
     for (int j = 0; j < NP; ++j) f[j] = *(const typename Vec8<E>::type*)(a + j * PLANE);
 }
 // A operand of the second product: the tile transposed, channel = 32 dt + lane % 32, slot e of half h = row 16 s + 8 (e / 4) + 4 h + e % 4
 template <typename E, int NP, int DHP, int PLANE>
-__device__ __forceinline__ void read_cols(const E* tile, int sub, int s, int dt, int lane, typename Vec8<E>::type (&f)[NP]) {
+__device__ __forceinline__ void read_cols(const E* tile, int sub, int s, int dt, const Lanes<DHP>& at, typename Vec8<E>::type (&f)[NP]) {
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    const int r = 4 * (lane >> 5) + ((lane & 15) >> 2), c = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ turn<DHP>(r);
-    const E* base = tile + (sub * 32 + 16 * s) * DHP + 4 * (lane & 1);
-    const E* a0 = base + r * DHP + (c ^ (4 * dt)) * 8;
-    const E* a1 = base + (r + 8) * DHP + (c ^ (4 * dt) ^ 2) * 8;             // turn(r + 8) = turn(r) ^ 2
+    const E* base = tile + (sub * 32 + 16 * s) * DHP;
+    const E* a0 = base + (at.col ^ (32 * dt));
+    const E* a1 = base + 8 * DHP + (at.col ^ (32 * dt) ^ 16);                // turn(r + 8) = turn(r) ^ 2
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
         const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a0 + j * PLANE));
@@ -316,9 +325,9 @@ __device__ __forceinline__ void first_product(const Group<A, KS>& g, const typen
     for (int j = 0; j < N; ++j) c = mfma(g.f[j][0], own[k0 + j][0], c);
 }
 template <typename A, int KS, int DHP, int PLANE>
-__device__ __forceinline__ void read_group_rows(const typename A::E* tile, int sub, int k0, int lane, Group<A, KS>& g) {
+__device__ __forceinline__ void read_group_rows(const typename A::E* tile, int sub, int k0, const Lanes<DHP>& at, Group<A, KS>& g) {
 #pragma unroll
-    for (int j = 0; j < group_of<A::NP, KS>(); ++j) read_rows<typename A::E, A::NP, DHP, PLANE>(tile, sub, k0 + j, lane, g.f[j]);
+    for (int j = 0; j < group_of<A::NP, KS>(); ++j) read_rows<typename A::E, A::NP, DHP, PLANE>(tile, sub, k0 + j, at, g.f[j]);
 }
 
 __device__ __forceinline__ f32x16 zero16() {
@@ -455,6 +464,7 @@ __global__ __launch_bounds__(256, A::NP == 3 && DHP == 128 ? 1 : 2) void attn_fw
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = zero16();
     float m = -INFINITY, l = 0.f;
+    Lanes<DHP> lanes(lane);
     St st;
     st.places(tid, p.dh, p.ks[1], p.vs[1]);
     int keep = 0;
@@ -475,11 +485,11 @@ __global__ __launch_bounds__(256, A::NP == 3 && DHP == 128 ? 1 : 2) void attn_fw
         Group<A, KS> buf[2];
         auto read = [&](int i) __attribute__((always_inline)) {
             Group<A, KS>& g = buf[i & 1];
-            if (i < NT * SG) read_group_rows<A, KS, DHP, PLANE>(Ks, i / SG, i % SG * GN, lane, g);
+            if (i < NT * SG) read_group_rows<A, KS, DHP, PLANE>(Ks, i / SG, i % SG * GN, lanes, g);
             else if (i < NT * (SG + PG)) {
                 const int n = (i - NT * SG) / PG, e0 = (i - NT * SG) % PG * GN;
 #pragma unroll
-                for (int j = 0; j < GN; ++j) read_cols<E, NP, DHP, PLANE>(Vs, n, (e0 + j) / DT, (e0 + j) % DT, lane, g.f[j]);
+                for (int j = 0; j < GN; ++j) read_cols<E, NP, DHP, PLANE>(Vs, n, (e0 + j) / DT, (e0 + j) % DT, lanes, g.f[j]);
             }
         };
         f32x16 s[NT];
@@ -665,6 +675,7 @@ __global__ __launch_bounds__(256, A::NP > 1 && DHP == 128 ? 1 : 2) void attn_dq_
     f32x16 dq[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) dq[d] = zero16();
+    Lanes<DHP> lanes(lane);
     St st;
     st.places(tid, p.dh, p.ks[1], p.vs[1]);
     int keep = 0;
@@ -688,11 +699,11 @@ __global__ __launch_bounds__(256, A::NP > 1 && DHP == 128 ? 1 : 2) void attn_dq_
             if (i == ALL) { ++n; i = 0; }
             if (n == NT) return;
             Group<A, KS>& g = buf[(n * ALL + i) & 1];
-            if (i < SG) read_group_rows<A, KS, DHP, PLANE>(Ks, n, i * GN, lane, g);
-            else if (i < 2 * SG) read_group_rows<A, KS, DHP, PLANE>(Vs, n, (i - SG) * GN, lane, g);
+            if (i < SG) read_group_rows<A, KS, DHP, PLANE>(Ks, n, i * GN, lanes, g);
+            else if (i < 2 * SG) read_group_rows<A, KS, DHP, PLANE>(Vs, n, (i - SG) * GN, lanes, g);
             else {
 #pragma unroll
-                for (int j = 0; j < GN; ++j) { const int e = (i - 2 * SG) * GN + j; read_cols<E, NP, DHP, PLANE>(Ks, n, e / DT, e % DT, lane, g.f[j]); }
+                for (int j = 0; j < GN; ++j) { const int e = (i - 2 * SG) * GN + j; read_cols<E, NP, DHP, PLANE>(Ks, n, e / DT, e % DT, lanes, g.f[j]); }
             }
         };
         if (PIPE) read(0, 0);
@@ -804,6 +815,7 @@ __global__ __launch_bounds__(256, DHP == 128 || (A::NP == 3 && DHP == 64) ? 1 : 
     f32x16 dk[DT], dv[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
+    Lanes<DHP> lanes(lane);
     St st;
     float ref = -INFINITY, delta = 0.f;
     // the walk: query head by query head of the key head, R of its queries at a time
@@ -838,18 +850,19 @@ __global__ __launch_bounds__(256, DHP == 128 || (A::NP == 3 && DHP == 64) ? 1 : 
         if (t + 1 < t1) fetch();
         // per sub-tile: operand groups of the scores, of dP, of both sums (dV's and dK's in turn)
         constexpr int ALL = 2 * SG + 2 * PG;
+        if constexpr (DHP >= 64) lanes.again();
         Group<A, KS> buf[2];
         auto read = [&](int n, int i) __attribute__((always_inline)) {
             if (i == ALL) { ++n; i = 0; }
             if (n == NT) return;
             Group<A, KS>& g = buf[(n * ALL + i) & 1];
-            if (i < SG) read_group_rows<A, KS, DHP, PLANE>(Qs, n, i * GN, lane, g);
-            else if (i < 2 * SG) read_group_rows<A, KS, DHP, PLANE>(Os, n, (i - SG) * GN, lane, g);
+            if (i < SG) read_group_rows<A, KS, DHP, PLANE>(Qs, n, i * GN, lanes, g);
+            else if (i < 2 * SG) read_group_rows<A, KS, DHP, PLANE>(Os, n, (i - SG) * GN, lanes, g);
             else {
 #pragma unroll
                 for (int j = 0; j < GN; ++j) {
                     const int e = (i - 2 * SG) * GN + j;
-                    read_cols<E, NP, DHP, PLANE>(e & 1 ? Qs : Os, n, e / (2 * DT), e / 2 % DT, lane, g.f[j]);
+                    read_cols<E, NP, DHP, PLANE>(e & 1 ? Qs : Os, n, e / (2 * DT), e / 2 % DT, lanes, g.f[j]);
                 }
             }
         };
@@ -945,6 +958,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
     f32x16 dk[DT], dv[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) { dk[d] = zero16(); dv[d] = zero16(); }
+    Lanes<DHP> lanes(lane);
     St st;
     float ref = -INFINITY, delta = 0.f;
     // the walk: query head by query head of the key head, R of its queries at a time
@@ -978,15 +992,16 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
         __syncthreads();
         if (t + 1 < t1) fetch();
         // operand groups: scores, dP, then per half of the rows and k-step both sums
+        lanes.again();
         Group<A, KS> buf[2];
         auto read = [&](int i) __attribute__((always_inline)) {
             Group<A, KS>& g = buf[i & 1];
-            if (i < SG) read_group_rows<A, KS, DHP, PLANE>(Qs, h, i * GN, lane, g);
-            else if (i < 2 * SG) read_group_rows<A, KS, DHP, PLANE>(Os, h, (i - SG) * GN, lane, g);
+            if (i < SG) read_group_rows<A, KS, DHP, PLANE>(Qs, h, i * GN, lanes, g);
+            else if (i < 2 * SG) read_group_rows<A, KS, DHP, PLANE>(Os, h, (i - SG) * GN, lanes, g);
             else if (i < 2 * SG + 4) {
                 const int n = (i - 2 * SG) / 2 ? h ^ 1 : h, k = (i - 2 * SG) % 2;
 #pragma unroll
-                for (int j = 0; j < GN; ++j) read_cols<E, NP, DHP, PLANE>(j & 1 ? Qs : Os, n, k, 2 * h + j / 2, lane, g.f[j]);
+                for (int j = 0; j < GN; ++j) read_cols<E, NP, DHP, PLANE>(j & 1 ? Qs : Os, n, k, 2 * h + j / 2, lanes, g.f[j]);
             }
         };
         auto sums = [&](int i, V pk, V dsk) __attribute__((always_inline)) {
