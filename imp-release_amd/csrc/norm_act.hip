@@ -6,9 +6,14 @@
 // Tokens past an element's count do not exist: not read, 0 in y and dx.
 //
 // Sums are taken in 64 bits around the group's first element (no cancellation, and the sign of x - mean, where the slope of relu / lrelu jumps, is that of the
-// exact mean: the mean is kept as two floats).  Bound by memory: x is read for the statistics and again to normalise (from the 256-MB cache where it fits).
+// exact mean: the mean is kept as two floats).
+//
+// Two ways, both bound by memory.  HELD: a workgroup takes whole groups of one batch element, 64 bytes of channels or more, and keeps all their tokens in registers (16 vectors of
+// 16 bytes per thread): one launch, x (and dy) read once.  Where the tokens do not fit: a launch that sums parts, a small one that joins them in a fixed order, and an
+// elementwise one - x is read twice, the second time from the 256-MB cache where it fits.
 #include "../../include/imp_hip.h"
 #include "imp_kernels.h"
+#include <type_traits>
 
 int imp_fail(int code, const char* msg);   // context.hip: sets imp_last_error()
 
@@ -30,26 +35,49 @@ struct NormOp {
 };
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
+// the same as it is held in registers
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+template <typename T, int V> using Raw = std::conditional_t<sizeof(T) * V == 16, u32x4, T>;
+template <typename T, int V> __device__ __forceinline__ Pack<T, V> unpack(const Raw<T, V>& r) { return __builtin_bit_cast(Pack<T, V>, r); }
 
 __device__ __forceinline__ int len_of(const NormOp& p, int b) { return p.lens ? min(max(p.lens[b], 0), p.N) : p.N; }
 
-__device__ __forceinline__ float act_of(int act, float z) {
-    switch (act) {
-        case IMP_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
-        case IMP_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-        case IMP_ACT_LRELU: return z > 0.f ? z : 0.1f * z;
-        case IMP_ACT_SILU: return z / (1.f + __expf(-z));
-        default: return z;
-    }
+// the normal distribution function and (unscaled) density of z, by the rational approximation 7.1.26 of Abramowitz & Stegun's handbook (|error| of erf below 1.5e-7, what fp32
+// leaves of 1 + erf): one exponential serves both
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+    const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.f));
+    e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);               // exp(-z^2 / 2)
+    float q = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+    q = __builtin_fmaf(q, t, 1.421413741f);
+    q = __builtin_fmaf(q, t, -0.284496736f);
+    q = __builtin_fmaf(q, t, 0.254829592f);
+    q *= 0.5f * t * e;
+    return z > 0.f ? 1.f - q : q;
+}
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f)); }
+template <int ACT> __device__ __forceinline__ float act_of(float z) {
+    if constexpr (ACT == IMP_ACT_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
+    else if constexpr (ACT == IMP_ACT_GELU) { float e; return z * normal_cdf(z, e); }
+    else if constexpr (ACT == IMP_ACT_LRELU) return z > 0.f ? z : 0.1f * z;
+    else if constexpr (ACT == IMP_ACT_SILU) return z * sigmoid(z);
+    else return z;
 }
 // act'(z); `above`: whether z > 0 in the precise sense
-__device__ __forceinline__ float slope_of(int act, float z, bool above) {
+template <int ACT> __device__ __forceinline__ float slope_of(float z, bool above) {
+    if constexpr (ACT == IMP_ACT_RELU) return above ? 1.f : 0.f;
+    else if constexpr (ACT == IMP_ACT_GELU) { float e; const float c = normal_cdf(z, e); return __builtin_fmaf(z * 0.3989422804014327f, e, c); }
+    else if constexpr (ACT == IMP_ACT_LRELU) return above ? 1.f : 0.1f;
+    else if constexpr (ACT == IMP_ACT_SILU) { const float s = sigmoid(z); return s * __builtin_fmaf(z, 1.f - s, 1.f); }
+    else return 1.f;
+}
+// f with the activation as a constant
+template <typename F> void with_act(int act, F f) {
     switch (act) {
-        case IMP_ACT_RELU: return above ? 1.f : 0.f;
-        case IMP_ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.3989422804014327f;
-        case IMP_ACT_LRELU: return above ? 1.f : 0.1f;
-        case IMP_ACT_SILU: { const float s = 1.f / (1.f + __expf(-z)); return s * (1.f + z * (1.f - s)); }
-        default: return 1.f;
+        case IMP_ACT_RELU: f(std::integral_constant<int, IMP_ACT_RELU>()); break;
+        case IMP_ACT_GELU: f(std::integral_constant<int, IMP_ACT_GELU>()); break;
+        case IMP_ACT_LRELU: f(std::integral_constant<int, IMP_ACT_LRELU>()); break;
+        case IMP_ACT_SILU: f(std::integral_constant<int, IMP_ACT_SILU>()); break;
+        default: f(std::integral_constant<int, IMP_ACT_NONE>());
     }
 }
 
@@ -90,6 +118,20 @@ template <int V> __device__ __forceinline__ Place place(const NormOp& p, int row
     return q;
 }
 
+// calls f(row, vectors...) for this thread's rows below `end`, four rows' loads under way at a time
+template <typename P, typename L, typename F> __device__ __forceinline__ void rows4(const Place& q, int end, L load, F f) {
+    int r = q.r0 + q.tr;
+    for (; r + 3 * q.step < end; r += 4 * q.step) {
+        P v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = load(r + j * q.step);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f(r + j * q.step, v[j]);
+    }
+    for (; r < end; r += q.step) f(r, load(r));
+}
+template <typename P> struct Two { P x, d; };
+
 // sums over the token rows of a workgroup -> part[b][c][chunk]
 template <int V> __device__ __forceinline__ void write_part(const NormOp& p, const Place& q, const double (&s)[V], const double (&t)[V]) {
     __shared__ double2 sm[256];
@@ -114,17 +156,27 @@ __global__ __launch_bounds__(256) void norm_sums_kernel(NormOp p) {
     double s[V], t[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) { s[i] = 0; t[i] = 0; piv[i] = q.on ? (float)x[(q.c0 + i) / p.cg * p.cg] : 0.f; }
+    using P = Pack<T, V>;
     if (q.on)
-        for (int r = q.r0 + q.tr; r < end; r += q.step) {
-            const Pack<T, V> v = *(const Pack<T, V>*)(x + (int64_t)r * p.C + q.c0);
+        rows4<P>(q, end, [&](int r) { return *(const P*)(x + (int64_t)r * p.C + q.c0); }, [&](int, const P& v) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const double d = (float)v.v[i] - piv[i];
                 s[i] += d;
                 t[i] += d * d;
             }
-        }
+        });
     write_part<V>(p, q, s, t);
+}
+
+// mean and rstd (two floats each) from the sums around the pivot
+__device__ __forceinline__ float4 stats_of(const NormOp& p, int len, double s, double t, float pivot) {
+    const double cnt = (double)len * p.cg, off = cnt > 0 ? s / cnt : 0, var = cnt > 0 ? t / cnt - off * off : 0;
+    const double mean = (double)pivot + off, r = 1.0 / sqrt((var < 0 ? 0 : var) + (double)p.eps);
+    float4 o;
+    o.x = (float)mean; o.y = (float)(mean - (double)o.x);
+    o.z = (float)r; o.w = (float)(r - (double)o.z);
+    return o;
 }
 
 __device__ __forceinline__ double wave_sum(double v) {
@@ -133,31 +185,35 @@ __device__ __forceinline__ double wave_sum(double v) {
     return v;
 }
 
-// one wave per (batch element, group)
+// one workgroup per (batch element, group)
 template <typename T>
 __global__ __launch_bounds__(256) void norm_stats_kernel(NormOp p) {
-    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (at >= (int64_t)p.B * p.G) return;
-    const int b = (int)(at / p.G), g = (int)(at % p.G);
+    __shared__ double2 sm[4];
+    const int at = blockIdx.x, b = at / p.G, g = at % p.G;
     const double2* part = p.part + ((int64_t)b * p.C + (int64_t)g * p.cg) * p.chunks;
     const int64_t n = (int64_t)p.cg * p.chunks;
     double s = 0, t = 0;
-    for (int64_t i = lane; i < n; i += 64) { s += part[i].x; t += part[i].y; }
+    for (int64_t i = threadIdx.x; i < n; i += 256) { s += part[i].x; t += part[i].y; }
     s = wave_sum(s);
     t = wave_sum(t);
-    if (lane) return;
-    const int len = len_of(p, b);
-    const double cnt = (double)len * p.cg, off = cnt > 0 ? s / cnt : 0, var = cnt > 0 ? t / cnt - off * off : 0;
-    const double mean = (double)(float)((const T*)p.x)[(int64_t)b * p.N * p.C + (int64_t)g * p.cg] + off;
-    const double r = 1.0 / sqrt((var < 0 ? 0 : var) + (double)p.eps);
-    float4 o;
-    o.x = (float)mean; o.y = (float)(mean - (double)o.x);
-    o.z = (float)r; o.w = (float)(r - (double)o.z);
-    p.stats[at] = o;
+    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = double2{s, t};
+    __syncthreads();
+    if (threadIdx.x) return;
+    s = (sm[0].x + sm[1].x) + (sm[2].x + sm[3].x);
+    t = (sm[0].y + sm[1].y) + (sm[2].y + sm[3].y);
+    p.stats[at] = stats_of(p, len_of(p, b), s, t, (float)((const T*)p.x)[(int64_t)b * p.N * p.C + (int64_t)g * p.cg]);
 }
 
-template <typename T, int V>
+// the rows of this thread that do not exist
+template <typename T, int V> __device__ __forceinline__ void zero_rows(const NormOp& p, const Place& q, int len, T* to) {
+    Pack<T, V> z;
+#pragma unroll
+    for (int i = 0; i < V; ++i) z.v[i] = (T)0.f;
+    for (int r = q.r0 + q.tr; r < q.r1; r += q.step)
+        if (r >= len) *(Pack<T, V>*)(to + (int64_t)r * p.C) = z;
+}
+
+template <typename T, int V, int ACT>
 __global__ __launch_bounds__(256) void norm_apply_kernel(NormOp p) {
     const Place q = place<V>(p, p.rows);
     if (!q.on) return;
@@ -166,28 +222,24 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormOp p) {
     T* y = (T*)p.y + (int64_t)q.b * p.N * p.C + q.c0;
     Chan<V> ch;
     ch.load(p, q.b, q.c0);
-    for (int r = q.r0 + q.tr; r < q.r1; r += q.step) {
-        Pack<T, V> o;
-        if (r < len) {
-            const Pack<T, V> v = *(const Pack<T, V>*)(x + (int64_t)r * p.C);
+    using P = Pack<T, V>;
+    rows4<P>(q, min(q.r1, len), [&](int r) { return *(const P*)(x + (int64_t)r * p.C); }, [&](int r, const P& v) {
+        P o;
 #pragma unroll
-            for (int i = 0; i < V; ++i) o.v[i] = (T)act_of(p.act, __builtin_fmaf(ch.xh((float)v.v[i], i), ch.w[i], ch.b[i]));
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) o.v[i] = (T)0.f;
-        }
-        *(Pack<T, V>*)(y + (int64_t)r * p.C) = o;
-    }
+        for (int i = 0; i < V; ++i) o.v[i] = (T)act_of<ACT>(__builtin_fmaf(ch.xh((float)v.v[i], i), ch.w[i], ch.b[i]));
+        *(P*)(y + (int64_t)r * p.C) = o;
+    });
+    zero_rows<T, V>(p, q, len, y);
 }
 
-template <int V> __device__ __forceinline__ float dz_of(const NormOp& p, const Chan<V>& ch, int b, int c, int i, float x, float dy, float& xh) {
+template <int V, int ACT> __device__ __forceinline__ float dz_of(const NormOp& p, const Chan<V>& ch, int b, int c, int i, float x, float dy, float& xh) {
     xh = ch.xh(x, i);
     const float z = __builtin_fmaf(xh, ch.w[i], ch.b[i]);
-    const bool jump = p.act == IMP_ACT_RELU || p.act == IMP_ACT_LRELU;
-    return dy * slope_of(p.act, z, jump && above_zero(p, b, c, x, ch.mh[i], ch.ml[i], xh, ch.w[i], ch.b[i]));
+    constexpr bool jump = ACT == IMP_ACT_RELU || ACT == IMP_ACT_LRELU;
+    return dy * slope_of<ACT>(z, jump && above_zero(p, b, c, x, ch.mh[i], ch.ml[i], xh, ch.w[i], ch.b[i]));
 }
 
-template <typename T, int V>
+template <typename T, int V, int ACT>
 __global__ __launch_bounds__(256) void norm_grad_sums_kernel(NormOp p) {
     const Place q = place<V>(p, p.rows);
     const T* x = (const T*)p.x + (int64_t)q.b * p.N * p.C + q.c0;
@@ -199,28 +251,26 @@ __global__ __launch_bounds__(256) void norm_grad_sums_kernel(NormOp p) {
     if (q.on) {
         Chan<V> ch;
         ch.load(p, q.b, q.c0);
-        for (int r = q.r0 + q.tr; r < end; r += q.step) {
-            const Pack<T, V> v = *(const Pack<T, V>*)(x + (int64_t)r * p.C), d = *(const Pack<T, V>*)(dy + (int64_t)r * p.C);
+        using P = Pack<T, V>;
+        rows4<Two<P>>(q, end, [&](int r) { return Two<P>{*(const P*)(x + (int64_t)r * p.C), *(const P*)(dy + (int64_t)r * p.C)}; }, [&](int, const Two<P>& v) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 float xh;
-                const double dz = dz_of<V>(p, ch, q.b, q.c0 + i, i, (float)v.v[i], (float)d.v[i], xh);
+                const double dz = dz_of<V, ACT>(p, ch, q.b, q.c0 + i, i, (float)v.x.v[i], (float)v.d.v[i], xh);
                 s[i] += dz;
                 t[i] += dz * xh;
             }
-        }
+        });
     }
     write_part<V>(p, q, s, t);
 }
 
-// one wave per (batch element, group): sums per channel, and the two means of the group
+// one workgroup per (batch element, group): sums per channel (a wave each in turn), and the two means of the group
 __global__ __launch_bounds__(256) void norm_grad_means_kernel(NormOp p) {
-    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (at >= (int64_t)p.B * p.G) return;
-    const int b = (int)(at / p.G), g = (int)(at % p.G);
+    __shared__ double2 sm[4];
+    const int at = blockIdx.x, b = at / p.G, g = at % p.G, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     double m1 = 0, m2 = 0;
-    for (int c = g * p.cg; c < (g + 1) * p.cg; ++c) {
+    for (int c = g * p.cg + wave; c < (g + 1) * p.cg; c += 4) {
         const double2* part = p.part + ((int64_t)b * p.C + c) * p.chunks;
         double s = 0, t = 0;
         for (int i = lane; i < p.chunks; i += 64) { s += part[i].x; t += part[i].y; }
@@ -231,8 +281,13 @@ __global__ __launch_bounds__(256) void norm_grad_means_kernel(NormOp p) {
         m1 += w * s;
         m2 += w * t;
     }
+    if (lane == 0) sm[wave] = double2{m1, m2};
+    __syncthreads();
+    if (threadIdx.x) return;
     const double cnt = (double)len_of(p, b) * p.cg;
-    if (lane == 0) p.mom[at] = float2{cnt > 0 ? (float)(m1 / cnt) : 0.f, cnt > 0 ? (float)(m2 / cnt) : 0.f};
+    m1 = (sm[0].x + sm[1].x) + (sm[2].x + sm[3].x);
+    m2 = (sm[0].y + sm[1].y) + (sm[2].y + sm[3].y);
+    p.mom[at] = float2{cnt > 0 ? (float)(m1 / cnt) : 0.f, cnt > 0 ? (float)(m2 / cnt) : 0.f};
 }
 
 __global__ __launch_bounds__(256) void norm_affine_kernel(NormOp p) {
@@ -244,7 +299,7 @@ __global__ __launch_bounds__(256) void norm_affine_kernel(NormOp p) {
     if (p.dw) p.dw[c] = (float)t;
 }
 
-template <typename T, int V>
+template <typename T, int V, int ACT>
 __global__ __launch_bounds__(256) void norm_grad_kernel(NormOp p) {
     const Place q = place<V>(p, p.rows);
     if (!q.on) return;
@@ -257,21 +312,188 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(NormOp p) {
     float m1[V], m2[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) { const float2 m = p.mom[(int64_t)q.b * p.G + (q.c0 + i) / p.cg]; m1[i] = m.x; m2[i] = m.y; }
-    for (int r = q.r0 + q.tr; r < q.r1; r += q.step) {
-        Pack<T, V> o;
+    using P = Pack<T, V>;
+    rows4<Two<P>>(q, min(q.r1, len), [&](int r) { return Two<P>{*(const P*)(x + (int64_t)r * p.C), *(const P*)(dy + (int64_t)r * p.C)}; }, [&](int r, const Two<P>& v) {
+        P o;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float xh;
+            const float dz = dz_of<V, ACT>(p, ch, q.b, q.c0 + i, i, (float)v.x.v[i], (float)v.d.v[i], xh);
+            o.v[i] = (T)((dz * ch.w[i] - m1[i] - xh * m2[i]) * ch.rh[i]);
+        }
+        *(P*)(dx + (int64_t)r * p.C) = o;
+    });
+    zero_rows<T, V>(p, q, len, dx);
+}
+
+// ------------------------------------------------------------------------------------------------------------------------- held
+// A workgroup of 512 threads: tc columns of V channels (whole groups) x 512 / tc token rows, HOLD rows per thread.  K: rows that a thread really has, a template so that short
+// sequences do not pay for long ones.
+constexpr int HOLD = 16, HELD_THREADS = 512;      // (8 rows of 16-bit types with their gradients: eight channels a vector, twice the arithmetic per register)
+// sums of 2 V values per thread over the token rows, then over the channels of a group (group sums and, where wanted, channel sums)
+template <int V> __device__ __forceinline__ void reduce_rows(double2* sm, int tc, const double (&s)[V], const double (&t)[V], double2* chan) {
+    const int col = threadIdx.x % tc, row = threadIdx.x / tc, rows = HELD_THREADS / tc, slab = tc * V;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (row < rows) sm[(col * V + i) * rows + row] = double2{s[i], t[i]};
+    __syncthreads();
+    // a channel's rows by HELD_THREADS / slab threads (one at least), then by one
+    const int per = slab >= HELD_THREADS ? 1 : HELD_THREADS / slab;
+    double2 a = {0, 0};
+    const int c = threadIdx.x / per, k = threadIdx.x % per;
+    if (c < slab)
+        for (int r = k; r < rows; r += per) { const double2 v = sm[c * rows + r]; a.x += v.x; a.y += v.y; }
+    __syncthreads();
+    if (c < slab) sm[c * per + k] = a;
+    __syncthreads();
+    if (threadIdx.x < slab) {
+        double2 v = {0, 0};
+        for (int i = 0; i < per; ++i) { const double2 w = sm[threadIdx.x * per + i]; v.x += w.x; v.y += w.y; }
+        chan[threadIdx.x] = v;
+    }
+    __syncthreads();
+}
+
+// Workgroups go to the eight XCDs in turn; each XCD takes neighbouring slabs here, so that the two halves of a cache line are asked for through one L2
+__device__ __forceinline__ int slab_of(int id, int total) {
+    const int x = id & 7, i = id >> 3, q = total >> 3, r = total & 7;
+    return x * q + min(x, r) + i;
+}
+
+template <typename T, int V, int K, int ACT>
+__global__ __launch_bounds__(HELD_THREADS) void norm_held_kernel(NormOp p) {
+    using P = Pack<T, V>;
+    __shared__ double2 sm[HELD_THREADS * V], chan[HELD_THREADS];
+    __shared__ float4 st[HELD_THREADS];
+    const int col = threadIdx.x % p.tc, tr = threadIdx.x / p.tc, step = HELD_THREADS / p.tc, slab = p.tc * V;
+    const int slabs = (p.C + slab - 1) / slab, w = slab_of(blockIdx.x, gridDim.x), b = w / slabs, c0 = (w - b * slabs) * slab, c = c0 + col * V, len = len_of(p, b);
+    const bool on = c < p.C && tr < step;      // (threads past the last whole row of columns have nothing)
+    const T* x = (const T*)p.x + (int64_t)b * p.N * p.C + c;
+    T* y = (T*)p.y + (int64_t)b * p.N * p.C + c;
+    Raw<T, V> v[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (on && tr + k * step < len) v[k] = *(const Raw<T, V>*)(x + (int64_t)(tr + k * step) * p.C);
+    float piv[V];
+    double s[V], t[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) { s[i] = 0; t[i] = 0; piv[i] = on ? (float)((const T*)p.x)[(int64_t)b * p.N * p.C + (c + i) / p.cg * p.cg] : 0.f; }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (on && tr + k * step < len) {
+            const P vk = unpack<T, V>(v[k]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const double d = (float)vk.v[i] - piv[i];
+                s[i] += d;
+                t[i] += d * d;
+            }
+        }
+    reduce_rows<V>(sm, p.tc, s, t, chan);
+    const int groups = min(slab, p.C - c0) / p.cg;
+    if ((int)threadIdx.x < groups) {
+        double a = 0, q = 0;
+        for (int i = 0; i < p.cg; ++i) { a += chan[threadIdx.x * p.cg + i].x; q += chan[threadIdx.x * p.cg + i].y; }
+        const float4 o = stats_of(p, len, a, q, (float)((const T*)p.x)[(int64_t)b * p.N * p.C + c0 + threadIdx.x * p.cg]);
+        st[threadIdx.x] = o;
+        p.stats[(int64_t)b * p.G + c0 / p.cg + threadIdx.x] = o;
+    }
+    __syncthreads();
+    if (!on) return;
+    Chan<V> ch;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const float4 q = st[(col * V + i) / p.cg];
+        ch.mh[i] = q.x; ch.ml[i] = q.y; ch.rh[i] = q.z;
+        ch.w[i] = p.w ? p.w[c + i] : 1.f;
+        ch.b[i] = p.b ? p.b[c + i] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int r = tr + k * step;
+        P o;
         if (r < len) {
-            const Pack<T, V> v = *(const Pack<T, V>*)(x + (int64_t)r * p.C), d = *(const Pack<T, V>*)(dy + (int64_t)r * p.C);
+            const P vk = unpack<T, V>(v[k]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.v[i] = (T)act_of<ACT>(__builtin_fmaf(ch.xh((float)vk.v[i], i), ch.w[i], ch.b[i]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.v[i] = (T)0.f;
+        }
+        if (r < p.N) *(P*)(y + (int64_t)r * p.C) = o;
+    }
+}
+
+template <typename T, int V, int K, int ACT>
+__global__ __launch_bounds__(HELD_THREADS) void norm_grad_held_kernel(NormOp p) {
+    using P = Pack<T, V>;
+    __shared__ double2 sm[HELD_THREADS * V], chan[HELD_THREADS];
+    __shared__ float2 mom[HELD_THREADS];
+    const int col = threadIdx.x % p.tc, tr = threadIdx.x / p.tc, step = HELD_THREADS / p.tc, slab = p.tc * V;
+    const int slabs = (p.C + slab - 1) / slab, w = slab_of(blockIdx.x, gridDim.x), b = w / slabs, c0 = (w - b * slabs) * slab, c = c0 + col * V, len = len_of(p, b);
+    const bool on = c < p.C && tr < step;
+    const int64_t base = (int64_t)b * p.N * p.C + c;
+    const T *x = (const T*)p.x + base, *dy = (const T*)p.dy + base;
+    T* dx = (T*)p.dx + base;
+    Raw<T, V> v[K], d[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (on && tr + k * step < len) {
+            v[k] = *(const Raw<T, V>*)(x + (int64_t)(tr + k * step) * p.C);
+            d[k] = *(const Raw<T, V>*)(dy + (int64_t)(tr + k * step) * p.C);
+        }
+    Chan<V> ch;
+    double s[V], t[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) { s[i] = 0; t[i] = 0; }
+    if (on) ch.load(p, b, c);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (on && tr + k * step < len) {
+            const P vk = unpack<T, V>(v[k]), dk = unpack<T, V>(d[k]);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 float xh;
-                const float dz = dz_of<V>(p, ch, q.b, q.c0 + i, i, (float)v.v[i], (float)d.v[i], xh);
+                const double dz = dz_of<V, ACT>(p, ch, b, c + i, i, (float)vk.v[i], (float)dk.v[i], xh);
+                s[i] += dz;
+                t[i] += dz * xh;
+            }
+        }
+    reduce_rows<V>(sm, p.tc, s, t, chan);
+    const int here = min(slab, p.C - c0), groups = here / p.cg;
+    if ((int)threadIdx.x < here && p.chan) p.chan[(int64_t)b * p.C + c0 + threadIdx.x] = chan[threadIdx.x];
+    if ((int)threadIdx.x < groups) {
+        double m1 = 0, m2 = 0;
+        for (int i = 0; i < p.cg; ++i) {
+            const double w = p.w ? p.w[c0 + threadIdx.x * p.cg + i] : 1.0;
+            m1 += w * chan[threadIdx.x * p.cg + i].x;
+            m2 += w * chan[threadIdx.x * p.cg + i].y;
+        }
+        const double cnt = (double)len * p.cg;
+        mom[threadIdx.x] = float2{cnt > 0 ? (float)(m1 / cnt) : 0.f, cnt > 0 ? (float)(m2 / cnt) : 0.f};
+    }
+    __syncthreads();
+    if (!on) return;
+    float m1[V], m2[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) { const float2 m = mom[(col * V + i) / p.cg]; m1[i] = m.x; m2[i] = m.y; }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int r = tr + k * step;
+        P o;
+        if (r < len) {
+            const P vk = unpack<T, V>(v[k]), dk = unpack<T, V>(d[k]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float xh;
+                const float dz = dz_of<V, ACT>(p, ch, b, c + i, i, (float)vk.v[i], (float)dk.v[i], xh);
                 o.v[i] = (T)((dz * ch.w[i] - m1[i] - xh * m2[i]) * ch.rh[i]);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i) o.v[i] = (T)0.f;
         }
-        *(Pack<T, V>*)(dx + (int64_t)r * p.C) = o;
+        if (r < p.N) *(P*)(dx + (int64_t)r * p.C) = o;
     }
 }
 
@@ -302,11 +524,31 @@ Shape shape_of(int dtype, int B, int N, int C) {
     return s;
 }
 
+// The held way: columns per workgroup (0: it does not fit).  Whole groups, whole vectors, 64 bytes of a row where that fits (a cache line's worth), at most HELD_THREADS channels
+struct Held { int tc, k; };
+Held held_of(int dtype, int B, int N, int C, int cg, int vec, int hold) {
+    const int size = dtype == IMP_DTYPE_F32 ? 4 : 2;
+    auto fits = [&](int slab, Held& h) {
+        if (slab % vec || slab > HELD_THREADS) return false;
+        h.tc = slab / vec;
+        if (h.tc > HELD_THREADS || (int64_t)((C + slab - 1) / slab) * B > 0x7fffffff) return false;
+        h.k = (N + HELD_THREADS / h.tc - 1) / (HELD_THREADS / h.tc);
+        return h.k <= hold;
+    };
+    Held best = {0, 0}, h;
+    for (int slab = cg; slab <= HELD_THREADS; slab += cg) {
+        if (!fits(slab, h)) continue;
+        best = h;
+        if (slab * size >= 64 || slab >= C) break;
+    }
+    return best;
+}
+
 const char* bad(int dtype, int B, int N, int C, int G, int act, const void* x, std::initializer_list<const void*> ptrs) {
     if (dtype != IMP_DTYPE_F32 && dtype != IMP_DTYPE_F16 && dtype != IMP_DTYPE_BF16) return "unknown dtype";
     if (B < 1 || N < 1 || C < 1 || B > 65535) return "batch must be between 1 and 65535, tokens and channels at least 1";
     if (G < 1 || C % G) return "channels must be a multiple of groups";
-    if (C > (1 << 20) || N > (1 << 30)) return "too many channels or tokens";
+    if (C > (1 << 20) || N > (1 << 30) || (int64_t)B * G > 0x7fffffff) return "too many channels, tokens or groups";
     if (act < IMP_ACT_RELU || act > IMP_ACT_NONE) return "unknown activation";
     if (!x) return "null argument";
     for (const void* q : ptrs) if ((uintptr_t)q & 15) return "tensors must be aligned to 16 bytes";
@@ -352,15 +594,25 @@ int imp_group_norm_act_forward(int dtype, int batch, int n, int channels, int gr
     p.B = batch; p.N = n; p.C = channels; p.G = groups; p.cg = channels / groups; p.act = act; p.eps = eps;
     p.tc = s.tc; p.chunks = s.chunks; p.rows = s.rows;
     const hipStream_t st = (hipStream_t)stream;
-    by_type(dtype, s.vec, [&](auto* t, auto v) {
+    const Held h = held_of(dtype, batch, n, channels, p.cg, s.vec, HOLD);
+    by_type(dtype, s.vec, [&](auto* t, auto v) { with_act(act, [&](auto which) {
         using T = std::remove_pointer_t<decltype(t)>;
-        constexpr int V = decltype(v)::value;
+        constexpr int V = decltype(v)::value, A = decltype(which)::value;
+        if (h.tc) {
+            NormOp a = p;
+            a.tc = h.tc;
+            const unsigned grid = (unsigned)((channels + h.tc * V - 1) / (h.tc * V)) * (unsigned)batch;
+            if (h.k <= 1) norm_held_kernel<T, V, 1, A><<<grid, HELD_THREADS, 0, st>>>(a);
+            else if (h.k <= 4) norm_held_kernel<T, V, 4, A><<<grid, HELD_THREADS, 0, st>>>(a);
+            else norm_held_kernel<T, V, HOLD, A><<<grid, HELD_THREADS, 0, st>>>(a);
+            return;
+        }
         norm_sums_kernel<T, V><<<dim3(s.chunks, s.cols, batch), 256, 0, st>>>(p);
-        norm_stats_kernel<T><<<(unsigned)(((int64_t)batch * groups + 3) / 4), 256, 0, st>>>(p);
+        norm_stats_kernel<T><<<(unsigned)(batch * groups), 256, 0, st>>>(p);
         NormOp a = p;
         a.chunks = s.achunks; a.rows = s.arows;
-        norm_apply_kernel<T, V><<<dim3(s.achunks, s.cols, batch), 256, 0, st>>>(a);
-    });
+        norm_apply_kernel<T, V, A><<<dim3(s.achunks, s.cols, batch), 256, 0, st>>>(a);
+    }); });
     return done();
 }
 
@@ -380,16 +632,28 @@ int imp_group_norm_act_backward(int dtype, int batch, int n, int channels, int g
     p.B = batch; p.N = n; p.C = channels; p.G = groups; p.cg = channels / groups; p.act = act;
     p.tc = s.tc; p.chunks = s.chunks; p.rows = s.rows;
     const hipStream_t st = (hipStream_t)stream;
-    by_type(dtype, s.vec, [&](auto* t, auto v) {
+    const Held h = held_of(dtype, batch, n, channels, p.cg, s.vec, dtype == IMP_DTYPE_F32 ? HOLD : HOLD / 2);
+    by_type(dtype, s.vec, [&](auto* t, auto v) { with_act(act, [&](auto which) {
         using T = std::remove_pointer_t<decltype(t)>;
-        constexpr int V = decltype(v)::value;
-        norm_grad_sums_kernel<T, V><<<dim3(s.chunks, s.cols, batch), 256, 0, st>>>(p);
-        norm_grad_means_kernel<<<(unsigned)(((int64_t)batch * groups + 3) / 4), 256, 0, st>>>(p);
+        constexpr int V = decltype(v)::value, A = decltype(which)::value;
+        if (h.tc) {
+            NormOp a = p;
+            a.tc = h.tc;
+            if (!dweight && !dbias) a.chan = nullptr;
+            const unsigned grid = (unsigned)((channels + h.tc * V - 1) / (h.tc * V)) * (unsigned)batch;
+            if (h.k <= 1) norm_grad_held_kernel<T, V, 1, A><<<grid, HELD_THREADS, 0, st>>>(a);
+            else if (h.k <= 4) norm_grad_held_kernel<T, V, 4, A><<<grid, HELD_THREADS, 0, st>>>(a);
+            else norm_grad_held_kernel<T, V, sizeof(T) == 4 ? HOLD : HOLD / 2, A><<<grid, HELD_THREADS, 0, st>>>(a);
+            if (dweight || dbias) norm_affine_kernel<<<(channels + 255) / 256, 256, 0, st>>>(p);
+            return;
+        }
+        norm_grad_sums_kernel<T, V, A><<<dim3(s.chunks, s.cols, batch), 256, 0, st>>>(p);
+        norm_grad_means_kernel<<<(unsigned)(batch * groups), 256, 0, st>>>(p);
         if (dweight || dbias) norm_affine_kernel<<<(channels + 255) / 256, 256, 0, st>>>(p);
         NormOp a = p;
         a.chunks = s.achunks; a.rows = s.arows;
-        norm_grad_kernel<T, V><<<dim3(s.achunks, s.cols, batch), 256, 0, st>>>(a);
-    });
+        norm_grad_kernel<T, V, A><<<dim3(s.achunks, s.cols, batch), 256, 0, st>>>(a);
+    }); });
     return done();
 }
 
