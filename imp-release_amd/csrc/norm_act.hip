@@ -81,28 +81,33 @@ template <typename F> void with_act(int act, F f) {
     }
 }
 
-// what a thread needs of its V channels
-template <int V> struct Chan {
-    float mh[V], ml[V], rh[V], w[V], b[V];
-    __device__ void load(const NormOp& p, int bi, int c0) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float4 s = p.stats[(int64_t)bi * p.G + (c0 + i) / p.cg];
-            mh[i] = s.x; ml[i] = s.y; rh[i] = s.z;
-            w[i] = p.w ? p.w[c0 + i] : 1.f;
-            b[i] = p.b ? p.b[c0 + i] : 0.f;
+// What a thread needs of its V channels.  The slope of relu / lrelu jumps where z = w xh + b passes 0, that is where x passes mean - b / (w rstd): one threshold per channel,
+// formed in 64 bits and rounded down, decides for every x exactly (up: +-1, the sign of w; x is compared as up x)
+template <int V, int ACT> struct Chan {
+    static constexpr bool JUMP = ACT == IMP_ACT_RELU || ACT == IMP_ACT_LRELU;
+    float mh[V], ml[V], rh[V], w[V], b[V], up[JUMP ? V : 1], edge[JUMP ? V : 1];
+    __device__ void set(const NormOp& p, int c, int i, const float4& s) {
+        mh[i] = s.x; ml[i] = s.y; rh[i] = s.z;
+        w[i] = p.w ? p.w[c] : 1.f;
+        b[i] = p.b ? p.b[c] : 0.f;
+        if constexpr (JUMP) {
+            up[i] = w[i] < 0.f ? -1.f : 1.f;
+            const double e = (double)up[i] * (((double)s.x + s.y) - (double)b[i] / (((double)s.z + s.w) * w[i]));
+            float f = (float)e;
+            if ((double)f > e) f = nextafterf(f, -INFINITY);
+            edge[i] = w[i] == 0.f ? (b[i] > 0.f ? -INFINITY : INFINITY) : f;
         }
     }
+    __device__ void load(const NormOp& p, int bi, int c0) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) set(p, c0 + i, i, p.stats[(int64_t)bi * p.G + (c0 + i) / p.cg]);
+    }
     __device__ float xh(float x, int i) const { return ((x - mh[i]) - ml[i]) * rh[i]; }
+    __device__ bool above(float x, int i) const {
+        if constexpr (JUMP) return up[i] * x > edge[i];
+        else return false;
+    }
 };
-// z > 0.  Without an affine part that is the sign of x - mean; with one, z next to 0 is formed again in 64 bits
-__device__ __forceinline__ bool above_zero(const NormOp& p, int bi, int c, float x, float mh, float ml, float xh, float w, float b) {
-    const float a = xh * w, z = a + b;
-    if (!p.b && !p.w) return xh > 0.f;
-    if (fabsf(z) > 1e-5f * (fabsf(a) + fabsf(b))) return z > 0.f;
-    const float4 s = p.stats[(int64_t)bi * p.G + c / p.cg];
-    return (((double)x - mh) - ml) * ((double)s.z + s.w) * w + b > 0.0;
-}
 
 // tokens [r0, r1) of batch element b, V channels from c0: 256 threads = tc columns x 256 / tc token rows
 struct Place { int b, c0, tr, step, r0, r1; bool on; };
@@ -118,15 +123,15 @@ template <int V> __device__ __forceinline__ Place place(const NormOp& p, int row
     return q;
 }
 
-// calls f(row, vectors...) for this thread's rows below `end`, four rows' loads under way at a time
-template <typename P, typename L, typename F> __device__ __forceinline__ void rows4(const Place& q, int end, L load, F f) {
+// calls f(row, vectors) for this thread's rows below `end`, U rows' loads under way at a time
+template <typename P, int U, typename L, typename F> __device__ __forceinline__ void rows_by(const Place& q, int end, L load, F f) {
     int r = q.r0 + q.tr;
-    for (; r + 3 * q.step < end; r += 4 * q.step) {
-        P v[4];
+    for (; r + (U - 1) * q.step < end; r += U * q.step) {
+        P v[U];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = load(r + j * q.step);
+        for (int j = 0; j < U; ++j) v[j] = load(r + j * q.step);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f(r + j * q.step, v[j]);
+        for (int j = 0; j < U; ++j) f(r + j * q.step, v[j]);
     }
     for (; r < end; r += q.step) f(r, load(r));
 }
@@ -158,7 +163,7 @@ __global__ __launch_bounds__(256) void norm_sums_kernel(NormOp p) {
     for (int i = 0; i < V; ++i) { s[i] = 0; t[i] = 0; piv[i] = q.on ? (float)x[(q.c0 + i) / p.cg * p.cg] : 0.f; }
     using P = Pack<T, V>;
     if (q.on)
-        rows4<P>(q, end, [&](int r) { return *(const P*)(x + (int64_t)r * p.C + q.c0); }, [&](int, const P& v) {
+        rows_by<P, 4>(q, end, [&](int r) { return *(const P*)(x + (int64_t)r * p.C + q.c0); }, [&](int, const P& v) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const double d = (float)v.v[i] - piv[i];
@@ -220,10 +225,10 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormOp p) {
     const int len = len_of(p, q.b);
     const T* x = (const T*)p.x + (int64_t)q.b * p.N * p.C + q.c0;
     T* y = (T*)p.y + (int64_t)q.b * p.N * p.C + q.c0;
-    Chan<V> ch;
+    Chan<V, ACT> ch;
     ch.load(p, q.b, q.c0);
     using P = Pack<T, V>;
-    rows4<P>(q, min(q.r1, len), [&](int r) { return *(const P*)(x + (int64_t)r * p.C); }, [&](int r, const P& v) {
+    rows_by<P, 4>(q, min(q.r1, len), [&](int r) { return *(const P*)(x + (int64_t)r * p.C); }, [&](int r, const P& v) {
         P o;
 #pragma unroll
         for (int i = 0; i < V; ++i) o.v[i] = (T)act_of<ACT>(__builtin_fmaf(ch.xh((float)v.v[i], i), ch.w[i], ch.b[i]));
@@ -232,15 +237,13 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormOp p) {
     zero_rows<T, V>(p, q, len, y);
 }
 
-template <int V, int ACT> __device__ __forceinline__ float dz_of(const NormOp& p, const Chan<V>& ch, int b, int c, int i, float x, float dy, float& xh) {
+template <int V, int ACT> __device__ __forceinline__ float dz_of(const Chan<V, ACT>& ch, int i, float x, float dy, float& xh) {
     xh = ch.xh(x, i);
-    const float z = __builtin_fmaf(xh, ch.w[i], ch.b[i]);
-    constexpr bool jump = ACT == IMP_ACT_RELU || ACT == IMP_ACT_LRELU;
-    return dy * slope_of<ACT>(z, jump && above_zero(p, b, c, x, ch.mh[i], ch.ml[i], xh, ch.w[i], ch.b[i]));
+    return dy * slope_of<ACT>(__builtin_fmaf(xh, ch.w[i], ch.b[i]), ch.above(x, i));
 }
 
 template <typename T, int V, int ACT>
-__global__ __launch_bounds__(256) void norm_grad_sums_kernel(NormOp p) {
+__global__ __launch_bounds__(256, 4) void norm_grad_sums_kernel(NormOp p) {
     const Place q = place<V>(p, p.rows);
     const T* x = (const T*)p.x + (int64_t)q.b * p.N * p.C + q.c0;
     const T* dy = (const T*)p.dy + (int64_t)q.b * p.N * p.C + q.c0;
@@ -249,14 +252,14 @@ __global__ __launch_bounds__(256) void norm_grad_sums_kernel(NormOp p) {
 #pragma unroll
     for (int i = 0; i < V; ++i) { s[i] = 0; t[i] = 0; }
     if (q.on) {
-        Chan<V> ch;
+        Chan<V, ACT> ch;
         ch.load(p, q.b, q.c0);
         using P = Pack<T, V>;
-        rows4<Two<P>>(q, end, [&](int r) { return Two<P>{*(const P*)(x + (int64_t)r * p.C), *(const P*)(dy + (int64_t)r * p.C)}; }, [&](int, const Two<P>& v) {
+        rows_by<Two<P>, V == 8 ? 2 : 4>(q, end, [&](int r) { return Two<P>{*(const P*)(x + (int64_t)r * p.C), *(const P*)(dy + (int64_t)r * p.C)}; }, [&](int, const Two<P>& v) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 float xh;
-                const double dz = dz_of<V, ACT>(p, ch, q.b, q.c0 + i, i, (float)v.x.v[i], (float)v.d.v[i], xh);
+                const double dz = dz_of<V, ACT>(ch, i, (float)v.x.v[i], (float)v.d.v[i], xh);
                 s[i] += dz;
                 t[i] += dz * xh;
             }
@@ -300,25 +303,25 @@ __global__ __launch_bounds__(256) void norm_affine_kernel(NormOp p) {
 }
 
 template <typename T, int V, int ACT>
-__global__ __launch_bounds__(256) void norm_grad_kernel(NormOp p) {
+__global__ __launch_bounds__(256, 4) void norm_grad_kernel(NormOp p) {
     const Place q = place<V>(p, p.rows);
     if (!q.on) return;
     const int len = len_of(p, q.b);
     const int64_t base = (int64_t)q.b * p.N * p.C + q.c0;
     const T *x = (const T*)p.x + base, *dy = (const T*)p.dy + base;
     T* dx = (T*)p.dx + base;
-    Chan<V> ch;
+    Chan<V, ACT> ch;
     ch.load(p, q.b, q.c0);
     float m1[V], m2[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) { const float2 m = p.mom[(int64_t)q.b * p.G + (q.c0 + i) / p.cg]; m1[i] = m.x; m2[i] = m.y; }
     using P = Pack<T, V>;
-    rows4<Two<P>>(q, min(q.r1, len), [&](int r) { return Two<P>{*(const P*)(x + (int64_t)r * p.C), *(const P*)(dy + (int64_t)r * p.C)}; }, [&](int r, const Two<P>& v) {
+    rows_by<Two<P>, V == 8 ? 2 : 4>(q, min(q.r1, len), [&](int r) { return Two<P>{*(const P*)(x + (int64_t)r * p.C), *(const P*)(dy + (int64_t)r * p.C)}; }, [&](int r, const Two<P>& v) {
         P o;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             float xh;
-            const float dz = dz_of<V, ACT>(p, ch, q.b, q.c0 + i, i, (float)v.x.v[i], (float)v.d.v[i], xh);
+            const float dz = dz_of<V, ACT>(ch, i, (float)v.x.v[i], (float)v.d.v[i], xh);
             o.v[i] = (T)((dz * ch.w[i] - m1[i] - xh * m2[i]) * ch.rh[i]);
         }
         *(P*)(dx + (int64_t)r * p.C) = o;
@@ -400,14 +403,9 @@ __global__ __launch_bounds__(HELD_THREADS) void norm_held_kernel(NormOp p) {
     }
     __syncthreads();
     if (!on) return;
-    Chan<V> ch;
+    Chan<V, ACT> ch;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const float4 q = st[(col * V + i) / p.cg];
-        ch.mh[i] = q.x; ch.ml[i] = q.y; ch.rh[i] = q.z;
-        ch.w[i] = p.w ? p.w[c + i] : 1.f;
-        ch.b[i] = p.b ? p.b[c + i] : 0.f;
-    }
+    for (int i = 0; i < V; ++i) ch.set(p, c + i, i, st[(col * V + i) / p.cg]);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const int r = tr + k * step;
@@ -442,7 +440,7 @@ __global__ __launch_bounds__(HELD_THREADS) void norm_grad_held_kernel(NormOp p) 
             v[k] = *(const Raw<T, V>*)(x + (int64_t)(tr + k * step) * p.C);
             d[k] = *(const Raw<T, V>*)(dy + (int64_t)(tr + k * step) * p.C);
         }
-    Chan<V> ch;
+    Chan<V, ACT> ch;
     double s[V], t[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) { s[i] = 0; t[i] = 0; }
@@ -454,7 +452,7 @@ __global__ __launch_bounds__(HELD_THREADS) void norm_grad_held_kernel(NormOp p) 
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 float xh;
-                const double dz = dz_of<V, ACT>(p, ch, b, c + i, i, (float)vk.v[i], (float)dk.v[i], xh);
+                const double dz = dz_of<V, ACT>(ch, i, (float)vk.v[i], (float)dk.v[i], xh);
                 s[i] += dz;
                 t[i] += dz * xh;
             }
@@ -486,7 +484,7 @@ __global__ __launch_bounds__(HELD_THREADS) void norm_grad_held_kernel(NormOp p) 
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 float xh;
-                const float dz = dz_of<V, ACT>(p, ch, b, c + i, i, (float)vk.v[i], (float)dk.v[i], xh);
+                const float dz = dz_of<V, ACT>(ch, i, (float)vk.v[i], (float)dk.v[i], xh);
                 o.v[i] = (T)((dz * ch.w[i] - m1[i] - xh * m2[i]) * ch.rh[i]);
             }
         } else {
