@@ -507,7 +507,7 @@ __global__ __launch_bounds__(256, A::NP == 3 && DHP == 128 ? 1 : 2) void attn_fw
             }
             if (CHECK || (t + 1) * R > klen) add_rows(s[n], kb + 32 * n, half);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
+            for (int i = 0; i < 16; ++i) mx = __builtin_amdgcn_fmed3f(mx, s[n][i], INFINITY);      // the larger one, without the quieting that fmaxf adds
         }
         mx = other_half_max(mx) * c;
         const bool up = mx > m + LAZY;

@@ -5,9 +5,12 @@
 // The sum leaves the largest element out, l = log1p(s): the log probability of a sure match is near 0, and 1 + s would round it away (and with it H and 1 - p,
 // which is -expm1(logp)).  Columns of -inf are masked: no probability, never an alternative; a row of nothing else has logp = -inf, H = 0 and no gradient.
 //
-// Forward: one pass over the row.  A thread keeps (m, s, U = sum e (m - x)) of its elements; two such states join as
+// Forward: one pass over the row, bound by reading it.  A wave takes pieces of 32 elements per lane, as vectors of 16 bytes (any alignment), into registers, finds a piece's largest element, and
+// sums the rest relative to the largest so far - one exponential and four more instructions per element, no per-lane bookkeeping.  What it keeps is (m, s, U = sum e (m - x));
+// two such states join as
 //   m = max, s = s_a + (s_b + 1) f, U = U_a + f (U_b + d (s_b + 1)), f = exp(-d), d = m_a - m_b >= 0            (the smaller maximum becomes an ordinary element)
-// lanes, waves and - when there are few rows - shares of a row are joined in a fixed order.  Bound by reading the logits.
+// waves and - when there are few rows - shares of a row are joined in a fixed order.  The alternatives are taken out of the registers one by one, largest first, as long as the
+// piece holds something larger than the last place of the wave's list.
 #include "../../include/imp_hip.h"
 #include "imp_kernels.h"
 
@@ -48,167 +51,55 @@ __device__ __forceinline__ State join(State a, State b) {
 }
 __device__ __forceinline__ State shfl_state(State a, int o) { return {__shfl_xor(a.m, o), __shfl_xor(a.s, o), __shfl_xor(a.u, o)}; }
 
-// the K best (value, index) of a thread, best first; index INT_MAX marks an empty place
-template <int K> struct Best {
-    float v[K ? K : 1];
-    int i[K ? K : 1];
-    __device__ void clear() {
-#pragma unroll
-        for (int k = 0; k < K; ++k) { v[k] = -INFINITY; i[k] = 0x7fffffff; }
-    }
-    // elements come in rising index order per thread: a tie goes behind
-    __device__ void take(float x, int at) {
-        if (K == 0 || !(x > v[K ? K - 1 : 0])) return;
-#pragma unroll
-        for (int k = K - 1; k >= 0; --k) {
-            const bool up = k > 0 && x > v[k > 0 ? k - 1 : 0];
-            const float nv = up ? v[k > 0 ? k - 1 : 0] : x;
-            const int ni = up ? i[k > 0 ? k - 1 : 0] : at;
-            if (x > v[k]) { v[k] = nv; i[k] = ni; }
-        }
-    }
-    __device__ void pop() {
-#pragma unroll
-        for (int k = 0; k + 1 < K; ++k) { v[k] = v[k + 1]; i[k] = i[k + 1]; }
-        if (K) { v[K - 1] = -INFINITY; i[K - 1] = 0x7fffffff; }
-    }
-};
 __device__ __forceinline__ bool better(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
 
 template <typename T> __device__ __forceinline__ float to_f(T v) { return (float)v; }
+// 16 bytes of a row at any alignment of its type
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Loose { T v[16 / sizeof(T)]; };
 
-// calls f(index, value) for this thread's elements of [c0, c1) in rising order: single elements up to the first 16-byte boundary, then vectors, then the rest
-template <typename T, typename F, typename G>
-__device__ __forceinline__ void walk(const T* x, int c0, int c1, int tid, int threads, F one, G vec) {
-    constexpr int V = 16 / sizeof(T);
-    const int head0 = (int)((16 - ((uintptr_t)(x + c0) & 15)) & 15) / (int)sizeof(T);
-    const int head = head0 < c1 - c0 ? head0 : c1 - c0;
-    const int body = (c1 - c0 - head) / V;
-    if (tid < head) one(c0 + tid, to_f(x[c0 + tid]));
-    for (int i = tid; i < body; i += threads) vec(c0 + head + i * V);
-    const int tail = c0 + head + body * V + tid;
-    if (tail < c1) one(tail, to_f(x[tail]));
+// over the 64 lanes with DPP row operations; every lane gets the result
+__device__ __forceinline__ float readlane_f(float v, int l) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l)); }
+#define LP_DPP(v, ctrl, rows) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), ctrl, rows, 0xf, false))
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, LP_DPP(v, 0xB1, 0xf));
+    v = fmaxf(v, LP_DPP(v, 0x4E, 0xf));
+    v = fmaxf(v, LP_DPP(v, 0x141, 0xf));
+    v = fmaxf(v, LP_DPP(v, 0x140, 0xf));
+    v = fmaxf(v, LP_DPP(v, 0x142, 0xa));
+    v = fmaxf(v, LP_DPP(v, 0x143, 0xc));
+    return readlane_f(v, 63);
 }
-template <typename T> struct alignas(16) Vec { T v[16 / sizeof(T)]; };
+#undef LP_DPP
+__device__ __forceinline__ float wave_sum(float v) {
+#define LP_DPP(ctrl, rows) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, rows, 0xf, false))
+    LP_DPP(0xB1, 0xf);
+    LP_DPP(0x4E, 0xf);
+    LP_DPP(0x141, 0xf);
+    LP_DPP(0x140, 0xf);
+    LP_DPP(0x142, 0xa);
+    LP_DPP(0x143, 0xc);
+#undef LP_DPP
+    return readlane_f(v, 63);
+}
 
-// W waves per row (W = 1: four rows per workgroup); one row or share of a row per group
-template <typename T, int K, int W>
-__global__ __launch_bounds__(256) void logp_forward_kernel(LogpOp p) {
-    constexpr int V = 16 / sizeof(T), THREADS = 64 * W, GROUPS = 4 / W;
-    __shared__ State sm_state[4];
-    __shared__ float sm_v[4][K ? K : 1];
-    __shared__ int sm_i[4][K ? K : 1];
-    const int tid = threadIdx.x % THREADS, group = threadIdx.x / THREADS, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t row = (int64_t)blockIdx.x * GROUPS + group;
-    if (W == 1 && row >= p.rows) return;
-    const int share = blockIdx.y;
-    const int c0 = (int)((int64_t)p.cols * share / p.shares), c1 = (int)((int64_t)p.cols * (share + 1) / p.shares);
-    const T* x = (const T*)p.x + row * p.ld;
-    State st = empty_state();
-    Best<K> best;
-    best.clear();
-    bool bad = false;
-    auto one = [&](int at, float v) {
-        if (v != v) bad = true;
-        else if (v != -INFINITY) st = join(st, {v, 0.f, 0.f});
-        if (K) best.take(v, at);
-    };
-    walk<T>(x, c0, c1, tid, THREADS, one, [&](int at) {
-        const Vec<T> v = *(const Vec<T>*)(x + at);
-        float f[V], mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < V; ++i) { f[i] = to_f(v.v[i]); mx = fmaxf(mx, f[i]); }
-        if (mx > st.m) {                 // a new maximum of this thread: it leaves the sum, the old one enters it
-            State nw = {mx, 0.f, 0.f};
-            bool out = false;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const bool self = f[i] == mx && !out;
-                out |= self;
-                const float d = f[i] - mx, e = self || f[i] == -INFINITY ? 0.f : exp_neg(d);
-                nw.s += e;
-                nw.u -= e == 0.f ? 0.f : e * d;
-                bad |= f[i] != f[i];
-            }
-            st = join(nw, st);
-        } else if (st.m != -INFINITY) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float d = f[i] - st.m, e = exp_neg(d);
-                st.s += e;
-                st.u -= e == 0.f ? 0.f : e * d;         // NaN logits pass through e
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) bad |= f[i] != f[i];
-        }
-        if (K) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) best.take(f[i], at + i);
-        }
-    });
-    if (p.bin && share == p.shares - 1 && tid == 0) one(p.cols, *p.bin);
-    if (bad) { st.s = NAN; st.u = NAN; }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const State b = shfl_state(st, o);
-        st = (lane & o) ? join(b, st) : join(st, b);
+// a wave's list of the `top` best, place k in lane k
+struct List {
+    int top;
+    float v = -INFINITY;
+    int i = 0x7fffffff;
+    __device__ float last() const { return readlane_f(v, top - 1); }
+    // x, at: uniform; later elements have higher indices, so a tie goes behind
+    __device__ void insert(float x, int at, int lane) {
+        const int pos = __popcll(__ballot(lane < top && v >= x));
+        const float pv = __shfl_up(v, 1);
+        const int pi = __shfl_up(i, 1);
+        if (lane > pos) { v = pv; i = pi; }
+        if (lane == pos) { v = x; i = at; }
     }
-    // NaN states survive a join only through s: a lane that saw nothing but NaN has m = -inf, so the flag is carried beside it
-    const bool any_bad = __ballot(bad) != 0;
-    float bv[K ? K : 1];
-    int bi[K ? K : 1];
-    if (K) {
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            float v = best.v[0];
-            int i = best.i[0];
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const float w = __shfl_xor(v, o);
-                const int j = __shfl_xor(i, o);
-                if (better(w, j, v, i)) { v = w; i = j; }
-            }
-            bv[k] = v;
-            bi[k] = i;
-            if (best.i[0] == i) best.pop();
-        }
-    }
-    if (any_bad || st.m == INFINITY) { st.s = NAN; st.u = NAN; if (st.m == -INFINITY) st.m = 0.f; }
-    if (W > 1) {
-        if (lane == 0) {
-            sm_state[wave] = st;
-#pragma unroll
-            for (int k = 0; k < K; ++k) { sm_v[wave][k] = bv[k]; sm_i[wave][k] = bi[k]; }
-        }
-        __syncthreads();
-        if (threadIdx.x != 0) return;
-        st = sm_state[0];
-        for (int w = 1; w < W; ++w) st = join(st, sm_state[w]);
-        if (K) {
-            int at[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                int from = 0;
-                float v = -INFINITY;
-                int i = 0x7fffffff;
-                for (int w = 0; w < W; ++w)
-                    if (at[w] < K && better(sm_v[w][at[w]], sm_i[w][at[w]], v, i)) { v = sm_v[w][at[w]]; i = sm_i[w][at[w]]; from = w; }
-                for (int w = 0; w < W; ++w) at[w] += w == from;
-                bv[k] = v;
-                bi[k] = i;
-            }
-        }
-    } else if (lane != 0) return;
-    if (p.shares > 1) {
-        const int64_t at = row * p.shares + share;
-        p.part[3 * at] = st.m;
-        p.part[3 * at + 1] = st.s;
-        p.part[3 * at + 2] = st.u;
-#pragma unroll
-        for (int k = 0; k < K; ++k) { p.part_v[at * K + k] = bv[k]; p.part_i[at * K + k] = bi[k]; }
-        return;
-    }
+};
+
+// what a row's state says, and its target's log probability (one lane)
+template <typename T> __device__ __forceinline__ void finish(const LogpOp& p, int64_t row, const State& st) {
     const float l = log1pf(st.s);
     const bool none = st.m == -INFINITY;
     p.stats[2 * row] = st.m;
@@ -216,68 +107,243 @@ __global__ __launch_bounds__(256) void logp_forward_kernel(LogpOp p) {
     p.entropy[row] = none ? 0.f : l + st.u / (1.f + st.s);
     const int64_t t = p.target[row];
     float lp = 0.f;
-    if (t >= 0 && t < p.cols) lp = none ? -INFINITY : (to_f(x[t]) - st.m) - l;
+    if (t >= 0 && t < p.cols) lp = none ? -INFINITY : (to_f(((const T*)p.x)[row * p.ld + t]) - st.m) - l;
     else if (p.bin && (t == -1 || t == p.cols)) lp = none ? -INFINITY : (*p.bin - st.m) - l;
     else if (t != -1 && t != -2) lp = NAN;
     p.logp[row] = lp;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-        if (k < p.top) {
-            const bool has = bv[k] != -INFINITY;
-            p.top_logp[row * p.top + k] = has ? (bv[k] - st.m) - l : -INFINITY;
-            p.top_id[row * p.top + k] = has ? bi[k] : -1;
-        }
 }
 
-// joins the shares of a row (one wave per row)
-template <typename T, int K>
+__device__ __forceinline__ void write_top(const LogpOp& p, int64_t row, int k, const State& st, float v, int i) {
+    const bool has = v != -INFINITY;
+    p.top_logp[row * p.top + k] = has ? (v - st.m) - log1pf(st.s) : -INFINITY;
+    p.top_id[row * p.top + k] = has ? i : -1;
+}
+
+// W waves per row (W = 1: four rows per workgroup); one row or share of a row per group.  U: vectors per lane in a piece
+template <typename T, bool TOP, int W, int U>
+__global__ __launch_bounds__(256) void logp_forward_kernel(LogpOp p) {
+    constexpr int V = 16 / sizeof(T), GROUPS = 4 / W;
+    __shared__ State sm_state[4];
+    __shared__ float sm_v[4][TOP_MAX];
+    __shared__ int sm_i[4][TOP_MAX];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = wave % W;
+    const int64_t row = (int64_t)blockIdx.x * GROUPS + wave / W;
+    if (W == 1 && row >= p.rows) return;
+    const int share = blockIdx.y;
+    const int c0 = (int)((int64_t)p.cols * share / p.shares), c1 = (int)((int64_t)p.cols * (share + 1) / p.shares);
+    const T* x = (const T*)p.x + row * p.ld;
+    // sums per lane, without the wave's largest element m: s = sum e, u = sum e (m - x)
+    float m = -INFINITY, s = 0.f, u = 0.f;
+    List list{p.top};
+    bool bad = false;
+    for (int base = c0; base < c1; base += 64 * W * V * U) {
+        float f[U][V], vm[U];
+        // vector j of a lane: columns at + 0 .. V - 1; in rising order over (j, wave, lane)
+        auto col = [&](int j) { return base + ((j * W + part) * 64 + lane) * V; };
+        Loose<T> raw[U];
+        if (base + 64 * W * V * U <= c1) {
+#pragma unroll
+            for (int j = 0; j < U; ++j) raw[j] = *(const Loose<T>*)(x + col(j));
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+#pragma unroll
+                for (int i = 0; i < V; ++i) f[j][i] = to_f(raw[j].v[i]);
+        } else {                         // the last piece: places past the end hold -inf
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+                if (col(j) + V <= c1) raw[j] = *(const Loose<T>*)(x + col(j));
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                const int at = col(j);
+#pragma unroll
+                for (int i = 0; i < V; ++i) f[j][i] = at + V <= c1 ? to_f(raw[j].v[i]) : -INFINITY;
+                if (at + V > c1 && at < c1) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) if (at + i < c1) f[j][i] = to_f(x[at + i]);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            vm[j] = f[j][0];
+#pragma unroll
+            for (int i = 1; i < V; ++i) vm[j] = fmaxf(vm[j], f[j][i]);
+        }
+        float best = vm[0];
+#pragma unroll
+        for (int j = 1; j < U; ++j) best = fmaxf(best, vm[j]);
+        const float top = wave_max(best);
+        // the first place of `top`: its lane and vector, in the order of the columns
+        auto first_of = [&](float mine, float v, int& jl) {
+            int j0 = U;
+#pragma unroll
+            for (int j = U - 1; j >= 0; --j) j0 = vm[j] == v ? j : j0;
+            unsigned long long who = __ballot(mine == v);
+            if (who & (who - 1)) {       // several lanes: the lowest vector, then the lowest lane
+                for (int j = 0; j < U; ++j) {
+                    const unsigned long long w = __ballot(mine == v && j0 == j);
+                    if (w) { who = w; break; }
+                }
+            }
+            const int l = __builtin_ctzll(who);
+            jl = __builtin_amdgcn_readlane(j0, l);
+            return l;
+        };
+        // the first place of value v in vector jl of lane l, and another value for a place
+        auto place_of = [&](int l, int jl, float v) {
+            int place = 0;
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+                if (j == jl) {
+#pragma unroll
+                    for (int i = V - 1; i >= 0; --i) place = f[j][i] == v ? i : place;
+                }
+            return __builtin_amdgcn_readlane(place, l);
+        };
+        auto put = [&](int l, int jl, int at, float v) {
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+                if (j == jl) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) f[j][i] = lane == l && i == at ? v : f[j][i];
+                    vm[j] = f[j][0];
+#pragma unroll
+                    for (int i = 1; i < V; ++i) vm[j] = fmaxf(vm[j], f[j][i]);
+                }
+        };
+        int out_l = 0, out_j = 0, out_i = 0;
+        bool out = false;
+        if (top > m) {                   // (uniform) a new largest element: it leaves the sum, the old one enters it
+            if (m != -INFINITY) {
+                const float d = fminf(top - m, 1e30f), g = exp_neg(-d);
+                u = g * __builtin_fmaf(d, s, u);
+                s *= g;
+                if (lane == 0) { s += g; u = __builtin_fmaf(g, d, u); }
+            }
+            m = top;
+            out = true;
+            out_l = first_of(best, top, out_j);
+            out_i = place_of(out_l, out_j, top);
+            put(out_l, out_j, out_i, -INFINITY);
+        }
+        if (m != -INFINITY) {
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float d = f[j][i] - m, e = exp_neg(d);
+                    s += e;
+                    u = __builtin_fmaf(-e, fmaxf(d, -1e30f), u);      // (a masked column: e = 0)
+                }
+        } else {
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+#pragma unroll
+                for (int i = 0; i < V; ++i) bad |= f[j][i] != f[j][i];
+        }
+        if constexpr (TOP) {
+            if (out) put(out_l, out_j, out_i, m);
+            for (float last = list.last();;) {
+                best = vm[0];
+#pragma unroll
+                for (int j = 1; j < U; ++j) best = fmaxf(best, vm[j]);
+                const float v = wave_max(best);
+                if (!(v > last)) break;
+                int jl;
+                const int l = first_of(best, v, jl);
+                const int i = place_of(l, jl, v);
+                put(l, jl, i, -INFINITY);
+                list.insert(v, base + ((jl * W + part) * 64 + l) * V + i, lane);
+                last = list.last();
+            }
+        }
+    }
+    if (TOP && p.bin && share == p.shares - 1 && part == W - 1 && *p.bin > list.last()) list.insert(*p.bin, p.cols, lane);
+    s = wave_sum(s);
+    u = wave_sum(u);
+    State st = {m, s, u};
+    if (p.bin && share == p.shares - 1 && part == W - 1) {
+        const float v = *p.bin;
+        if (v != v) bad = true;
+        else if (v != -INFINITY) st = join(st, {v, 0.f, 0.f});
+    }
+    // (a wave that saw nothing but NaN has m = -inf)
+    if (__ballot(bad) || st.m == INFINITY) { st.s = NAN; st.u = NAN; if (st.m == -INFINITY) st.m = 0.f; }
+    if (W > 1) {
+        if (lane == 0) sm_state[wave] = st;
+        if (TOP && lane < p.top) { sm_v[wave][lane] = list.v; sm_i[wave][lane] = list.i; }
+        __syncthreads();
+        if (wave != 0) return;
+        st = sm_state[0];
+        for (int w = 1; w < W; ++w) st = join(st, sm_state[w]);
+        if (TOP) {                       // the lists in the order of their waves' columns is not that of all columns: merged by value and index
+            int at[4] = {0, 0, 0, 0};
+            float mine = -INFINITY;
+            int mi = 0x7fffffff;
+            for (int k = 0; k < p.top; ++k) {
+                int from = 0;
+                float v = -INFINITY;
+                int i = 0x7fffffff;
+#pragma unroll
+                for (int w = 0; w < W; ++w)
+                    if (at[w] < p.top && better(sm_v[w][at[w]], sm_i[w][at[w]], v, i)) { v = sm_v[w][at[w]]; i = sm_i[w][at[w]]; from = w; }
+#pragma unroll
+                for (int w = 0; w < W; ++w) at[w] += w == from;
+                if (lane == k) { mine = v; mi = i; }
+            }
+            list.v = mine;
+            list.i = mi;
+        }
+    }
+    if (p.shares > 1) {
+        const int64_t at = row * p.shares + share;
+        if (lane == 0) {
+            p.part[3 * at] = st.m;
+            p.part[3 * at + 1] = st.s;
+            p.part[3 * at + 2] = st.u;
+        }
+        if (TOP && lane < p.top) { p.part_v[at * p.top + lane] = list.v; p.part_i[at * p.top + lane] = list.i; }
+        return;
+    }
+    if (lane == 0) finish<T>(p, row, st);
+    if (TOP && lane < p.top) write_top(p, row, lane, st, list.v, list.i);
+}
+
+// joins the shares of a row (one wave per row, a share per lane: its list is walked through a place at a time)
+template <typename T>
 __global__ __launch_bounds__(256) void logp_join_kernel(LogpOp p) {
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (row >= p.rows) return;
     State st = empty_state();
-    Best<K> best;
-    best.clear();
-    if (lane < p.shares) {
-        const int64_t at = row * p.shares + lane;
-        st = {p.part[3 * at], p.part[3 * at + 1], p.part[3 * at + 2]};
-#pragma unroll
-        for (int k = 0; k < K; ++k) { best.v[k] = p.part_v[at * K + k]; best.i[k] = p.part_i[at * K + k]; }
-    }
+    const int64_t at = row * p.shares + lane;
+    if (lane < p.shares) st = {p.part[3 * at], p.part[3 * at + 1], p.part[3 * at + 2]};
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const State b = shfl_state(st, o);
         st = (lane & o) ? join(b, st) : join(st, b);
     }
-    const float l = log1pf(st.s);
-    const bool none = st.m == -INFINITY;
+    int place = 0;
+    auto head = [&](float& v, int& i) {
+        const bool in = lane < p.shares && place < p.top;
+        v = in ? p.part_v[at * p.top + place] : -INFINITY;
+        i = in ? p.part_i[at * p.top + place] : 0x7fffffff;
+    };
+    float hv = -INFINITY;
+    int hi = 0x7fffffff;
+    if (p.top) head(hv, hi);
     for (int k = 0; k < p.top; ++k) {
-        float v = K ? best.v[0] : -INFINITY;
-        int i = K ? best.i[0] : 0x7fffffff;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const float w = __shfl_xor(v, o);
-            const int j = __shfl_xor(i, o);
-            if (better(w, j, v, i)) { v = w; i = j; }
-        }
-        if (K && best.i[0] == i) best.pop();
-        if (lane == 0) {
-            const bool has = v != -INFINITY;
-            p.top_logp[row * p.top + k] = has ? (v - st.m) - l : -INFINITY;
-            p.top_id[row * p.top + k] = has ? i : -1;
+        const float v = wave_max(hv);
+        // shares lie in the order of their columns: the first lane with the value has the lowest index
+        const int l = __builtin_ctzll(__ballot(hv == v));
+        const int i = __builtin_amdgcn_readlane(hi, l);
+        if (lane == 0) write_top(p, row, k, st, v, i);
+        if (lane == l) {
+            ++place;
+            head(hv, hi);
         }
     }
-    if (lane) return;
-    p.stats[2 * row] = st.m;
-    p.stats[2 * row + 1] = l;
-    p.entropy[row] = none ? 0.f : l + st.u / (1.f + st.s);
-    const int64_t t = p.target[row];
-    const T* x = (const T*)p.x + row * p.ld;
-    float lp = 0.f;
-    if (t >= 0 && t < p.cols) lp = none ? -INFINITY : (to_f(x[t]) - st.m) - l;
-    else if (p.bin && (t == -1 || t == p.cols)) lp = none ? -INFINITY : (*p.bin - st.m) - l;
-    else if (t != -1 && t != -2) lp = NAN;
-    p.logp[row] = lp;
+    if (lane == 0) finish<T>(p, row, st);
 }
 
 // dx of one row, or of a share of it
@@ -307,22 +373,31 @@ __global__ __launch_bounds__(256) void logp_backward_kernel(LogpOp p) {
         return (at == ti ? -g * expm1f(lp) : -g * pr) - ent;
     };
     if (dx) {
-        if ((((uintptr_t)x ^ (uintptr_t)dx) & 15) == 0) {
-            walk<T>(x, c0, c1, tid, THREADS, [&](int at, float v) { dx[at] = (T)grad(at, v); },
-                    [&](int at) {
-                        const Vec<T> v = *(const Vec<T>*)(x + at);
-                        Vec<T> o;
-                        if (ti >= at && ti < at + V) {
+        constexpr int U = 4;             // vectors under way per thread
+        for (int base = c0; base < c1; base += THREADS * V * U) {
+            Loose<T> v[U];
 #pragma unroll
-                            for (int i = 0; i < V; ++i) o.v[i] = (T)grad(at + i, to_f(v.v[i]));
-                        } else {
+            for (int j = 0; j < U; ++j) {
+                const int at = base + (j * THREADS + tid) * V;
+                if (at + V <= c1) v[j] = *(const Loose<T>*)(x + at);
+            }
 #pragma unroll
-                            for (int i = 0; i < V; ++i) o.v[i] = (T)grad(-2, to_f(v.v[i]));
-                        }
-                        *(Vec<T>*)(dx + at) = o;
-                    });
-        } else {
-            for (int i = c0 + tid; i < c1; i += THREADS) dx[i] = (T)grad(i, to_f(x[i]));
+            for (int j = 0; j < U; ++j) {
+                const int at = base + (j * THREADS + tid) * V;
+                if (at + V <= c1) {
+                    Loose<T> o;
+                    if (ti >= at && ti < at + V) {
+#pragma unroll
+                        for (int i = 0; i < V; ++i) o.v[i] = (T)grad(at + i, to_f(v[j].v[i]));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < V; ++i) o.v[i] = (T)grad(-2, to_f(v[j].v[i]));
+                    }
+                    *(Loose<T>*)(dx + at) = o;
+                } else if (at < c1) {
+                    for (int i = at; i < c1; ++i) dx[i] = (T)grad(i, to_f(x[i]));
+                }
+            }
         }
     }
     if (p.bin && p.part_bin && share == 0 && tid == 0) p.part_bin[row] = (double)grad(p.cols, *p.bin);
@@ -348,7 +423,6 @@ int shares_of(int64_t rows, int cols) {
     const int64_t s = want < most ? want : most;
     return s < 1 ? 1 : (s > 64 ? 64 : (int)s);
 }
-int padded_top(int top) { return top == 0 ? 0 : top <= 1 ? 1 : top <= 4 ? 4 : top <= 8 ? 8 : TOP_MAX; }
 // a wave per row where rows are short or there are plenty of them; four waves otherwise
 bool wave_rows(int64_t rows, int cols) { return cols <= 512 || (cols <= 4096 && rows >= 4096); }
 
@@ -366,19 +440,24 @@ int ready(int device) {
     return e == hipSuccess ? 0 : imp_fail(IMP_E_HIP, hipGetErrorString(e));
 }
 
-template <typename T, int K> void forward(const LogpOp& p, hipStream_t st) {
-    if (p.shares == 1 && wave_rows(p.rows, p.cols)) logp_forward_kernel<T, K, 1><<<dim3((unsigned)((p.rows + 3) / 4), 1), 256, 0, st>>>(p);
-    else logp_forward_kernel<T, K, 4><<<dim3((unsigned)p.rows, (unsigned)p.shares), 256, 0, st>>>(p);
-    if (p.shares > 1) logp_join_kernel<T, K><<<(unsigned)((p.rows + 3) / 4), 256, 0, st>>>(p);
+// pieces of 2 vectors per lane, or of 32 elements: short rows do not pay for places that they leave empty
+template <typename T, bool TOP> void forward(const LogpOp& p, hipStream_t st) {
+    constexpr int V = 16 / sizeof(T), U = 32 / V;
+    const int per = (p.cols + p.shares - 1) / p.shares;
+    if (p.shares == 1 && wave_rows(p.rows, p.cols)) {
+        const unsigned grid = (unsigned)((p.rows + 3) / 4);
+        if (per <= 64 * V * 2) logp_forward_kernel<T, TOP, 1, 2><<<grid, 256, 0, st>>>(p);
+        else logp_forward_kernel<T, TOP, 1, U><<<grid, 256, 0, st>>>(p);
+    } else {
+        const dim3 grid((unsigned)p.rows, (unsigned)p.shares);
+        if (per <= 256 * V * 2) logp_forward_kernel<T, TOP, 4, 2><<<grid, 256, 0, st>>>(p);
+        else logp_forward_kernel<T, TOP, 4, U><<<grid, 256, 0, st>>>(p);
+    }
+    if (p.shares > 1) logp_join_kernel<T><<<(unsigned)((p.rows + 3) / 4), 256, 0, st>>>(p);
 }
 template <typename T> void forward_top(const LogpOp& p, hipStream_t st) {
-    switch (padded_top(p.top)) {
-        case 0: forward<T, 0>(p, st); break;
-        case 1: forward<T, 1>(p, st); break;
-        case 4: forward<T, 4>(p, st); break;
-        case 8: forward<T, 8>(p, st); break;
-        default: forward<T, TOP_MAX>(p, st);
-    }
+    if (p.top) forward<T, true>(p, st);
+    else forward<T, false>(p, st);
 }
 template <typename T> void backward(const LogpOp& p, hipStream_t st) {
     if (p.shares == 1 && wave_rows(p.rows, p.cols)) logp_backward_kernel<T, 1><<<dim3((unsigned)((p.rows + 3) / 4), 1), 256, 0, st>>>(p);
@@ -393,7 +472,7 @@ int imp_log_probs_workspace(int64_t rows, int cols, int top, int backward, uint6
     if (!bytes || rows < 1 || cols < 0 || top < 0 || top > TOP_MAX) return imp_fail(IMP_E_ARG, "imp_log_probs_workspace: bad argument");
     const int s = shares_of(rows, cols);
     if (backward) *bytes = (uint64_t)rows * 8;
-    else *bytes = s > 1 ? (uint64_t)rows * s * (12 + 8 * padded_top(top)) : 0;
+    else *bytes = s > 1 ? (uint64_t)rows * s * (12 + 8 * top) : 0;
     return IMP_OK;
 }
 
@@ -411,7 +490,7 @@ int imp_log_probs_forward(int dtype, int64_t rows, int cols, int64_t ld, const v
     p.rows = rows; p.ld = ld; p.cols = cols; p.top = top; p.shares = shares_of(rows, cols);
     p.part = (float*)workspace;
     p.part_v = p.part + 3 * rows * p.shares;
-    p.part_i = (int*)(p.part_v + rows * p.shares * padded_top(top));
+    p.part_i = (int*)(p.part_v + rows * p.shares * top);
     const hipStream_t st = (hipStream_t)stream;
     if (dtype == IMP_DTYPE_F32) forward_top<float>(p, st);
     else if (dtype == IMP_DTYPE_F16) forward_top<_Float16>(p, st);
