@@ -184,8 +184,8 @@ def lib():
     L.imp_sp_op_conv.argtypes = [P, I, P, I, I, I, P, I, I, P]
     U, L64 = C.c_uint64, C.c_int64
     L.imp_attn_workspace.argtypes = [C.POINTER(ImpAttnDesc), I, C.POINTER(U)]
-    L.imp_attn_forward.argtypes = [C.POINTER(ImpAttnDesc), P, P, P, P, P, P, U, I, P]
-    L.imp_attn_backward.argtypes = [C.POINTER(ImpAttnDesc), P, P, P, P, P, P, P, P, P, P, U, I, P]
+    L.imp_attn_forward.argtypes = [C.POINTER(ImpAttnDesc), P, P, P, P, P, P, P, U, I, P]
+    L.imp_attn_backward.argtypes = [C.POINTER(ImpAttnDesc), P, P, P, P, P, P, P, P, P, P, P, U, I, P]
     L.imp_group_norm_act_workspace.argtypes = [I, I, I, I, I, I, C.POINTER(U)]
     L.imp_group_norm_act_forward.argtypes = [I, I, I, I, I, P, P, P, P, F, I, P, P, P, U, I, P]
     L.imp_group_norm_act_backward.argtypes = [I, I, I, I, I, P, P, P, P, I, P, P, P, P, P, P, U, I, P]

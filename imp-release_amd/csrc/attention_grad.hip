@@ -17,7 +17,8 @@
 // Few rows: the walk is cut in shares (partials in the caller's workspace, joined in a fixed order by a second launch).
 //
 // Arithmetic (accumulators, softmax statistics and D in fp32; what the operands of the products are rounded to):
-//   bf16  one bf16 MFMA per product; P and dS rounded to bf16, half a step of 2^-8: the inputs' own precision
+//   bf16  one bf16 MFMA per product; P and dS rounded to bf16, half a step of 2^-8: the inputs' own precision.  D is formed from the unrounded O (the forward also writes
+//         what rounding left of it): taken from the rounded one it put as much error into dQ and dK of few keys as all other roundings together
 //   fp16  one f16 MFMA; P carries a factor 2^10 (weights of long rows stay normal numbers) and dS a power of two per owned row, raised or lowered as the walk meets larger
 //         values (LaneScale), so that gradients far below the fp16 range keep their bits
 //   fp32, many rows: split halves as in the inference kernels (x = hi + lo in f16, 22 bits, three MFMAs), each tensor scaled per key head by a power of two that a first
@@ -42,8 +43,8 @@ constexpr int OWN = 128;                 // owned rows per workgroup
 constexpr int SPLIT_ROWS = 256;          // fp32: rows and keys from which the split halves' extra launch pays
 
 struct AttnOp {
-    const void *q, *k, *v, *out, *dout;  // out: read by the backward
-    void *o, *dq, *dk, *dv;
+    const void *q, *k, *v, *out, *rest, *dout;      // out and what its rounding left: read by the backward
+    void *o, *orest, *dq, *dk, *dv;
     float *lse, *delta, *part, *part_lse;
     const uint8_t* mask;
     const int32_t *q_lens, *k_lens;
@@ -174,6 +175,9 @@ template <typename T> __device__ __forceinline__ void store4(T* p, float a, floa
         *(v4*)p = v4{(T)a, (T)b, (T)c, (T)d};
     }
 }
+
+// what rounding to T leaves of a value
+template <typename T> __device__ __forceinline__ float left_of(float x) { return x - (float)(T)x; }
 
 __device__ __forceinline__ int clamp_len(const int32_t* lens, int b, int n) { return lens ? min(max(lens[b], 0), n) : n; }
 
@@ -566,7 +570,11 @@ __global__ __launch_bounds__(256, A::NP == 3 && DHP == 128 ? 1 : 2) void attn_fw
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int col = 32 * d + 8 * g + 4 * half;
-                if (col < p.dh) store4(out + col, o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv);
+                if (col < p.dh) {
+                    const float x0 = o[d][4 * g] * inv, x1 = o[d][4 * g + 1] * inv, x2 = o[d][4 * g + 2] * inv, x3 = o[d][4 * g + 3] * inv;
+                    store4(out + col, x0, x1, x2, x3);
+                    if (sizeof(T) == 2 && p.orest) store4((T*)p.orest + row * p.dh + col, left_of<T>(x0), left_of<T>(x1), left_of<T>(x2), left_of<T>(x3));
+                }
             }
         if (!half && p.lse) p.lse[stat_row(p, b, hk, r)] = lse;
     }
@@ -593,7 +601,10 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnOp p) {
             const float ws = __shfl(w, s);
             if (c < p.dh && ws != 0.f) acc += ws * p.part[(s * rows + row) * p.dh + c];
         }
-        if (c < p.dh) ((T*)p.o)[row * p.dh + c] = (T)(acc * inv);
+        if (c < p.dh) {
+            ((T*)p.o)[row * p.dh + c] = (T)(acc * inv);
+            if (sizeof(T) == 2 && p.orest) ((T*)p.orest)[row * p.dh + c] = (T)left_of<T>(acc * inv);
+        }
     }
     if (lane == 0 && p.lse) {
         const int h = (int)(row % p.H);
@@ -617,6 +628,14 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(AttnOp p) {
         float x[8], y[8];
         a.get(x);
         b.get(y);
+        if (sizeof(T) == 2 && p.rest) {
+            Chunk<T> r;
+            r.load((const T*)p.rest + row * p.dh + col);
+            float z[8];
+            r.get(z);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] += z[i];
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(x[i], y[i], sum);
     }
@@ -1078,11 +1097,13 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
     store_dkv<T, DT>(p, b, hk, key, share, 64 * h, half, dk, dv, p.scale * unp * (A::LANE ? ls.inverse() : 1.f), unp);
 }
 
-// out[i] = sum over the shares, in their order (4 elements per thread; n % 4 == 0)
+// out[i] = sum over the shares, in their order (4 elements per thread; n % 4 == 0); blockIdx.y: dk, dv
 template <typename T>
-__global__ __launch_bounds__(256) void attn_sum_kernel(const float* part, int64_t n, int64_t stride, int shares, T* out) {
+__global__ __launch_bounds__(256) void attn_sum_kernel(const float* part, int64_t n, int64_t stride, int shares, T* out0, T* out1) {
     const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= n) return;
+    T* out = blockIdx.y ? out1 : out0;
+    part += blockIdx.y * n;
     f32x4 a = *(const f32x4*)(part + i);
     for (int s = 1; s < shares; ++s) a += *(const f32x4*)(part + s * stride + i);
     store4(out + i, a[0], a[1], a[2], a[3]);
@@ -1202,16 +1223,16 @@ int imp_attn_workspace(const imp_attn_desc* d, int backward, uint64_t* bytes) {
     return IMP_OK;
 }
 
-int imp_attn_forward(const imp_attn_desc* d, const void* q, const void* k, const void* v, void* out, float* lse, void* workspace, uint64_t workspace_bytes,
-                     int device, void* stream) {
+int imp_attn_forward(const imp_attn_desc* d, const void* q, const void* k, const void* v, void* out, void* out_rest, float* lse, void* workspace,
+                     uint64_t workspace_bytes, int device, void* stream) {
     if (const char* why = bad_desc(d)) return imp_fail(IMP_E_ARG, why);
     if (!q || !k || !v || !out) return imp_fail(IMP_E_ARG, "imp_attn_forward: null argument");
     const Plan pl = plan(*d);
-    if (unaligned({q, k, v, out, workspace})) return imp_fail(IMP_E_ARG, "imp_attn_forward: pointers must be aligned to 16 bytes");
+    if (unaligned({q, k, v, out, out_rest, workspace})) return imp_fail(IMP_E_ARG, "imp_attn_forward: pointers must be aligned to 16 bytes");
     if (workspace_bytes < pl.fwd_bytes || (pl.fwd_bytes && !workspace)) return imp_fail(IMP_E_NOMEM, "imp_attn_forward: workspace too small (imp_attn_workspace)");
     if (int rc = on_device(device)) return rc;
     AttnOp p = op_of(*d);
-    p.q = q; p.k = k; p.v = v; p.o = out; p.lse = lse;
+    p.q = q; p.k = k; p.v = v; p.o = out; p.orest = out_rest; p.lse = lse;
     p.shares = pl.fwd;
     p.amax = (float*)workspace;
     p.chunks = pl.chunks;
@@ -1229,16 +1250,16 @@ int imp_attn_forward(const imp_attn_desc* d, const void* q, const void* k, const
     return launched("imp_attn_forward");
 }
 
-int imp_attn_backward(const imp_attn_desc* d, const void* q, const void* k, const void* v, const void* out, const float* lse, const void* dout, void* dq,
-                      void* dk, void* dv, void* workspace, uint64_t workspace_bytes, int device, void* stream) {
+int imp_attn_backward(const imp_attn_desc* d, const void* q, const void* k, const void* v, const void* out, const void* out_rest, const float* lse,
+                      const void* dout, void* dq, void* dk, void* dv, void* workspace, uint64_t workspace_bytes, int device, void* stream) {
     if (const char* why = bad_desc(d)) return imp_fail(IMP_E_ARG, why);
     if (!q || !k || !v || !out || !lse || !dout || (!dq && !dk && !dv) || (!dk != !dv)) return imp_fail(IMP_E_ARG, "imp_attn_backward: null argument");
     const Plan pl = plan(*d);
-    if (unaligned({q, k, v, out, dout, dq, dk, dv, workspace})) return imp_fail(IMP_E_ARG, "imp_attn_backward: pointers must be aligned to 16 bytes");
+    if (unaligned({q, k, v, out, out_rest, dout, dq, dk, dv, workspace})) return imp_fail(IMP_E_ARG, "imp_attn_backward: pointers must be aligned to 16 bytes");
     if (workspace_bytes < pl.bwd_bytes || !workspace) return imp_fail(IMP_E_NOMEM, "imp_attn_backward: workspace too small (imp_attn_workspace)");
     if (int rc = on_device(device)) return rc;
     AttnOp p = op_of(*d);
-    p.q = q; p.k = k; p.v = v; p.out = out; p.lse = const_cast<float*>(lse); p.dout = dout; p.dq = dq; p.dk = dk; p.dv = dv;
+    p.q = q; p.k = k; p.v = v; p.out = out; p.rest = out_rest; p.lse = const_cast<float*>(lse); p.dout = dout; p.dq = dq; p.dk = dk; p.dv = dv;
     p.amax = (float*)workspace;
     p.chunks = pl.chunks;
     p.delta = (float*)((char*)workspace + pl.amax_bytes);
@@ -1255,22 +1276,22 @@ int imp_attn_backward(const imp_attn_desc* d, const void* q, const void* k, cons
         using T = std::remove_pointer_t<decltype(t)>;
         attn_delta_kernel<T><<<(unsigned)((pl.q_rows + 15) / 16), 256, 0, st>>>(p);
     });
-    auto join = [&](int64_t rows, int parts, int which, void* to) {
+    auto join = [&](int64_t rows, int parts, void* to0, void* to1) {
         const int64_t n = rows * d->head_dim;
         each([&](auto* t) {
             using T = std::remove_pointer_t<decltype(t)>;
-            attn_sum_kernel<T><<<(unsigned)((n / 4 + 255) / 256), 256, 0, st>>>(p.part + which * n, n, parts * n, p.shares, (T*)to);
+            attn_sum_kernel<T><<<dim3((unsigned)((n / 4 + 255) / 256), parts), 256, 0, st>>>(p.part, n, parts * n, p.shares, (T*)to0, (T*)to1);
         });
     };
     if (dk) {
         p.shares = pl.dkv;
         launch_any(dt, pl.split, 2, p, st);
-        if (p.shares > 1) { join(pl.k_rows, 2, 0, dk); join(pl.k_rows, 2, 1, dv); }
+        if (p.shares > 1) join(pl.k_rows, 2, dk, dv);
     }
     if (dq) {
         p.shares = pl.dq;
         launch_any(dt, pl.split, 1, p, st);
-        if (p.shares > 1) join(pl.q_rows, 1, 0, dq);
+        if (p.shares > 1) join(pl.q_rows, 1, dq, nullptr);
     }
     return launched("imp_attn_backward");
 }

@@ -323,11 +323,16 @@ __global__ __launch_bounds__(256) void logp_join_kernel(LogpOp p) {
         const State b = shfl_state(st, o);
         st = (lane & o) ? join(b, st) : join(st, b);
     }
+    __shared__ float lv[4][64 * TOP_MAX];
+    __shared__ int li[4][64 * TOP_MAX];
+    const int wave = threadIdx.x >> 6;
+    for (int i = lane; i < p.shares * p.top; i += 64) { lv[wave][i] = p.part_v[row * p.shares * p.top + i]; li[wave][i] = p.part_i[row * p.shares * p.top + i]; }
+    __builtin_amdgcn_wave_barrier();     // (a wave reads only what it wrote)
     int place = 0;
     auto head = [&](float& v, int& i) {
         const bool in = lane < p.shares && place < p.top;
-        v = in ? p.part_v[at * p.top + place] : -INFINITY;
-        i = in ? p.part_i[at * p.top + place] : 0x7fffffff;
+        v = in ? lv[wave][lane * p.top + place] : -INFINITY;
+        i = in ? li[wave][lane * p.top + place] : 0x7fffffff;
     };
     float hv = -INFINITY;
     int hi = 0x7fffffff;
@@ -417,9 +422,9 @@ __global__ __launch_bounds__(1024) void logp_bin_kernel(const double* part, int6
 }
 
 // ------------------------------------------------------------------------------------------------------------------------- host
-// shares of a row: enough workgroups for four per CU, each with at least 4096 columns; at most 64 (a lane each in the join)
+// shares of a row: enough workgroups for four per CU, each with at least 2048 columns; at most 64 (a lane each in the join)
 int shares_of(int64_t rows, int cols) {
-    const int64_t want = (1024 + rows - 1) / rows, most = cols / 4096;
+    const int64_t want = (1024 + rows - 1) / rows, most = cols / 2048;
     const int64_t s = want < most ? want : most;
     return s < 1 ? 1 : (s > 64 ? 64 : (int)s);
 }

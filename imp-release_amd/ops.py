@@ -60,6 +60,20 @@ def _where(t):
     return i, torch._C._cuda_getCurrentRawStream(i)
 
 
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _once(backward):
+    """torch's once_differentiable, which only does something where a graph of the backward pass is asked for: left out where it is not"""
+    guarded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def call(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return call
+
+
 def _dense(t, dtype):
     """a gradient as the kernels take it"""
     if t.dtype != dtype:
@@ -112,33 +126,33 @@ def _attn_desc(q, k, v, mask, q_lens, k_lens, scale):
     return d, fwd, bwd
 
 
-def _attn_forward(q, k, v, mask, q_lens, k_lens, scale, want_lse):
+def _attn_forward(q, k, v, mask, q_lens, k_lens, scale, want_lse, want_rest=False):
     d, need, _ = _attn_desc(q, k, v, mask, q_lens, k_lens, scale)
     out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    rest = torch.empty_like(out) if want_rest else None
     lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), device=q.device, dtype=torch.float32) if want_lse else None
     ws = _scratch(need, q.device)
-    _check(_lib.lib().imp_attn_forward(d, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if want_lse else None,
-                                       ws.data_ptr() if need else None, need, *_where(q)))
-    return out, lse
+    _check(_lib.lib().imp_attn_forward(d, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _at(rest), _at(lse), _at(ws), need, *_where(q)))
+    return out, rest, lse
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, q_lens, k_lens, scale):
         q, k, v = _rows(q), _rows(k), _rows(v)
-        out, lse = _attn_forward(q, k, v, mask, q_lens, k_lens, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, mask, q_lens, k_lens)
+        out, rest, lse = _attn_forward(q, k, v, mask, q_lens, k_lens, scale, True, q.dtype != torch.float32)
+        ctx.save_for_backward(q, k, v, out, rest, lse, mask, q_lens, k_lens)
         ctx.scale = scale
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
         return out, lse
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout, _):
         if dout is None:
             return None, None, None, None, None, None, None
-        q, k, v, out, lse, mask, q_lens, k_lens = ctx.saved_tensors
+        q, k, v, out, rest, lse, mask, q_lens, k_lens = ctx.saved_tensors
         dout = _dense(dout, out.dtype)
         d, _, need = _attn_desc(q, k, v, mask, q_lens, k_lens, ctx.scale)
         want_q, want_k, want_v = ctx.needs_input_grad[:3]
@@ -146,11 +160,10 @@ class _Attention(torch.autograd.Function):
         dk = dv = None
         if want_k or want_v:
             dk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
-            dv = torch.empty(v.shape, device=v.device, dtype=v.dtype)
+            dv = torch.empty_like(dk)
         ws = _scratch(need, q.device)
-        _check(_lib.lib().imp_attn_backward(d, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
-                                            dq.data_ptr() if want_q else None, None if dk is None else dk.data_ptr(), None if dv is None else dv.data_ptr(),
-                                            ws.data_ptr(), need, *_where(q)))
+        _check(_lib.lib().imp_attn_backward(d, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _at(rest), lse.data_ptr(), dout.data_ptr(), _at(dq), _at(dk),
+                                            _at(dv), ws.data_ptr(), need, *_where(q)))
         return dq, dk if want_k else None, dv if want_v else None, None, None, None, None
 
 
@@ -188,7 +201,7 @@ def attention(q, k, v, key_mask: Optional[torch.Tensor] = None, q_lens=None, k_l
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _Attention.apply(q, k, v, key_mask, q_lens, k_lens, scale)
     else:
-        out, lse = _attn_forward(_rows(q), _rows(k), _rows(v), key_mask, q_lens, k_lens, scale, return_lse)
+        out, _, lse = _attn_forward(_rows(q), _rows(k), _rows(v), key_mask, q_lens, k_lens, scale, return_lse)
     return (out, lse) if return_lse else out
 
 
@@ -198,10 +211,6 @@ def _norm_scratch(dtype, b, n, c, groups, backward):
     need = C.c_uint64()
     _check(_lib.lib().imp_group_norm_act_workspace(dtype, b, n, c, groups, backward, C.byref(need)))
     return need.value
-
-
-def _at(t):
-    return None if t is None else t.data_ptr()
 
 
 def _norm_forward(x, weight, bias, lens, groups, eps, act):
@@ -225,7 +234,7 @@ class _GroupNormAct(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         x, weight, bias, lens, stats = ctx.saved_tensors
         b, n, c = x.shape
@@ -266,14 +275,14 @@ def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-3, ac
     lens = _lens(lens, 'lens', b, x.device)
     if x.numel() == 0:
         return x + sum(t.sum() * 0 for t in (weight, bias) if t is not None)
-    flat = x.reshape(b, -1, c).contiguous()
+    flat = (x if x.dim() == 3 else x.reshape(b, -1, c)).contiguous()
     flat = flat if flat.data_ptr() % 16 == 0 else flat.clone()
     weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         y = _GroupNormAct.apply(flat, weight, bias, lens, groups, eps, OP_ACT_IDS[act])
     else:
         y, _ = _norm_forward(flat, weight, bias, lens, groups, eps, OP_ACT_IDS[act])
-    return y.view(x.shape)
+    return y if x.dim() == 3 else y.view(x.shape)
 
 
 # ------------------------------------------------------------------------------------------------------------------- log probabilities
@@ -312,7 +321,7 @@ class _LogProbs(torch.autograd.Function):
         return logp, entropy, top_logp, top_ids
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dlogp, dentropy, _, __):
         x, bin_score, targets, entropy, stats = ctx.saved_tensors
         want_x, want_bin = ctx.needs_input_grad[0], bin_score is not None and ctx.needs_input_grad[1]
@@ -354,12 +363,15 @@ def match_log_probs(logits, targets, bin_score=None, top: int = 0):
     if rows == 0:
         z = logits.sum(-1).float() * 0 + (0 if bin_score is None else bin_score.sum() * 0)
         return z, z * 1, logits.new_empty(*lead, top, dtype=torch.float32), logits.new_empty(*lead, top, dtype=torch.int64)
-    x = logits.reshape(rows, cols)
+    flat = logits.dim() == 2
+    x = logits if flat else logits.reshape(rows, cols)
     if (cols > 1 and x.stride(1) != 1) or (rows > 1 and x.stride(0) < cols):
         x = x.contiguous()
-    t = targets.reshape(rows).contiguous()
+    t = (targets if flat else targets.reshape(rows)).contiguous()
     if torch.is_grad_enabled() and (logits.requires_grad or (bin_score is not None and bin_score.requires_grad)):
         logp, entropy, top_logp, top_ids = _LogProbs.apply(x, bin_score, t, top)
     else:
         logp, entropy, _, top_logp, top_ids = _logp_forward(x, t, bin_score, top)
+    if flat:
+        return logp, entropy, top_logp, top_ids
     return logp.view(lead), entropy.view(lead), top_logp.view(*lead, top), top_ids.view(*lead, top)

@@ -505,12 +505,14 @@ typedef struct imp_attn_desc {
     const int32_t* k_lens;
 } imp_attn_desc;
 int imp_attn_workspace(const imp_attn_desc* d, int backward, uint64_t* bytes);
-/* out [batch][nq][heads][head_dim] contiguous, lse [batch][heads][nq] float32 (optional: needed by the backward) */
-int imp_attn_forward(const imp_attn_desc* d, const void* q, const void* k, const void* v, void* out, float* lse, void* workspace, uint64_t workspace_bytes,
-                     int device, void* stream);
-/* gradients from dout (contiguous like out) and the forward's out and lse; dq like out, dk, dv [batch][nk][kv_heads][head_dim] contiguous: dq, or dk and dv, may be NULL */
-int imp_attn_backward(const imp_attn_desc* d, const void* q, const void* k, const void* v, const void* out, const float* lse, const void* dout, void* dq, void* dk,
-                      void* dv, void* workspace, uint64_t workspace_bytes, int device, void* stream);
+/* out [batch][nq][heads][head_dim] contiguous, lse [batch][heads][nq] float32 (optional: needed by the backward); out_rest like out (optional, 16-bit types: what rounding left
+ * of the output, which makes the backward's rowsum(dout out) exact) */
+int imp_attn_forward(const imp_attn_desc* d, const void* q, const void* k, const void* v, void* out, void* out_rest, float* lse, void* workspace,
+                     uint64_t workspace_bytes, int device, void* stream);
+/* gradients from dout (contiguous like out) and the forward's out, out_rest (or NULL) and lse; dq like out, dk, dv [batch][nk][kv_heads][head_dim] contiguous: dq, or dk and
+ * dv, may be NULL */
+int imp_attn_backward(const imp_attn_desc* d, const void* q, const void* k, const void* v, const void* out, const void* out_rest, const float* lse, const void* dout,
+                      void* dq, void* dk, void* dv, void* workspace, uint64_t workspace_bytes, int device, void* stream);
 
 /* Group norm + activation on token-major data (csrc/norm_act.hip; groups == channels: the InstanceNorm + activation of nets/layers.py:59-77): x, y [batch][n][channels] of
  * `dtype`, weight / bias float32 [channels] (optional), lens int32 [batch] (optional; clamped to 0 .. n; tokens past it are not read, y and dx are 0 there), act IMP_ACT_*,

@@ -37,16 +37,16 @@ def test_attention_calls_refused():
     L, d, buf = _lib.lib(), desc(), C.create_string_buffer(4096)
     at = (C.addressof(buf) + 15) // 16 * 16
     p, odd = C.c_void_p(at), C.c_void_p(at + 4)
-    assert L.imp_attn_forward(C.byref(d), None, p, p, p, None, None, 0, 0, None) == BAD
-    assert L.imp_attn_forward(C.byref(d), p, p, p, None, None, None, 0, 0, None) == BAD
-    assert L.imp_attn_forward(C.byref(d), p, odd, p, p, None, None, 0, 0, None) == BAD
-    assert L.imp_attn_backward(C.byref(d), p, p, p, p, None, p, p, p, p, p, 1 << 40, 0, None) == BAD          # no lse
-    assert L.imp_attn_backward(C.byref(d), p, p, p, p, p, p, None, None, None, p, 1 << 40, 0, None) == BAD    # no gradient wanted
-    assert L.imp_attn_backward(C.byref(d), p, p, p, p, p, p, p, p, None, p, 1 << 40, 0, None) == BAD          # dk without dv
-    assert L.imp_attn_backward(C.byref(d), p, p, p, p, p, p, p, p, p, p, 8, 0, None) == NOMEM
-    assert L.imp_attn_backward(C.byref(d), p, p, p, p, p, p, p, p, p, None, 1 << 40, 0, None) == NOMEM
+    assert L.imp_attn_forward(C.byref(d), None, p, p, p, None, None, None, 0, 0, None) == BAD
+    assert L.imp_attn_forward(C.byref(d), p, p, p, None, None, None, None, 0, 0, None) == BAD
+    assert L.imp_attn_forward(C.byref(d), p, odd, p, p, None, None, None, 0, 0, None) == BAD
+    assert L.imp_attn_backward(C.byref(d), p, p, p, p, None, None, p, p, p, p, p, 1 << 40, 0, None) == BAD          # no lse
+    assert L.imp_attn_backward(C.byref(d), p, p, p, p, None, p, p, None, None, None, p, 1 << 40, 0, None) == BAD    # no gradient wanted
+    assert L.imp_attn_backward(C.byref(d), p, p, p, p, None, p, p, p, p, None, p, 1 << 40, 0, None) == BAD          # dk without dv
+    assert L.imp_attn_backward(C.byref(d), p, p, p, p, None, p, p, p, p, p, p, 8, 0, None) == NOMEM
+    assert L.imp_attn_backward(C.byref(d), p, p, p, p, None, p, p, p, p, p, None, 1 << 40, 0, None) == NOMEM
     long = desc(nq=1, nk=4096)
-    assert L.imp_attn_forward(C.byref(long), p, p, p, p, None, None, 0, 0, None) == NOMEM
+    assert L.imp_attn_forward(C.byref(long), p, p, p, p, None, None, None, 0, 0, None) == NOMEM
 
 
 def test_attention_scratch_grows_with_the_problem():
