@@ -1200,14 +1200,9 @@ void launch_any(int dtype, bool split, int which, const AttnOp& p, hipStream_t s
     else launch_dh<ArithPlanes>(which, p, st);
 }
 
-int on_device(int device) {
-    hipError_t e = hipSetDevice(device);
-    return e == hipSuccess ? 0 : imp_fail(IMP_E_HIP, hipGetErrorString(e));
-}
-int launched(const char* what) {
+int launched() {
     hipError_t e = hipGetLastError();
     if (e == hipSuccess) return IMP_OK;
-    (void)what;
     return imp_fail(IMP_E_HIP, hipGetErrorString(e));
 }
 
@@ -1230,7 +1225,8 @@ int imp_attn_forward(const imp_attn_desc* d, const void* q, const void* k, const
     const Plan pl = plan(*d);
     if (unaligned({q, k, v, out, out_rest, workspace})) return imp_fail(IMP_E_ARG, "imp_attn_forward: pointers must be aligned to 16 bytes");
     if (workspace_bytes < pl.fwd_bytes || (pl.fwd_bytes && !workspace)) return imp_fail(IMP_E_NOMEM, "imp_attn_forward: workspace too small (imp_attn_workspace)");
-    if (int rc = on_device(device)) return rc;
+    const DeviceScope on(device);
+    if (on.error != hipSuccess) return imp_fail(IMP_E_HIP, hipGetErrorString(on.error));
     AttnOp p = op_of(*d);
     p.q = q; p.k = k; p.v = v; p.o = out; p.orest = out_rest; p.lse = lse;
     p.shares = pl.fwd;
@@ -1247,7 +1243,7 @@ int imp_attn_forward(const imp_attn_desc* d, const void* q, const void* k, const
         else if (d->dtype == IMP_DTYPE_BF16) attn_join_kernel<__bf16><<<grid, 256, 0, st>>>(p);
         else attn_join_kernel<_Float16><<<grid, 256, 0, st>>>(p);
     }
-    return launched("imp_attn_forward");
+    return launched();
 }
 
 int imp_attn_backward(const imp_attn_desc* d, const void* q, const void* k, const void* v, const void* out, const void* out_rest, const float* lse,
@@ -1257,7 +1253,8 @@ int imp_attn_backward(const imp_attn_desc* d, const void* q, const void* k, cons
     const Plan pl = plan(*d);
     if (unaligned({q, k, v, out, out_rest, dout, dq, dk, dv, workspace})) return imp_fail(IMP_E_ARG, "imp_attn_backward: pointers must be aligned to 16 bytes");
     if (workspace_bytes < pl.bwd_bytes || !workspace) return imp_fail(IMP_E_NOMEM, "imp_attn_backward: workspace too small (imp_attn_workspace)");
-    if (int rc = on_device(device)) return rc;
+    const DeviceScope on(device);
+    if (on.error != hipSuccess) return imp_fail(IMP_E_HIP, hipGetErrorString(on.error));
     AttnOp p = op_of(*d);
     p.q = q; p.k = k; p.v = v; p.out = out; p.rest = out_rest; p.lse = const_cast<float*>(lse); p.dout = dout; p.dq = dq; p.dk = dk; p.dv = dv;
     p.amax = (float*)workspace;
@@ -1293,7 +1290,7 @@ int imp_attn_backward(const imp_attn_desc* d, const void* q, const void* k, cons
         launch_any(dt, pl.split, 1, p, st);
         if (p.shares > 1) join(pl.q_rows, 1, dq, nullptr);
     }
-    return launched("imp_attn_backward");
+    return launched();
 }
 
 }  // extern "C"

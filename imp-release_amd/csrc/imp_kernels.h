@@ -31,6 +31,20 @@ __host__ __device__ __forceinline__ int attn_side_splits(int nq, int nk) {
 __device__ __forceinline__ int imp_count(const RaggedCounts& rc, int img, int b, int uniform) { return rc.on ? rc.n[img][b] : uniform; }
 #endif
 
+// a call on `device`: makes it current, and leaves the caller's device current again
+struct DeviceScope {
+    int before = -1;
+    hipError_t error;
+    explicit DeviceScope(int device) {
+        error = hipGetDevice(&before);
+        if (error != hipSuccess || before == device) before = -1;
+        else error = hipSetDevice(device);
+    }
+    ~DeviceScope() { if (before >= 0) (void)hipSetDevice(before); }
+    DeviceScope(const DeviceScope&) = delete;
+    DeviceScope& operator=(const DeviceScope&) = delete;
+};
+
 // opt-in to more than 48 KB of dynamic LDS for `kernel`: the attribute is per device, so the largest size already granted is
 // tracked per (device, kernel) under a mutex (worker threads launch concurrently; a process may drive several GPUs)
 hipError_t imp_grant_dynamic_lds(const void* kernel, size_t bytes);

@@ -440,10 +440,6 @@ const char* bad(int dtype, int64_t rows, int cols, int64_t ld, const void* x, bo
     if ((uintptr_t)x & (dtype == IMP_DTYPE_F32 ? 3 : 1)) return "logits are not aligned to their type";
     return nullptr;
 }
-int ready(int device) {
-    hipError_t e = hipSetDevice(device);
-    return e == hipSuccess ? 0 : imp_fail(IMP_E_HIP, hipGetErrorString(e));
-}
 
 // pieces of 2 vectors per lane, or of 32 elements: short rows do not pay for places that they leave empty
 template <typename T, bool TOP> void forward(const LogpOp& p, hipStream_t st) {
@@ -489,7 +485,8 @@ int imp_log_probs_forward(int dtype, int64_t rows, int cols, int64_t ld, const v
     uint64_t need = 0;
     imp_log_probs_workspace(rows, cols, top, 0, &need);
     if (workspace_bytes < need || (need && (!workspace || ((uintptr_t)workspace & 3)))) return imp_fail(IMP_E_NOMEM, "imp_log_probs_forward: workspace too small");
-    if (int rc = ready(device)) return rc;
+    const DeviceScope on(device);
+    if (on.error != hipSuccess) return imp_fail(IMP_E_HIP, hipGetErrorString(on.error));
     LogpOp p = {};
     p.x = logits; p.target = targets; p.bin = bin_score; p.logp = logp; p.entropy = entropy; p.stats = stats; p.top_logp = top_logp; p.top_id = top_ids;
     p.rows = rows; p.ld = ld; p.cols = cols; p.top = top; p.shares = shares_of(rows, cols);
@@ -512,7 +509,8 @@ int imp_log_probs_backward(int dtype, int64_t rows, int cols, int64_t ld, const 
     if ((uintptr_t)dlogits & (dtype == IMP_DTYPE_F32 ? 3 : 1)) return imp_fail(IMP_E_ARG, "dlogits are not aligned to their type");
     if (dbin && (workspace_bytes < (uint64_t)rows * 8 || !workspace || ((uintptr_t)workspace & 7)))
         return imp_fail(IMP_E_NOMEM, "imp_log_probs_backward: workspace too small");
-    if (int rc = ready(device)) return rc;
+    const DeviceScope on(device);
+    if (on.error != hipSuccess) return imp_fail(IMP_E_HIP, hipGetErrorString(on.error));
     LogpOp p = {};
     p.x = logits; p.target = targets; p.bin = bin_score; p.entropy = const_cast<float*>(entropy); p.stats = const_cast<float*>(stats);
     p.dlogp = dlogp; p.dentropy = dentropy; p.dx = dlogits; p.rows = rows; p.ld = ld; p.cols = cols; p.shares = shares_of(rows, cols);

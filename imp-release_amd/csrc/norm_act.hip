@@ -560,10 +560,6 @@ template <typename F> void by_type(int dtype, int vec, F f) {
     else if (dtype == IMP_DTYPE_F16) { if (vec > 1) f((_Float16*)nullptr, std::integral_constant<int, 8>()); else f((_Float16*)nullptr, std::integral_constant<int, 1>()); }
     else { if (vec > 1) f((__bf16*)nullptr, std::integral_constant<int, 8>()); else f((__bf16*)nullptr, std::integral_constant<int, 1>()); }
 }
-int ready(int device) {
-    hipError_t e = hipSetDevice(device);
-    return e == hipSuccess ? 0 : imp_fail(IMP_E_HIP, hipGetErrorString(e));
-}
 int done() {
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? IMP_OK : imp_fail(IMP_E_HIP, hipGetErrorString(e));
@@ -586,7 +582,8 @@ int imp_group_norm_act_forward(int dtype, int batch, int n, int channels, int gr
     if (!y || !stats || !(eps > 0.f)) return imp_fail(IMP_E_ARG, "imp_group_norm_act_forward: null argument, or eps not positive");
     const Shape s = shape_of(dtype, batch, n, channels);
     if (!workspace || workspace_bytes < fwd_bytes(s, batch, channels)) return imp_fail(IMP_E_NOMEM, "imp_group_norm_act_forward: workspace too small");
-    if (int rc = ready(device)) return rc;
+    const DeviceScope on(device);
+    if (on.error != hipSuccess) return imp_fail(IMP_E_HIP, hipGetErrorString(on.error));
     NormOp p = {};
     p.x = x; p.y = y; p.w = weight; p.b = bias; p.lens = lens; p.stats = (float4*)stats; p.part = (double2*)workspace;
     p.B = batch; p.N = n; p.C = channels; p.G = groups; p.cg = channels / groups; p.act = act; p.eps = eps;
@@ -621,7 +618,8 @@ int imp_group_norm_act_backward(int dtype, int batch, int n, int channels, int g
     if (!stats || !dy || !dx) return imp_fail(IMP_E_ARG, "imp_group_norm_act_backward: null argument");
     const Shape s = shape_of(dtype, batch, n, channels);
     if (!workspace || workspace_bytes < bwd_bytes(s, batch, channels, groups)) return imp_fail(IMP_E_NOMEM, "imp_group_norm_act_backward: workspace too small");
-    if (int rc = ready(device)) return rc;
+    const DeviceScope on(device);
+    if (on.error != hipSuccess) return imp_fail(IMP_E_HIP, hipGetErrorString(on.error));
     NormOp p = {};
     p.x = x; p.dy = dy; p.dx = dx; p.w = weight; p.b = bias; p.lens = lens; p.stats = (float4*)const_cast<float*>(stats); p.dw = dweight; p.db = dbias;
     p.part = (double2*)workspace;

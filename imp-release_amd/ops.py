@@ -54,10 +54,15 @@ def _scratch(nbytes, device):
     return torch.empty((int(nbytes) + 15) // 16 * 2, device=device, dtype=torch.int64) if nbytes else None
 
 
+def _stream(index):
+    """the current stream of a device"""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def _where(t):
     """(device index, its current stream)"""
     i = t.device.index
-    return i, torch._C._cuda_getCurrentRawStream(i)
+    return i, _stream(i)
 
 
 def _at(t):
@@ -102,37 +107,47 @@ def _rows(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-@functools.lru_cache(maxsize=1024)
-def _attn_plan(dtype, q_shape, k_shape, q_stride, k_stride, v_stride, scale):
-    """(the description of a problem of these sizes, without masks; scratch bytes of the forward; of the backward)"""
-    d = ImpAttnDesc()
-    d.dtype, d.batch, d.nq, d.nk, d.heads, d.kv_heads, d.head_dim, d.scale = dtype, q_shape[0], q_shape[1], k_shape[1], q_shape[2], k_shape[2], q_shape[3], scale
-    for field, shape, stride in ((d.q_stride, q_shape, q_stride), (d.k_stride, k_shape, k_stride), (d.v_stride, k_shape, v_stride)):
-        for i in range(3):
-            field[i] = 0 if shape[i] == 1 else stride[i]
-    need = []
-    for backward in (0, 1):
-        n = C.c_uint64()
-        _check(_lib.lib().imp_attn_workspace(C.byref(d), backward, C.byref(n)))
-        need.append(n.value)
-    return d, need[0], need[1]
+class _AttnPlan:
+    """what a problem of these sizes and strides needs: its description (without masks), scratch bytes, and the device"""
+    __slots__ = ('desc', 'forward', 'backward', 'device', 'index', 'out', 'lse', 'dk')
+
+    def __init__(self, dtype, device, q_shape, k_shape, q_stride, k_stride, v_stride, scale):
+        d = ImpAttnDesc()
+        d.dtype, d.batch, d.nq, d.nk, d.heads, d.kv_heads = DTYPE_IDS[dtype], q_shape[0], q_shape[1], k_shape[1], q_shape[2], k_shape[2]
+        d.head_dim, d.scale = q_shape[3], scale
+        for field, shape, stride in ((d.q_stride, q_shape, q_stride), (d.k_stride, k_shape, k_stride), (d.v_stride, k_shape, v_stride)):
+            for i in range(3):
+                field[i] = 0 if shape[i] == 1 else stride[i]
+        need = []
+        for backward in (0, 1):
+            n = C.c_uint64()
+            _check(_lib.lib().imp_attn_workspace(C.byref(d), backward, C.byref(n)))
+            need.append(n.value)
+        self.desc, self.forward, self.backward, self.device, self.index = d, need[0], need[1], device, device.index
+        self.out, self.lse, self.dk = tuple(q_shape), (q_shape[0], q_shape[2], q_shape[1]), tuple(k_shape)
+
+    def with_masks(self, mask, q_lens, k_lens):
+        if mask is None and q_lens is None and k_lens is None:
+            return self.desc
+        d = ImpAttnDesc.from_buffer_copy(self.desc)
+        d.key_mask, d.q_lens, d.k_lens = _at(mask), _at(q_lens), _at(k_lens)
+        return d
 
 
-def _attn_desc(q, k, v, mask, q_lens, k_lens, scale):
-    d, fwd, bwd = _attn_plan(DTYPE_IDS[q.dtype], q.shape, k.shape, q.stride(), k.stride(), v.stride(), scale)
-    if mask is not None or q_lens is not None or k_lens is not None:
-        d = ImpAttnDesc.from_buffer_copy(d)
-        d.key_mask, d.q_lens, d.k_lens = (None if t is None else t.data_ptr() for t in (mask, q_lens, k_lens))
-    return d, fwd, bwd
+_attn_plan = functools.lru_cache(maxsize=1024)(_AttnPlan)
 
 
-def _attn_forward(q, k, v, mask, q_lens, k_lens, scale, want_lse, want_rest=False):
-    d, need, _ = _attn_desc(q, k, v, mask, q_lens, k_lens, scale)
-    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+def _plan_of(q, k, v, scale):
+    return _attn_plan(q.dtype, q.device, q.shape, k.shape, q.stride(), k.stride(), v.stride(), scale)
+
+
+def _attn_forward(plan, q, k, v, mask, q_lens, k_lens, want_lse, want_rest=False):
+    out = torch.empty(plan.out, device=plan.device, dtype=q.dtype)
     rest = torch.empty_like(out) if want_rest else None
-    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), device=q.device, dtype=torch.float32) if want_lse else None
-    ws = _scratch(need, q.device)
-    _check(_lib.lib().imp_attn_forward(d, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _at(rest), _at(lse), _at(ws), need, *_where(q)))
+    lse = torch.empty(plan.lse, device=plan.device, dtype=torch.float32) if want_lse else None
+    ws = _scratch(plan.forward, plan.device)
+    _check(_lib.lib().imp_attn_forward(plan.with_masks(mask, q_lens, k_lens), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _at(rest), _at(lse), _at(ws),
+                                       plan.forward, plan.index, _stream(plan.index)))
     return out, rest, lse
 
 
@@ -140,9 +155,9 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, q_lens, k_lens, scale):
         q, k, v = _rows(q), _rows(k), _rows(v)
-        out, rest, lse = _attn_forward(q, k, v, mask, q_lens, k_lens, scale, True, q.dtype != torch.float32)
+        ctx.plan = plan = _plan_of(q, k, v, scale)
+        out, rest, lse = _attn_forward(plan, q, k, v, mask, q_lens, k_lens, True, q.dtype != torch.float32)
         ctx.save_for_backward(q, k, v, out, rest, lse, mask, q_lens, k_lens)
-        ctx.scale = scale
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
         return out, lse
@@ -153,17 +168,17 @@ class _Attention(torch.autograd.Function):
         if dout is None:
             return None, None, None, None, None, None, None
         q, k, v, out, rest, lse, mask, q_lens, k_lens = ctx.saved_tensors
+        plan = ctx.plan
         dout = _dense(dout, out.dtype)
-        d, _, need = _attn_desc(q, k, v, mask, q_lens, k_lens, ctx.scale)
         want_q, want_k, want_v = ctx.needs_input_grad[:3]
-        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype) if want_q else None
+        dq = torch.empty_like(out) if want_q else None
         dk = dv = None
         if want_k or want_v:
-            dk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+            dk = torch.empty(plan.dk, device=plan.device, dtype=k.dtype)
             dv = torch.empty_like(dk)
-        ws = _scratch(need, q.device)
-        _check(_lib.lib().imp_attn_backward(d, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _at(rest), lse.data_ptr(), dout.data_ptr(), _at(dq), _at(dk),
-                                            _at(dv), ws.data_ptr(), need, *_where(q)))
+        ws = _scratch(plan.backward, plan.device)
+        _check(_lib.lib().imp_attn_backward(plan.with_masks(mask, q_lens, k_lens), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _at(rest), lse.data_ptr(),
+                                            dout.data_ptr(), _at(dq), _at(dk), _at(dv), ws.data_ptr(), plan.backward, plan.index, _stream(plan.index)))
         return dq, dk if want_k else None, dv if want_v else None, None, None, None, None
 
 
@@ -201,7 +216,8 @@ def attention(q, k, v, key_mask: Optional[torch.Tensor] = None, q_lens=None, k_l
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _Attention.apply(q, k, v, key_mask, q_lens, k_lens, scale)
     else:
-        out, _, lse = _attn_forward(_rows(q), _rows(k), _rows(v), key_mask, q_lens, k_lens, scale, return_lse)
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        out, _, lse = _attn_forward(_plan_of(q, k, v, scale), q, k, v, key_mask, q_lens, k_lens, return_lse)
     return (out, lse) if return_lse else out
 
 
