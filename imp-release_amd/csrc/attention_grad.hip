@@ -17,7 +17,7 @@
 // Few rows: the walk is cut in shares (partials in the caller's workspace, joined in a fixed order by a second launch).
 //
 // Arithmetic (accumulators, softmax statistics and D in fp32; what the operands of the products are rounded to):
-//   bf16  one bf16 MFMA per product; P and dS rounded to bf16, half a step of 2^-8: the inputs' own precision.  D is formed from the unrounded O (the forward also writes
+//   bf16  one bf16 MFMA per product; P and dS rounded to bf16, half a step of 2^-8: the inputs' own precision (two planes each, 16 bits, in small problems: FINE_SCORES).  D is formed from the unrounded O (the forward also writes
 //         what rounding left of it): taken from the rounded one it put as much error into dQ and dK of few keys as all other roundings together
 //   fp16  one f16 MFMA; P carries a factor 2^10 (weights of long rows stay normal numbers) and dS a power of two per owned row, raised or lowered as the walk meets larger
 //         values (LaneScale), so that gradients far below the fp16 range keep their bits
@@ -40,6 +40,10 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int OWN = 128;                 // owned rows per workgroup
+// 16-bit types: scores (heads x queries x keys) up to which P and dS are carried in two planes, so that nothing but the output is rounded to the type.  There the launches bound
+// the call and the second plane is free (2^24 scores, 64 channels, bf16: backward 57 us with it, 57-60 without); beyond, the matrix work bounds and it costs a fifth to a third
+// (2^26: 124 against 100 us; 2^27, 128 channels: 396 against 284), for an error of 1.0 instead of 1.4 times that of rounding the result
+constexpr double FINE_SCORES = 1 << 24;
 constexpr int SPLIT_ROWS = 256;          // fp32: rows and keys from which the split halves' extra launch pays
 
 struct AttnOp {
@@ -64,32 +68,32 @@ template <> struct Vec8<_Float16> { using type = f16x8; };
 __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
-// operand type, planes, tensors scaled per head, dS scaled per owned row, log2 of the factor P carries, rows per tile of the walk
-template <typename T_, typename E_, int NP_, bool SCALED_, bool LANE_, int SHIFT_, int R_> struct Arith {
+// operand type, planes of the tensors, planes of P and dS, tensors scaled per head, dS scaled per owned row, log2 of the factor P carries, rows per tile of the walk
+template <typename T_, typename E_, int NP_, int WP_, bool SCALED_, bool LANE_, int SHIFT_, int R_> struct Arith {
     using T = T_;
     using E = E_;
     using V = typename Vec8<E_>::type;
-    static constexpr int NP = NP_, SHIFT = SHIFT_, R = R_;
+    static constexpr int NP = NP_, WP = WP_, SHIFT = SHIFT_, R = R_;
     static constexpr bool SCALED = SCALED_, LANE = LANE_;
 };
-using ArithBf16 = Arith<__bf16, __bf16, 1, false, false, 0, 64>;
-using ArithF16 = Arith<_Float16, _Float16, 1, false, true, 10, 64>;
-using ArithSplit = Arith<float, _Float16, 2, true, true, 10, 32>;
+using ArithBf16 = Arith<__bf16, __bf16, 1, 1, false, false, 0, 64>;
+using ArithF16 = Arith<_Float16, _Float16, 1, 1, false, true, 10, 64>;
+using ArithBf16Fine = Arith<__bf16, __bf16, 1, 2, false, false, 0, 64>;
+using ArithF16Fine = Arith<_Float16, _Float16, 1, 2, false, true, 10, 64>;
+using ArithSplit = Arith<float, _Float16, 2, 2, true, true, 10, 32>;
+using ArithPlanes = Arith<float, __bf16, 3, 3, false, false, 0, 32>;
 constexpr float LAZY = 5.f;              // the softmax reference of a row follows its maximum when that is 2^LAZY above it: P stays below 2^(SHIFT + LAZY)
-using ArithPlanes = Arith<float, __bf16, 3, false, false, 0, 32>;
 
 // c += a b over the planes, the small products first
-template <int NP, typename V>
-__device__ __forceinline__ f32x16 mfma_planes(const V (&a)[NP], const V (&b)[NP], f32x16 c) {
+template <int NP, int WP, typename V>
+__device__ __forceinline__ f32x16 mfma_planes(const V (&a)[NP], const V (&b)[WP], f32x16 c) {
     if constexpr (NP == 3) {
         c = mfma(a[1], b[1], c);
         c = mfma(a[0], b[2], c);
         c = mfma(a[2], b[0], c);
     }
-    if constexpr (NP >= 2) {
-        c = mfma(a[0], b[1], c);
-        c = mfma(a[1], b[0], c);
-    }
+    if constexpr (WP >= 2) c = mfma(a[0], b[1], c);
+    if constexpr (NP >= 2) c = mfma(a[1], b[0], c);
     return mfma(a[0], b[0], c);
 }
 
@@ -439,7 +443,7 @@ __global__ __launch_bounds__(256, A::NP == 3 && DHP == 128 ? 1 : 2) void attn_fw
     using T = typename A::T;
     using E = typename A::E;
     using V = typename A::V;
-    constexpr int NP = A::NP, R = A::R;
+    constexpr int NP = A::NP, WP = A::WP, R = A::R;
     using St = Stage<T, E, NP, DHP, R>;
     constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32, GN = group_of<NP, KS>(), SG = KS / GN, PG = 2 * DT / GN;
     constexpr bool PIPE = true;
@@ -530,16 +534,16 @@ __global__ __launch_bounds__(256, A::NP == 3 && DHP == 128 ? 1 : 2) void attn_fw
                 s[n][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], c, ref));
                 l += s[n][i];
             }
-            V pf[2][NP];
+            V pf[2][WP];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) pack<NP, E>(s[n], k, pf[k]);
+            for (int k = 0; k < 2; ++k) pack<WP, E>(s[n], k, pf[k]);
 #pragma unroll
             for (int i = 0; i < PG; ++i) {
                 const int at = NT * SG + n * PG + i;
                 read(at + 1);
                 if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < GN; ++j) o[(i * GN + j) % DT] = mfma_planes<NP, V>(buf[at & 1].f[j], pf[(i * GN + j) / DT], o[(i * GN + j) % DT]);
+                for (int j = 0; j < GN; ++j) o[(i * GN + j) % DT] = mfma_planes<NP, WP, V>(buf[at & 1].f[j], pf[(i * GN + j) / DT], o[(i * GN + j) % DT]);
                 if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -656,7 +660,7 @@ __global__ __launch_bounds__(256, A::NP > 1 && DHP == 128 ? 1 : 2) void attn_dq_
     using T = typename A::T;
     using E = typename A::E;
     using V = typename A::V;
-    constexpr int NP = A::NP, R = A::R;
+    constexpr int NP = A::NP, WP = A::WP, R = A::R;
     using St = Stage<T, E, NP, DHP, R>;
     constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32, GN = group_of<NP, KS>(), SG = KS / GN, PG = 2 * DT / GN;
     constexpr bool PIPE = !(DHP == 128 && NP == 1);      // no registers are left for it there
@@ -744,15 +748,15 @@ __global__ __launch_bounds__(256, A::NP > 1 && DHP == 128 ? 1 : 2) void attn_dq_
                 ls.step(s, dq);
                 s *= ls.f;
             }
-            V df[2][NP];
+            V df[2][WP];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) pack<NP, E>(s, k, df[k]);
+            for (int k = 0; k < 2; ++k) pack<WP, E>(s, k, df[k]);
 #pragma unroll
             for (int i = 2 * SG; i < ALL; ++i) {
                 read(n, PIPE ? i + 1 : i);
                 if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < GN; ++j) { const int e = (i - 2 * SG) * GN + j; dq[e % DT] = mfma_planes<NP, V>(buf[(n * ALL + i) & 1].f[j], df[e / DT], dq[e % DT]); }
+                for (int j = 0; j < GN; ++j) { const int e = (i - 2 * SG) * GN + j; dq[e % DT] = mfma_planes<NP, WP, V>(buf[(n * ALL + i) & 1].f[j], df[e / DT], dq[e % DT]); }
                 if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -806,7 +810,7 @@ __global__ __launch_bounds__(256, DHP == 128 || (A::NP == 3 && DHP == 64) ? 1 : 
     using T = typename A::T;
     using E = typename A::E;
     using V = typename A::V;
-    constexpr int NP = A::NP, R = A::R;
+    constexpr int NP = A::NP, WP = A::WP, R = A::R;
     using St = Stage<T, E, NP, DHP, R>;
     constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = DHP / 32, NT = R / 32, GN = group_of<NP, KS>(), SG = KS / GN, PG = 2 * DT / GN;
     constexpr bool PIPE = !(DHP == 64 && NP == 2);
@@ -912,11 +916,11 @@ __global__ __launch_bounds__(256, DHP == 128 || (A::NP == 3 && DHP == 64) ? 1 : 
                 ls.step(dp, dk);
                 dp *= ls.f;
             }
-            V pf[2][NP], df[2][NP];
+            V pf[2][WP], df[2][WP];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                pack<NP, E>(s, k, pf[k]);
-                pack<NP, E>(dp, k, df[k]);
+                pack<WP, E>(s, k, pf[k]);
+                pack<WP, E>(dp, k, df[k]);
             }
 #pragma unroll
             for (int i = 2 * SG; i < ALL; ++i) {
@@ -925,8 +929,8 @@ __global__ __launch_bounds__(256, DHP == 128 || (A::NP == 3 && DHP == 64) ? 1 : 
 #pragma unroll
                 for (int j = 0; j < GN; ++j) {
                     const int e = (i - 2 * SG) * GN + j, k = e / (2 * DT), d = e / 2 % DT;
-                    if (e & 1) dk[d] = mfma_planes<NP, V>(buf[(n * ALL + i) & 1].f[j], df[k], dk[d]);
-                    else dv[d] = mfma_planes<NP, V>(buf[(n * ALL + i) & 1].f[j], pf[k], dv[d]);
+                    if (e & 1) dk[d] = mfma_planes<NP, WP, V>(buf[(n * ALL + i) & 1].f[j], df[k], dk[d]);
+                    else dv[d] = mfma_planes<NP, WP, V>(buf[(n * ALL + i) & 1].f[j], pf[k], dv[d]);
                 }
                 if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
             }
@@ -951,14 +955,14 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
     using E = typename A::E;
     using V = typename A::V;
     static_assert(A::NP == 1 && A::R == 64);
-    constexpr int NP = 1, R = 64, DHP = 128;
+    constexpr int NP = 1, WP = A::WP, R = 64, DHP = 128;
     using St = Stage<T, E, NP, DHP, R>;
     constexpr int PLANE = St::PLANE, KS = DHP / 16, DT = 2, GN = group_of<NP, KS>(), SG = KS / GN;
     constexpr bool PIPE = false;
     __shared__ __attribute__((aligned(16))) E Qs[PLANE], Os[PLANE];
     __shared__ __attribute__((aligned(16))) float refs[R], deltas[R];
     __shared__ unsigned alive[R];
-    __shared__ __attribute__((aligned(16))) V hand[4][4][64];
+    __shared__ __attribute__((aligned(16))) V hand[4][4 * WP][64];
     __shared__ float largest[4][32];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = tid >> 6, h = wave & 1;
     const int b = blockIdx.y / p.Hkv, hk = blockIdx.y % p.Hkv, share = blockIdx.z;
@@ -1023,14 +1027,14 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
                 for (int j = 0; j < GN; ++j) read_cols<E, NP, DHP, PLANE>(j & 1 ? Qs : Os, n, k, 2 * h + j / 2, lanes, g.f[j]);
             }
         };
-        auto sums = [&](int i, V pk, V dsk) __attribute__((always_inline)) {
+        auto sums = [&](int i, const V (&pk)[WP], const V (&dsk)[WP]) __attribute__((always_inline)) {
             static_assert(GN == 2 * DT);
             read(PIPE ? i + 1 : i);
             if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                dv[d] = mfma(buf[i & 1].f[2 * d][0], pk, dv[d]);
-                dk[d] = mfma(buf[i & 1].f[2 * d + 1][0], dsk, dk[d]);
+                dv[d] = mfma_planes<NP, WP, V>(buf[i & 1].f[2 * d], pk, dv[d]);
+                dk[d] = mfma_planes<NP, WP, V>(buf[i & 1].f[2 * d + 1], dsk, dk[d]);
             }
             if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
         };
@@ -1065,24 +1069,27 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
             ls.step_max(fmaxf(m, largest[wave ^ 1][lane & 31]), dk);
             dp *= ls.f;
         }
-        V pf[2], df[2];
+        V pf[2][WP], df[2][WP];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            V one[1];
-            pack<NP, E>(s, k, one);
-            pf[k] = one[0];
-            pack<NP, E>(dp, k, one);
-            df[k] = one[0];
-            hand[wave][2 * k][lane] = pf[k];
-            hand[wave][2 * k + 1][lane] = df[k];
+            pack<WP, E>(s, k, pf[k]);
+            pack<WP, E>(dp, k, df[k]);
+#pragma unroll
+            for (int w = 0; w < WP; ++w) {
+                hand[wave][(2 * k) * WP + w][lane] = pf[k][w];
+                hand[wave][(2 * k + 1) * WP + w][lane] = df[k][w];
+            }
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) sums(2 * SG + k, pf[k], df[k]);
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            pf[k] = hand[wave ^ 1][2 * k][lane];
-            df[k] = hand[wave ^ 1][2 * k + 1][lane];
+#pragma unroll
+            for (int w = 0; w < WP; ++w) {
+                pf[k][w] = hand[wave ^ 1][(2 * k) * WP + w][lane];
+                df[k][w] = hand[wave ^ 1][(2 * k + 1) * WP + w][lane];
+            }
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) sums(2 * SG + 2 + k, pf[k], df[k]);
@@ -1110,14 +1117,14 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(const float* part, int64_
 }
 
 // ------------------------------------------------------------------------------------------------------------------------- host
-// shares of the walk: enough workgroups for two per CU, each with at least four tiles of the walk
+// shares of the walk: enough workgroups for two per CU, each with at least two tiles of the walk
 int shares_for(int64_t blocks, int64_t walked) {
-    const int64_t want = (512 + blocks - 1) / blocks, most = walked / 256;
+    const int64_t want = (512 + blocks - 1) / blocks, most = walked / 128;
     const int64_t s = want < most ? want : most;
     return s < 1 ? 1 : (s > 64 ? 64 : (int)s);
 }
 
-struct Plan { int fwd, dq, dkv, chunks; bool split; int64_t q_rows, k_rows; size_t amax_bytes, fwd_bytes, bwd_bytes; };
+struct Plan { int fwd, dq, dkv, chunks; bool split, fine; int64_t q_rows, k_rows; size_t amax_bytes, fwd_bytes, bwd_bytes; };
 Plan plan(const imp_attn_desc& d) {
     Plan p;
     const int64_t heads = (int64_t)d.batch * d.kv_heads, rows = (int64_t)d.nq * (d.heads / d.kv_heads);
@@ -1130,6 +1137,7 @@ Plan plan(const imp_attn_desc& d) {
     p.q_rows = (int64_t)d.batch * d.nq * d.heads;
     p.k_rows = (int64_t)d.batch * d.nk * d.kv_heads;
     p.split = d.dtype == IMP_DTYPE_F32 && rows >= SPLIT_ROWS && d.nk >= SPLIT_ROWS;
+    p.fine = (double)heads * rows * d.nk <= FINE_SCORES;
     const int64_t c = 256 / heads;
     p.chunks = (int)(c < 4 ? 4 : c > 64 ? 64 : c);
     p.amax_bytes = p.split ? (size_t)4 * heads * p.chunks * 4 : 0;
@@ -1193,9 +1201,9 @@ template <typename A> void launch_dh(int which, const AttnOp& p, hipStream_t st)
     else if (p.dh <= 64) launch<A, 64>(which, p, st);
     else launch<A, 128>(which, p, st);
 }
-void launch_any(int dtype, bool split, int which, const AttnOp& p, hipStream_t st) {
-    if (dtype == IMP_DTYPE_BF16) launch_dh<ArithBf16>(which, p, st);
-    else if (dtype == IMP_DTYPE_F16) launch_dh<ArithF16>(which, p, st);
+void launch_any(int dtype, bool split, bool fine, int which, const AttnOp& p, hipStream_t st) {
+    if (dtype == IMP_DTYPE_BF16) { if (fine) launch_dh<ArithBf16Fine>(which, p, st); else launch_dh<ArithBf16>(which, p, st); }
+    else if (dtype == IMP_DTYPE_F16) { if (fine) launch_dh<ArithF16Fine>(which, p, st); else launch_dh<ArithF16>(which, p, st); }
     else if (split) launch_dh<ArithSplit>(which, p, st);
     else launch_dh<ArithPlanes>(which, p, st);
 }
@@ -1236,7 +1244,7 @@ int imp_attn_forward(const imp_attn_desc* d, const void* q, const void* k, const
     p.part_lse = p.part + (int64_t)pl.fwd * pl.q_rows * d->head_dim;
     const hipStream_t st = (hipStream_t)stream;
     if (pl.split) attn_amax_kernel<<<dim3(pl.chunks, d->batch * d->kv_heads, 3), 256, 0, st>>>(p);
-    launch_any(d->dtype, pl.split, 0, p, st);
+    launch_any(d->dtype, pl.split, pl.fine, 0, p, st);
     if (pl.fwd > 1) {
         const unsigned grid = (unsigned)((pl.q_rows + 3) / 4);
         if (d->dtype == IMP_DTYPE_F32) attn_join_kernel<float><<<grid, 256, 0, st>>>(p);
@@ -1282,12 +1290,12 @@ int imp_attn_backward(const imp_attn_desc* d, const void* q, const void* k, cons
     };
     if (dk) {
         p.shares = pl.dkv;
-        launch_any(dt, pl.split, 2, p, st);
+        launch_any(dt, pl.split, pl.fine, 2, p, st);
         if (p.shares > 1) join(pl.k_rows, 2, dk, dv);
     }
     if (dq) {
         p.shares = pl.dq;
-        launch_any(dt, pl.split, 1, p, st);
+        launch_any(dt, pl.split, pl.fine, 1, p, st);
         if (p.shares > 1) join(pl.q_rows, 1, dq, nullptr);
     }
     return launched();
