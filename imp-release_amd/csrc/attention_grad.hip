@@ -601,9 +601,15 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnOp p) {
     for (int c0 = 0; c0 < p.dh; c0 += 64) {
         float acc = 0.f;
         const int c = c0 + lane;
-        for (int s = 0; s < p.shares; ++s) {
-            const float ws = __shfl(w, s);
-            if (c < p.dh && ws != 0.f) acc += ws * p.part[(s * rows + row) * p.dh + c];
+        for (int s0 = 0; s0 < p.shares; s0 += 16) {                // 16 loads under way: one after the other they took twice the time of the walk itself
+            float x[16];
+#pragma unroll
+            for (int s = 0; s < 16; ++s) x[s] = c < p.dh && s0 + s < p.shares ? p.part[((s0 + s) * rows + row) * p.dh + c] : 0.f;
+#pragma unroll
+            for (int s = 0; s < 16; ++s) {
+                const float ws = __shfl(w, s0 + s);                // (0 past the last share)
+                if (ws != 0.f) acc += ws * x[s];
+            }
         }
         if (c < p.dh) {
             ((T*)p.o)[row * p.dh + c] = (T)(acc * inv);
@@ -1112,6 +1118,7 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(const float* part, int64_
     T* out = blockIdx.y ? out1 : out0;
     part += blockIdx.y * n;
     f32x4 a = *(const f32x4*)(part + i);
+#pragma unroll 8
     for (int s = 1; s < shares; ++s) a += *(const f32x4*)(part + s * stride + i);
     store4(out + i, a[0], a[1], a[2], a[3]);
 }
