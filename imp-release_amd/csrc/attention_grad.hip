@@ -627,7 +627,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnOp p) {
 // D = rowsum(dO O): 16 lanes per row of [B][nq][H][dh]
 template <typename T>
 __global__ __launch_bounds__(256) void attn_delta_kernel(AttnOp p) {
-    const int64_t rows = (int64_t)p.B * p.nq * p.H, row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int64_t rows = (int64_t)p.B * p.nq * p.H, row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 16 + (threadIdx.x >> 4);
     if (row >= rows) return;
     const int col = (threadIdx.x & 15) * 8;
     float sum = 0.f;
@@ -1286,7 +1286,8 @@ int imp_attn_backward(const imp_attn_desc* d, const void* q, const void* k, cons
     if (pl.split) attn_amax_kernel<<<dim3(pl.chunks, d->batch * d->kv_heads, 4), 256, 0, st>>>(p);
     each([&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        attn_delta_kernel<T><<<(unsigned)((pl.q_rows + 15) / 16), 256, 0, st>>>(p);
+        const int64_t blocks = (pl.q_rows + 15) / 16, x = blocks < (1 << 22) ? blocks : 1 << 22;             // (a grid's x dimension reaches 2^32 threads)
+        attn_delta_kernel<T><<<dim3((unsigned)x, (unsigned)((blocks + x - 1) / x)), 256, 0, st>>>(p);
     });
     auto join = [&](int64_t rows, int parts, void* to0, void* to1) {
         const int64_t n = rows * d->head_dim;

@@ -120,6 +120,9 @@ __device__ __forceinline__ void write_top(const LogpOp& p, int64_t row, int k, c
 }
 
 // W waves per row (W = 1: four rows per workgroup); one row or share of a row per group.  U: vectors per lane in a piece
+// the group of rows of this workgroup: a grid's x dimension reaches 2^32 threads
+__device__ __forceinline__ int64_t rows_block() { return (int64_t)blockIdx.z * gridDim.x + blockIdx.x; }
+
 template <typename T, bool TOP, int W, int U>
 __global__ __launch_bounds__(256) void logp_forward_kernel(LogpOp p) {
     constexpr int V = 16 / sizeof(T), GROUPS = 4 / W;
@@ -127,8 +130,8 @@ __global__ __launch_bounds__(256) void logp_forward_kernel(LogpOp p) {
     __shared__ float sm_v[4][TOP_MAX];
     __shared__ int sm_i[4][TOP_MAX];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = wave % W;
-    const int64_t row = (int64_t)blockIdx.x * GROUPS + wave / W;
-    if (W == 1 && row >= p.rows) return;
+    const int64_t row = rows_block() * GROUPS + wave / W;
+    if (row >= p.rows) return;           // (whole waves; whole workgroups where their waves meet)
     const int share = blockIdx.y;
     const int c0 = (int)((int64_t)p.cols * share / p.shares), c1 = (int)((int64_t)p.cols * (share + 1) / p.shares);
     const T* x = (const T*)p.x + row * p.ld;
@@ -356,7 +359,7 @@ template <typename T, int W>
 __global__ __launch_bounds__(256) void logp_backward_kernel(LogpOp p) {
     constexpr int V = 16 / sizeof(T), THREADS = 64 * W, GROUPS = 4 / W;
     const int tid = threadIdx.x % THREADS, group = threadIdx.x / THREADS;
-    const int64_t row = (int64_t)blockIdx.x * GROUPS + group;
+    const int64_t row = rows_block() * GROUPS + group;
     if (row >= p.rows) return;
     const int share = blockIdx.y;
     const T* x = (const T*)p.x + row * p.ld;
@@ -412,6 +415,7 @@ __global__ __launch_bounds__(256) void logp_backward_kernel(LogpOp p) {
 __global__ __launch_bounds__(1024) void logp_bin_kernel(const double* part, int64_t rows, float* out) {
     __shared__ double sm[1024];
     double a = 0;
+#pragma unroll 8
     for (int64_t i = threadIdx.x; i < rows; i += 1024) a += part[i];
     sm[threadIdx.x] = a;
     for (int o = 512; o > 0; o >>= 1) {
@@ -436,9 +440,15 @@ const char* bad(int dtype, int64_t rows, int cols, int64_t ld, const void* x, bo
     if (rows < 1 || rows > 0x7fffffff) return "rows must be between 1 and 2^31 - 1";
     if (cols < (bin ? 0 : 1) || cols > (1 << 30)) return "cols must be between 1 (0 with a dustbin) and 2^30";
     if (ld < cols) return "the row stride is smaller than a row";
-    if (!x) return "null argument";
+    if (!x && cols) return "null argument";
     if ((uintptr_t)x & (dtype == IMP_DTYPE_F32 ? 3 : 1)) return "logits are not aligned to their type";
     return nullptr;
+}
+
+// `blocks` groups of rows as rows_block() counts them
+dim3 grid_of(int64_t blocks, int shares) {
+    const int64_t x = blocks < (1 << 22) ? blocks : 1 << 22;
+    return dim3((unsigned)x, (unsigned)shares, (unsigned)((blocks + x - 1) / x));
 }
 
 // pieces of 2 vectors per lane, or of 32 elements: short rows do not pay for places that they leave empty
@@ -446,11 +456,11 @@ template <typename T, bool TOP> void forward(const LogpOp& p, hipStream_t st) {
     constexpr int V = 16 / sizeof(T), U = 32 / V;
     const int per = (p.cols + p.shares - 1) / p.shares;
     if (p.shares == 1 && wave_rows(p.rows, p.cols)) {
-        const unsigned grid = (unsigned)((p.rows + 3) / 4);
+        const dim3 grid = grid_of((p.rows + 3) / 4, 1);
         if (per <= 64 * V * 2) logp_forward_kernel<T, TOP, 1, 2><<<grid, 256, 0, st>>>(p);
         else logp_forward_kernel<T, TOP, 1, U><<<grid, 256, 0, st>>>(p);
     } else {
-        const dim3 grid((unsigned)p.rows, (unsigned)p.shares);
+        const dim3 grid = grid_of(p.rows, p.shares);
         if (per <= 256 * V * 2) logp_forward_kernel<T, TOP, 4, 2><<<grid, 256, 0, st>>>(p);
         else logp_forward_kernel<T, TOP, 4, U><<<grid, 256, 0, st>>>(p);
     }
@@ -461,8 +471,8 @@ template <typename T> void forward_top(const LogpOp& p, hipStream_t st) {
     else forward<T, false>(p, st);
 }
 template <typename T> void backward(const LogpOp& p, hipStream_t st) {
-    if (p.shares == 1 && wave_rows(p.rows, p.cols)) logp_backward_kernel<T, 1><<<dim3((unsigned)((p.rows + 3) / 4), 1), 256, 0, st>>>(p);
-    else logp_backward_kernel<T, 4><<<dim3((unsigned)p.rows, (unsigned)p.shares), 256, 0, st>>>(p);
+    if (p.shares == 1 && wave_rows(p.rows, p.cols)) logp_backward_kernel<T, 1><<<grid_of((p.rows + 3) / 4, 1), 256, 0, st>>>(p);
+    else logp_backward_kernel<T, 4><<<grid_of(p.rows, p.shares), 256, 0, st>>>(p);
 }
 
 }  // namespace

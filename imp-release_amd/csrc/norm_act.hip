@@ -194,7 +194,7 @@ __device__ __forceinline__ double wave_sum(double v) {
 template <typename T>
 __global__ __launch_bounds__(256) void norm_stats_kernel(NormOp p) {
     __shared__ double2 sm[4];
-    const int at = blockIdx.x, b = at / p.G, g = at % p.G;
+    const int b = blockIdx.y, g = blockIdx.x, at = b * p.G + g;
     const double2* part = p.part + ((int64_t)b * p.C + (int64_t)g * p.cg) * p.chunks;
     const int64_t n = (int64_t)p.cg * p.chunks;
     double s = 0, t = 0;
@@ -271,7 +271,7 @@ __global__ __launch_bounds__(256, 4) void norm_grad_sums_kernel(NormOp p) {
 // one workgroup per (batch element, group): sums per channel (a wave each in turn), and the two means of the group
 __global__ __launch_bounds__(256) void norm_grad_means_kernel(NormOp p) {
     __shared__ double2 sm[4];
-    const int at = blockIdx.x, b = at / p.G, g = at % p.G, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int b = blockIdx.y, g = blockIdx.x, at = b * p.G + g, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     double m1 = 0, m2 = 0;
     for (int c = g * p.cg + wave; c < (g + 1) * p.cg; c += 4) {
         const double2* part = p.part + ((int64_t)b * p.C + c) * p.chunks;
@@ -293,11 +293,18 @@ __global__ __launch_bounds__(256) void norm_grad_means_kernel(NormOp p) {
     p.mom[at] = float2{cnt > 0 ? (float)(m1 / cnt) : 0.f, cnt > 0 ? (float)(m2 / cnt) : 0.f};
 }
 
+// dw, db: sums over the batch, 16 channels x 16 parts of it per workgroup
 __global__ __launch_bounds__(256) void norm_affine_kernel(NormOp p) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= p.C) return;
+    __shared__ double2 sm[16][16];
+    const int i = threadIdx.x % 16, part = threadIdx.x / 16, c = blockIdx.x * 16 + i;
     double s = 0, t = 0;
-    for (int b = 0; b < p.B; ++b) { const double2 v = p.chan[(int64_t)b * p.C + c]; s += v.x; t += v.y; }
+    if (c < p.C)
+#pragma unroll 4
+        for (int b = part; b < p.B; b += 16) { const double2 v = p.chan[(int64_t)b * p.C + c]; s += v.x; t += v.y; }
+    sm[part][i] = double2{s, t};
+    __syncthreads();
+    if (part || c >= p.C) return;
+    for (int k = 1; k < 16; ++k) { s += sm[k][i].x; t += sm[k][i].y; }
     if (p.db) p.db[c] = (float)s;
     if (p.dw) p.dw[c] = (float)t;
 }
@@ -369,7 +376,7 @@ __global__ __launch_bounds__(HELD_THREADS) void norm_held_kernel(NormOp p) {
     __shared__ double2 sm[HELD_THREADS * V], chan[HELD_THREADS];
     __shared__ float4 st[HELD_THREADS];
     const int col = threadIdx.x % p.tc, tr = threadIdx.x / p.tc, step = HELD_THREADS / p.tc, slab = p.tc * V;
-    const int slabs = (p.C + slab - 1) / slab, w = slab_of(blockIdx.x, gridDim.x), b = w / slabs, c0 = (w - b * slabs) * slab, c = c0 + col * V, len = len_of(p, b);
+    const int slabs = (p.C + slab - 1) / slab, w = slab_of(blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y), b = w / slabs, c0 = (w - b * slabs) * slab, c = c0 + col * V, len = len_of(p, b);
     const bool on = c < p.C && tr < step;      // (threads past the last whole row of columns have nothing)
     const T* x = (const T*)p.x + (int64_t)b * p.N * p.C + c;
     T* y = (T*)p.y + (int64_t)b * p.N * p.C + c;
@@ -428,7 +435,7 @@ __global__ __launch_bounds__(HELD_THREADS) void norm_grad_held_kernel(NormOp p) 
     __shared__ double2 sm[HELD_THREADS * V], chan[HELD_THREADS];
     __shared__ float2 mom[HELD_THREADS];
     const int col = threadIdx.x % p.tc, tr = threadIdx.x / p.tc, step = HELD_THREADS / p.tc, slab = p.tc * V;
-    const int slabs = (p.C + slab - 1) / slab, w = slab_of(blockIdx.x, gridDim.x), b = w / slabs, c0 = (w - b * slabs) * slab, c = c0 + col * V, len = len_of(p, b);
+    const int slabs = (p.C + slab - 1) / slab, w = slab_of(blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y), b = w / slabs, c0 = (w - b * slabs) * slab, c = c0 + col * V, len = len_of(p, b);
     const bool on = c < p.C && tr < step;
     const int64_t base = (int64_t)b * p.N * p.C + c;
     const T *x = (const T*)p.x + base, *dy = (const T*)p.dy + base;
@@ -596,14 +603,14 @@ int imp_group_norm_act_forward(int dtype, int batch, int n, int channels, int gr
         if (h.tc) {
             NormOp a = p;
             a.tc = h.tc;
-            const unsigned grid = (unsigned)((channels + h.tc * V - 1) / (h.tc * V)) * (unsigned)batch;
+            const dim3 grid((unsigned)((channels + h.tc * V - 1) / (h.tc * V)), (unsigned)batch);
             if (h.k <= 1) norm_held_kernel<T, V, 1, A><<<grid, HELD_THREADS, 0, st>>>(a);
             else if (h.k <= 4) norm_held_kernel<T, V, 4, A><<<grid, HELD_THREADS, 0, st>>>(a);
             else norm_held_kernel<T, V, HOLD, A><<<grid, HELD_THREADS, 0, st>>>(a);
             return;
         }
         norm_sums_kernel<T, V><<<dim3(s.chunks, s.cols, batch), 256, 0, st>>>(p);
-        norm_stats_kernel<T><<<(unsigned)(batch * groups), 256, 0, st>>>(p);
+        norm_stats_kernel<T><<<dim3((unsigned)groups, (unsigned)batch), 256, 0, st>>>(p);
         NormOp a = p;
         a.chunks = s.achunks; a.rows = s.arows;
         norm_apply_kernel<T, V, A><<<dim3(s.achunks, s.cols, batch), 256, 0, st>>>(a);
@@ -636,16 +643,16 @@ int imp_group_norm_act_backward(int dtype, int batch, int n, int channels, int g
             NormOp a = p;
             a.tc = h.tc;
             if (!dweight && !dbias) a.chan = nullptr;
-            const unsigned grid = (unsigned)((channels + h.tc * V - 1) / (h.tc * V)) * (unsigned)batch;
+            const dim3 grid((unsigned)((channels + h.tc * V - 1) / (h.tc * V)), (unsigned)batch);
             if (h.k <= 1) norm_grad_held_kernel<T, V, 1, A><<<grid, HELD_THREADS, 0, st>>>(a);
             else if (h.k <= 4) norm_grad_held_kernel<T, V, 4, A><<<grid, HELD_THREADS, 0, st>>>(a);
             else norm_grad_held_kernel<T, V, sizeof(T) == 4 ? HOLD : HOLD / 2, A><<<grid, HELD_THREADS, 0, st>>>(a);
-            if (dweight || dbias) norm_affine_kernel<<<(channels + 255) / 256, 256, 0, st>>>(p);
+            if (dweight || dbias) norm_affine_kernel<<<(channels + 15) / 16, 256, 0, st>>>(p);
             return;
         }
         norm_grad_sums_kernel<T, V, A><<<dim3(s.chunks, s.cols, batch), 256, 0, st>>>(p);
-        norm_grad_means_kernel<<<(unsigned)(batch * groups), 256, 0, st>>>(p);
-        if (dweight || dbias) norm_affine_kernel<<<(channels + 255) / 256, 256, 0, st>>>(p);
+        norm_grad_means_kernel<<<dim3((unsigned)groups, (unsigned)batch), 256, 0, st>>>(p);
+        if (dweight || dbias) norm_affine_kernel<<<(channels + 15) / 16, 256, 0, st>>>(p);
         NormOp a = p;
         a.chunks = s.achunks; a.rows = s.arows;
         norm_grad_kernel<T, V, A><<<dim3(s.achunks, s.cols, batch), 256, 0, st>>>(a);

@@ -6,7 +6,8 @@
 
 They take and return CUDA tensors (float32, float16, bfloat16), work on the current stream of the tensors' device, and are differentiable by autograd once (the gradients
 are no autograd functions themselves).  Nothing waits for the GPU and nothing is kept between calls, so they can be captured into a graph: forward, and backward with
-``torch.autograd.grad`` inside the capture.  Errors: ``ValueError`` / ``TypeError`` for arguments, ``ImpError`` from the library.  There is no CPU path.
+``torch.autograd.grad`` inside the capture, over leaves that no living eager graph holds (torch ties a leaf to the stream of its first use: give a captured pass its own,
+``leaf.detach().requires_grad_()``).  Errors: ``ValueError`` / ``TypeError`` for arguments, ``ImpError`` from the library.  There is no CPU path.
 """
 from __future__ import annotations
 
@@ -21,6 +22,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from ._lib import ACT_IDS, DTYPE_IDS, ImpAttnDesc, ImpError
 
+_INT = 2 ** 31 - 1
 OP_ACT_IDS = {**ACT_IDS, 'silu': 3, 'none': 4}
 
 
@@ -46,7 +48,15 @@ def _tensor(t, name, dtypes=tuple(DTYPE_IDS), device=None, shape=None):
 def _lens(t, name, batch, device):
     if t is None:
         return None
-    return _tensor(t, name, (torch.int32, torch.int64), device, (batch,)).to(torch.int32).contiguous()
+    _tensor(t, name, (torch.int32, torch.int64), device, (batch,))
+    return (t if t.dtype == torch.int32 else t.clamp(0, _INT).to(torch.int32)).contiguous()
+
+
+def _sizes(**sizes):
+    """the library counts in 32 bits (and has narrower bounds of its own)"""
+    for name, n in sizes.items():
+        if n > _INT:
+            raise ValueError(f'{name} must be at most {_INT}, got {n}')
 
 
 def _scratch(nbytes, device):
@@ -187,7 +197,7 @@ def attention(q, k, v, key_mask: Optional[torch.Tensor] = None, q_lens=None, k_l
 
     q [batch, nq, heads, head_dim]; k, v [batch, nk, kv_heads, head_dim] with heads a multiple of kv_heads (query head h reads key head h // (heads // kv_heads)) and
     head_dim a multiple of 8 up to 128.  Views of a packed projection are taken without a copy.  key_mask [batch, nk] bool / uint8, True = keep; q_lens, k_lens [batch]
-    int32: counts of a ragged batch.  scale: 1 / sqrt(head_dim) unless given.  -> out [batch, nq, heads, head_dim] (and lse float32 [batch, heads, nq], which carries no
+    int32: counts of a ragged batch.  batch x kv_heads is at most 65535.  scale: 1 / sqrt(head_dim) unless given.  -> out [batch, nq, heads, head_dim] (and lse float32 [batch, heads, nq], which carries no
     gradient).  A query without a key, or past its count, gives 0 and -inf and has no gradient."""
     _tensor(q, 'q')
     if q.dim() != 4:
@@ -198,6 +208,8 @@ def attention(q, k, v, key_mask: Optional[torch.Tensor] = None, q_lens=None, k_l
         if t.dim() != 4 or t.shape[0] != b or t.shape[3] != dh or t.shape != k.shape:
             raise ValueError(f'{name} must be [batch, tokens, kv_heads, head_dim] like q {tuple(q.shape)}, got {tuple(t.shape)}')
     nk, kv = k.shape[1], k.shape[2]
+    if max(b, nq, nk, h) > _INT:
+        _sizes(batch=b, nq=nq, nk=nk, heads=h)
     if dh < 8 or dh > 128 or dh % 8:
         raise ValueError(f'head_dim must be a multiple of 8 up to 128, got {dh}')
     if kv < 1 or h < 1 or h % kv:
@@ -271,7 +283,7 @@ def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-3, ac
 
     x [batch, ..., channels]; mean and (biased) variance over everything between batch and channels and over the channels of a group (``groups`` groups of neighbouring
     channels; groups == channels is InstanceNorm).  weight, bias: float32 [channels], optional.  act: 'relu', 'gelu', 'lrelu' (slope 0.1), 'silu' or 'none'.  lens [batch]
-    int32: only the first tokens of each element exist (x must then be [batch, tokens, channels]); the others are not read and give 0.  eps is the matcher's 1e-3."""
+    int32: only the first tokens of each element exist (x must then be [batch, tokens, channels]); the others are not read and give 0.  At most 65535 batch elements and 2^20 channels.  eps is the matcher's 1e-3."""
     _tensor(x, 'x')
     if x.dim() < 3:
         raise ValueError(f'x must be [batch, ..., channels], got {tuple(x.shape)}')
@@ -289,6 +301,8 @@ def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-3, ac
         if t is not None:
             _tensor(t, name, (torch.float32,), x.device, (c,))
     lens = _lens(lens, 'lens', b, x.device)
+    if x.numel() > _INT:
+        _sizes(batch=b, tokens=x.numel() // (b * c), channels=c)
     if x.numel() == 0:
         return x + sum(t.sum() * 0 for t in (weight, bias) if t is not None)
     flat = (x if x.dim() == 3 else x.reshape(b, -1, c)).contiguous()
@@ -347,6 +361,8 @@ class _LogProbs(torch.autograd.Function):
         dlogp, dentropy = (None if t is None else _dense(t, torch.float32) for t in (dlogp, dentropy))
         dx = torch.empty((rows, cols), device=x.device, dtype=x.dtype) if want_x else None
         dbin = torch.empty_like(bin_score) if want_bin else None
+        if cols == 0 and not want_bin:       # nothing but the dustbin
+            return dx, None, None, None
         need = _logp_scratch(rows, cols, 0, 1) if want_bin else 0
         ws = _scratch(need, x.device)
         _check(_lib.lib().imp_log_probs_backward(DTYPE_IDS[x.dtype], rows, cols, _ld(x), x.data_ptr(), _at(bin_score), targets.data_ptr(), entropy.data_ptr(),
@@ -376,6 +392,8 @@ def match_log_probs(logits, targets, bin_score=None, top: int = 0):
     elif cols == 0:
         raise ValueError('logits need at least one column, or a bin_score')
     rows = targets.numel()
+    if max(rows, cols) > _INT:
+        _sizes(rows=rows, cols=cols)
     if rows == 0:
         z = logits.sum(-1).float() * 0 + (0 if bin_score is None else bin_score.sum() * 0)
         return z, z * 1, logits.new_empty(*lead, top, dtype=torch.float32), logits.new_empty(*lead, top, dtype=torch.int64)

@@ -493,7 +493,8 @@ int imp_sp_op_conv(imp_sp_ctx* ctx, int layer, const float* in, int B, int H, in
 /* Multi-head attention with gradients (csrc/attention_grad.hip; the operation of nets/layers.py:121-131 with any number of heads, shared key heads and types):
  *   S = scale q.k   P = softmax of S over the kept keys   out = P v   lse = log sum exp S
  * q [batch][nq][heads][head_dim], k, v [batch][nk][kv_heads][head_dim], all of `dtype`, channels contiguous, other strides in elements (batch, token, head; multiples of
- * 16 bytes, so a packed q | k | v projection is taken as it lies; 64 tokens within 2^30 bytes); query head h reads key head h / (heads / kv_heads).  head_dim a multiple of 8 up to 128.
+ * 16 bytes, so a packed q | k | v projection is taken as it lies; 64 tokens within 2^30 bytes); query head h reads key head h / (heads / kv_heads).  head_dim a multiple of 8 up to 128,
+ * batch x kv_heads up to 65535.
  * key_mask: optional uint8 [batch][nk], 0 = the key does not exist; q_lens / k_lens: optional int32 [batch] counts of a ragged batch (clamped to 0 .. nq / nk).  What does not
  * exist is never read into a result (it may hold NaN).  A query without a key, and a query past its count: out 0, lse -inf, no gradient. */
 typedef struct imp_attn_desc {
@@ -516,7 +517,7 @@ int imp_attn_backward(const imp_attn_desc* d, const void* q, const void* k, cons
 
 /* Group norm + activation on token-major data (csrc/norm_act.hip; groups == channels: the InstanceNorm + activation of nets/layers.py:59-77): x, y [batch][n][channels] of
  * `dtype`, weight / bias float32 [channels] (optional), lens int32 [batch] (optional; clamped to 0 .. n; tokens past it are not read, y and dx are 0 there), act IMP_ACT_*,
- * stats float32 [batch][groups][4] (mean and rstd, two floats each): written by the forward, read by the backward. */
+ * batch up to 65535, channels up to 2^20, stats float32 [batch][groups][4] (mean and rstd, two floats each): written by the forward, read by the backward. */
 #define IMP_ACT_SILU 3      /* these operators only */
 #define IMP_ACT_NONE 4
 int imp_group_norm_act_workspace(int dtype, int batch, int n, int channels, int groups, int backward, uint64_t* bytes);

@@ -120,6 +120,16 @@ def test_attention_ragged_masks_and_garbage(dtype):
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('b,nq,nk,h,kv,dh', [(1, 70, 90, 6, 2, 32), (2, 5, 3001, 3, 1, 64), (1, 300, 400, 7, 1, 128), (1, 1000, 70, 10, 2, 64)])
+def test_attention_head_groups_of_any_size(dtype, b, nq, nk, h, kv, dh):
+    """3, 5 and 7 query heads per key head, and byte masks of any nonzero value"""
+    q, k, v = rand(b, nq, h, dh, seed=1, dtype=dtype), rand(b, nk, kv, dh, seed=2, dtype=dtype), rand(b, nk, kv, dh, seed=3, dtype=dtype)
+    mask = torch.randint(0, 3, (b, nk), generator=torch.Generator().manual_seed(5), dtype=torch.uint8).to(DEV) * 127
+    out, _ = attention_case(q, k, v, rand(b, nq, h, dh, seed=4, scale=0.1, dtype=dtype), TOL[dtype], key_mask=mask)
+    assert torch.equal(out, ops.attention(q, k, v, key_mask=mask != 0))
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
 def test_attention_packed_projection_and_strides(dtype):
     """q | k | v side by side, [batch, heads, tokens, channels] storage, and views that need a copy: the same bits as contiguous operands"""
     b, n, h, dh = 2, 77, 4, 32
@@ -512,6 +522,116 @@ def test_log_probs_refusals():
                 lambda: ops.match_log_probs(x.double(), t), lambda: ops.match_log_probs(x, t, torch.zeros((), device=DEV).half())):
         with pytest.raises((ValueError, TypeError)):
             bad()
+
+
+# ------------------------------------------------------------------------------------------------------------------------ far and many
+def test_sizes_past_32_bits_are_refused():
+    """a count that would wrap around in the library is refused, not taken modulo 2^32 (views without memory)"""
+    n = 2 ** 32 + 5
+    q = rand(1, 5, 2, 16)
+    far = rand(1, 1, 2, 16).expand(1, n, 2, 16)
+    for bad in (lambda: ops.attention(q, far, far), lambda: ops.attention(far, q, q), lambda: ops.group_norm_act(rand(1, 1, 8).expand(1, n, 8), 2),
+                lambda: ops.match_log_probs(rand(1, 1).expand(1, n), torch.zeros(1, dtype=torch.int64, device=DEV)),
+                lambda: ops.match_log_probs(rand(1, 1).expand(n, 1), torch.zeros(1, dtype=torch.int64, device=DEV).expand(n))):
+        with pytest.raises(ValueError, match='at most'):
+            bad()
+
+
+def test_counts_in_64_bits():
+    """a count beyond 2^32 is clamped to the tensor like any other that is too large"""
+    q, k = rand(2, 9, 2, 16, seed=1), rand(2, 40, 2, 16, seed=2)
+    big = torch.tensor([2 ** 32 + 3, -2 ** 33 - 7], device=DEV)
+    want = torch.tensor([2 ** 31 - 1, 0], device=DEV, dtype=torch.int32)
+    assert torch.equal(ops.attention(q, k, k, k_lens=big), ops.attention(q, k, k, k_lens=want))
+    x = rand(2, 30, 8, seed=3)
+    assert torch.equal(ops.group_norm_act(x, 4, lens=big), ops.group_norm_act(x, 4, lens=want))
+
+
+@pytest.mark.parametrize('nq', [1, 70])
+def test_attention_over_a_cache_past_32_bits(nq):
+    """keys and values as views of a storage whose tokens lie 2^19 elements apart: offsets past 2^32 bytes"""
+    nk, h, kv, dh, step = 4100, 4, 2, 64, 1 << 19
+    store = torch.empty(nk * step, device=DEV, dtype=torch.bfloat16)
+    k, v = (store.as_strided((1, nk, kv, dh), (nk * step, step, dh, 1), at) for at in (0, 4096))
+    k.copy_(rand(1, nk, kv, dh, seed=1, dtype=torch.bfloat16))
+    v.copy_(rand(1, nk, kv, dh, seed=2, dtype=torch.bfloat16))
+    q, dout = rand(1, nq, h, dh, seed=3, dtype=torch.bfloat16), rand(1, nq, h, dh, seed=4, dtype=torch.bfloat16)
+
+    def once(k, v):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = ops.attention(*leaves)
+        return (out.detach(),) + torch.autograd.grad(out, leaves, dout)
+    for a, b in zip(once(k, v), once(k.contiguous(), v.contiguous())):
+        assert torch.equal(a, b)
+
+
+def test_group_norm_past_32_bits():
+    n, c, tol = (1 << 25) + 7, 64, TOL[torch.float16]
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x, dy = (torch.randn(1, n, c, generator=g, device=DEV, dtype=torch.float16) for _ in range(2))
+    lx = x.detach().requires_grad_()
+    y = ops.group_norm_act(lx, c, act='none')
+    dx = torch.autograd.grad(y, lx, dy)[0]
+    sums = torch.zeros(4, c, device=DEV, dtype=torch.float64)
+    for i in range(0, n, 1 << 22):
+        a, d = x[0, i:i + (1 << 22)].double(), dy[0, i:i + (1 << 22)].double()
+        sums += torch.stack([a.sum(0), (a * a).sum(0), d.sum(0), (a * d).sum(0)])
+    mean, sq, m1, md = sums / n
+    r = 1 / (sq - mean * mean + 1e-3).sqrt()
+    m2 = (md - mean * m1) * r
+    for rows in (slice(0, 300), slice(n - 300, n)):
+        xh = (x[0, rows].double() - mean) * r
+        close(y[0, rows].detach(), xh, tol, 'y')
+        close(dx[0, rows], (dy[0, rows].double() - m1 - xh * m2) * r, tol, 'dx')
+
+
+def test_group_norm_of_many_elements():
+    """more workgroups than the x dimension of a grid has threads for, and an affine gradient summed over all of them"""
+    b, c = 65535, 2048
+    x, w = rand(1, 1, c, seed=1).expand(b, 2, c) * torch.linspace(1, 2, 2, device=DEV)[:, None], rand(c, seed=2)
+    lx, lw = x.detach().requires_grad_(), w.detach().requires_grad_()
+    y = ops.group_norm_act(lx, 128, lw, act='none')
+    dw, = torch.autograd.grad(y, lw, torch.ones_like(y))
+    want = norm64(x[:1], 128, w, act='none')
+    for i in (0, 32768, b - 1):
+        close(y[i:i + 1].detach(), want, F32, f'element {i}')
+    close(dw, (norm64(x[:1], 128, act='none').sum((0, 1)) * b), 2e-5, 'dw')            # (a sum of two normalised values of either sign: up to 4 times smaller than they are)
+
+
+def test_log_probs_of_many_rows():
+    """more rows than the x dimension of a grid has threads for"""
+    rows = (1 << 26) + 5
+    x = torch.randn(rows, 2, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).half()
+    t = torch.randint(0, 2, (rows,), generator=torch.Generator(device=DEV).manual_seed(2), device=DEV)
+    lx = x.detach().requires_grad_()
+    logp, ent, _, ids = ops.match_log_probs(lx, t, top=1)
+    dx = torch.autograd.grad(logp, lx, torch.ones_like(logp))[0]
+    d = x.double()
+    lp = d - torch.logsumexp(d, 1, keepdim=True)
+    close(logp.detach(), lp.gather(1, t[:, None])[:, 0], F32, 'logp')
+    close(ent.detach(), -(lp.exp() * lp).sum(1), F32, 'entropy')
+    assert torch.equal(ids[:, 0], (d[:, 1] > d[:, 0]).long())
+    close(dx, torch.nn.functional.one_hot(t, 2) - lp.exp(), TOL[torch.float16], 'dx')
+
+
+def test_log_probs_of_rows_far_apart():
+    store = torch.empty(4, 1 << 30, device=DEV, dtype=torch.float16)
+    x = store[:, :700]
+    x.copy_(rand(4, 700, seed=1, dtype=torch.float16))
+    t = torch.tensor([0, 699, 5, -1], device=DEV)
+    a, b = (ops.match_log_probs(v, t, top=3) for v in (x, x.contiguous()))
+    assert all(torch.equal(i, j) for i, j in zip(a, b))
+
+
+def test_log_probs_of_the_dustbin_alone():
+    z = torch.tensor(0.5, device=DEV, requires_grad=True)
+    x = torch.empty(3, 0, device=DEV, requires_grad=True)
+    t = torch.tensor([-1, 0, -2], device=DEV)
+    logp, ent, tl, ti = ops.match_log_probs(x, t, z, top=2)
+    assert (logp == 0).all() and (ent == 0).all() and (ti == torch.tensor([0, -1], device=DEV)).all() and (tl[:, 0] == 0).all() and (tl[:, 1] == -math.inf).all()
+    dx, dz = torch.autograd.grad(logp.sum() + ent.sum(), (x, z))
+    assert dx.shape == (3, 0) and dz == 0
+    assert torch.autograd.grad(ops.match_log_probs(x, t, z.detach())[0].sum(), x)[0].shape == (3, 0)
 
 
 # ------------------------------------------------------------------------------------------------------------------------- together
