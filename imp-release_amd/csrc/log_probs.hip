@@ -91,8 +91,9 @@ struct List {
     // x, at: uniform; later elements have higher indices, so a tie goes behind
     __device__ void insert(float x, int at, int lane) {
         const int pos = __popcll(__ballot(lane < top && v >= x));
-        const float pv = __shfl_up(v, 1);
-        const int pi = __shfl_up(i, 1);
+        // the neighbour's (a shift of the whole wave by one lane)
+        const float pv = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), 0x138, 0xf, 0xf, false));
+        const int pi = __builtin_amdgcn_update_dpp(i, i, 0x138, 0xf, 0xf, false);
         if (lane > pos) { v = pv; i = pi; }
         if (lane == pos) { v = x; i = at; }
     }
@@ -102,8 +103,7 @@ struct List {
 template <typename T> __device__ __forceinline__ void finish(const LogpOp& p, int64_t row, const State& st) {
     const float l = log1pf(st.s);
     const bool none = st.m == -INFINITY;
-    p.stats[2 * row] = st.m;
-    p.stats[2 * row + 1] = l;
+    if (p.stats) { p.stats[2 * row] = st.m; p.stats[2 * row + 1] = l; }
     p.entropy[row] = none ? 0.f : l + st.u / (1.f + st.s);
     const int64_t t = p.target[row];
     float lp = 0.f;
@@ -340,17 +340,20 @@ __global__ __launch_bounds__(256) void logp_join_kernel(LogpOp p) {
     float hv = -INFINITY;
     int hi = 0x7fffffff;
     if (p.top) head(hv, hi);
+    float mine = -INFINITY;              // place k in lane k
+    int mi = 0;
     for (int k = 0; k < p.top; ++k) {
         const float v = wave_max(hv);
         // shares lie in the order of their columns: the first lane with the value has the lowest index
         const int l = __builtin_ctzll(__ballot(hv == v));
         const int i = __builtin_amdgcn_readlane(hi, l);
-        if (lane == 0) write_top(p, row, k, st, v, i);
+        if (lane == k) { mine = v; mi = i; }
         if (lane == l) {
             ++place;
             head(hv, hi);
         }
     }
+    if (lane < p.top) write_top(p, row, lane, st, mine, mi);
     if (lane == 0) finish<T>(p, row, st);
 }
 
@@ -426,9 +429,10 @@ __global__ __launch_bounds__(1024) void logp_bin_kernel(const double* part, int6
 }
 
 // ------------------------------------------------------------------------------------------------------------------------- host
-// shares of a row: enough workgroups for four per CU, each with at least 2048 columns; at most 64 (a lane each in the join)
+// shares of a row: enough workgroups for four per CU, each with one short piece of 2048 columns where there are workgroups enough for that; at most 64 (a lane each in the
+// join).  Rows below 4096 columns stay whole: the second launch costs more
 int shares_of(int64_t rows, int cols) {
-    const int64_t want = (1024 + rows - 1) / rows, most = cols / 2048;
+    const int64_t want = (1024 + rows - 1) / rows, most = cols < 4096 ? 1 : (cols + 2047) / 2048;
     const int64_t s = want < most ? want : most;
     return s < 1 ? 1 : (s > 64 ? 64 : (int)s);
 }
@@ -491,7 +495,7 @@ int imp_log_probs_forward(int dtype, int64_t rows, int cols, int64_t ld, const v
                           float* entropy, float* stats, float* top_logp, int64_t* top_ids, void* workspace, uint64_t workspace_bytes, int device, void* stream) {
     if (const char* why = bad(dtype, rows, cols, ld, logits, bin_score != nullptr)) return imp_fail(IMP_E_ARG, why);
     if (top < 0 || top > TOP_MAX) return imp_fail(IMP_E_ARG, "top must be between 0 and 16");
-    if (!targets || !logp || !entropy || !stats || (top && (!top_logp || !top_ids))) return imp_fail(IMP_E_ARG, "imp_log_probs_forward: null argument");
+    if (!targets || !logp || !entropy || (top && (!top_logp || !top_ids))) return imp_fail(IMP_E_ARG, "imp_log_probs_forward: null argument");
     uint64_t need = 0;
     imp_log_probs_workspace(rows, cols, top, 0, &need);
     if (workspace_bytes < need || (need && (!workspace || ((uintptr_t)workspace & 3)))) return imp_fail(IMP_E_NOMEM, "imp_log_probs_forward: workspace too small");

@@ -327,16 +327,16 @@ def _ld(x):
     return x.shape[1] if x.shape[0] == 1 else x.stride(0)
 
 
-def _logp_forward(x, targets, bin_score, top):
+def _logp_forward(x, targets, bin_score, top, want_stats):
     rows, cols = x.shape
     dev = x.device
     need = _logp_scratch(rows, cols, top, 0)
     logp, entropy = torch.empty(rows, device=dev, dtype=torch.float32), torch.empty(rows, device=dev, dtype=torch.float32)
-    stats = torch.empty((rows, 2), device=dev, dtype=torch.float32)
+    stats = torch.empty((rows, 2), device=dev, dtype=torch.float32) if want_stats else None
     top_logp, top_ids = torch.empty((rows, top), device=dev, dtype=torch.float32), torch.empty((rows, top), device=dev, dtype=torch.int64)
     ws = _scratch(need, dev)
     _check(_lib.lib().imp_log_probs_forward(DTYPE_IDS[x.dtype], rows, cols, _ld(x), x.data_ptr(), _at(bin_score), targets.data_ptr(), top, logp.data_ptr(),
-                                            entropy.data_ptr(), stats.data_ptr(), top_logp.data_ptr() if top else None, top_ids.data_ptr() if top else None, _at(ws),
+                                            entropy.data_ptr(), _at(stats), top_logp.data_ptr() if top else None, top_ids.data_ptr() if top else None, _at(ws),
                                             need, *_where(x)))
     return logp, entropy, stats, top_logp, top_ids
 
@@ -344,7 +344,7 @@ def _logp_forward(x, targets, bin_score, top):
 class _LogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, bin_score, targets, top):
-        logp, entropy, stats, top_logp, top_ids = _logp_forward(x, targets, bin_score, top)
+        logp, entropy, stats, top_logp, top_ids = _logp_forward(x, targets, bin_score, top, True)
         ctx.save_for_backward(x, bin_score, targets, entropy, stats)
         ctx.mark_non_differentiable(top_logp, top_ids)
         ctx.set_materialize_grads(False)
@@ -405,7 +405,7 @@ def match_log_probs(logits, targets, bin_score=None, top: int = 0):
     if torch.is_grad_enabled() and (logits.requires_grad or (bin_score is not None and bin_score.requires_grad)):
         logp, entropy, top_logp, top_ids = _LogProbs.apply(x, bin_score, t, top)
     else:
-        logp, entropy, _, top_logp, top_ids = _logp_forward(x, t, bin_score, top)
+        logp, entropy, _, top_logp, top_ids = _logp_forward(x, t, bin_score, top, False)
     if flat:
         return logp, entropy, top_logp, top_ids
     return logp.view(lead), entropy.view(lead), top_logp.view(*lead, top), top_ids.view(*lead, top)

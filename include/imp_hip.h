@@ -531,7 +531,7 @@ int imp_group_norm_act_backward(int dtype, int batch, int n, int channels, int g
 /* Log probabilities of given matches (csrc/log_probs.hip; the row softmax of nets/layers.py:20-24 as a loss and as a confidence): logits [rows][cols] of `dtype`, row stride
  * `ld` elements; bin_score: optional DEVICE float32, the dustbin: one more column `cols` of that value in every row (cols may then be 0).  targets int64 [rows]: a column; -1 =
  * unmatched (the dustbin where there is one, else no target); -2 = no target; anything else gives NaN.  logp float32 [rows] = log softmax at the target (0 without a target),
- * entropy float32 [rows] of the whole row, stats float32 [rows][2] for the backward, top_logp float32 / top_ids int64 [rows][top] the `top` <= 16 largest columns, largest
+ * entropy float32 [rows] of the whole row, stats float32 [rows][2] (optional: needed by the backward), top_logp float32 / top_ids int64 [rows][top] the `top` <= 16 largest columns, largest
  * first, ties to the lower index (the dustbin is column `cols`; -inf / -1 where there are no more).  A logit of -inf is masked: no probability, never an alternative; a row of
  * nothing else: logp -inf, entropy 0, no gradient.  A row with a NaN or +inf: NaN. */
 int imp_log_probs_workspace(int64_t rows, int cols, int top, int backward, uint64_t* bytes);
