@@ -24,6 +24,13 @@
 //   fp32, many rows: split halves as in the inference kernels (x = hi + lo in f16, 22 bits, three MFMAs), each tensor scaled per key head by a power of two that a first
 //         small launch takes from its largest finite value - no operand limit, and what is small against the head's largest value keeps 2^-39 of that
 //   fp32, few rows: three bf16 planes (24 bits, the whole fp32 range) and six MFMAs - twice the matrix work where it does not bound, without the extra launch
+//
+// What bounds it: the matrix work, and beside it the vector work per score (an exponential and about ten instructions; at 32 channels that is what bounds).  Measured
+// against what a large library product reaches on the same card (bf16 1127, f16 1082, fp32 152 TF):
+//   bf16, 16 heads over 4, 128 channels, 8192 x 8192    forward 0.58 ms = 950 TF   dQ 0.75 ms = 1100 TF (three products)   dK / dV 1.24 ms = 890 TF (four)   D 17 us
+//   fp32, 8 x 4 heads, 64 channels, 2048 x 2048         forward 124 us = 277 TF (830 executed)   dQ 170 us = 303   dK / dV 220 us = 312   scales 10 - 13 us   D 7 us
+//   f16, 16 ragged pairs x 4 heads, 32 channels, 1531 x 1777    forward 47 us   dQ 62 us   dK / dV 63 us   D 9 us
+//   bf16, 1 query x 4096 keys x 4 heads of 64            walk 6 us (32 shares)   join 4 us
 #include "../../include/imp_hip.h"
 #include "imp_kernels.h"
 
@@ -438,6 +445,10 @@ __global__ __launch_bounds__(256) void attn_amax_kernel(AttnOp p) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------- forward
+// Bound by the matrix instructions (two per score and 32 channels; 85 % of a library product's rate at 128 channels) and, at 32 channels, by the exponentials.  64 keys a tile in
+// 16-bit types, 32 in fp32 (the planes fill LDS): the next tile's loads are under way during the whole of this one, and nothing waits for them before.  What the steps brought
+// (8192 keys bf16 / 8 x 2048 fp32): tiles without bank conflicts and two waves per SIMD 1010 -> 662 / 154 -> 133 us, fetches through buffer descriptors 676 -> 581 / 139 -> 125,
+// operands read a group ahead 581 -> 564.
 template <typename A, int DHP, bool CHECK>
 __global__ __launch_bounds__(256, A::NP == 3 && DHP == 128 ? 1 : 2) void attn_fwd_kernel(AttnOp p) {
     using T = typename A::T;
@@ -624,7 +635,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnOp p) {
 }
 
 // --------------------------------------------------------------------------------------------------------------------- backward
-// D = rowsum(dO O): 16 lanes per row of [B][nq][H][dh]
+// D = rowsum(dO O): 16 lanes per row of [B][nq][H][dh].  Bound by memory: 100 MB in 13 - 17 us at 8192 x 16 x 128 bf16
 template <typename T>
 __global__ __launch_bounds__(256) void attn_delta_kernel(AttnOp p) {
     const int64_t rows = (int64_t)p.B * p.nq * p.H, row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 16 + (threadIdx.x >> 4);
@@ -661,6 +672,9 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(AttnOp p) {
 // the exponent reference of a row: lse in log2 units, +inf (P = 0) for rows that do not exist or have no key
 __device__ __forceinline__ float row_ref(float lse) { return lse == -INFINITY ? INFINITY : lse * LOG2E; }
 
+// dQ: as the forward, with three products per score and no running maximum - P comes from the forward's lse.  Bound by the matrix instructions (bf16, 128 channels: what a
+// library product of this size reaches).  A dK / dV kernel that also summed dQ would save two of the seven products but have to add to dQ with atomics, in an order that changes
+// from run to run, or write a partial per tile of keys.
 template <typename A, int DHP, bool CHECK>
 __global__ __launch_bounds__(256, A::NP > 1 && DHP == 128 ? 1 : 2) void attn_dq_kernel(AttnOp p) {
     using T = typename A::T;
@@ -811,6 +825,8 @@ __device__ __forceinline__ void store_dkv(const AttnOp& p, int b, int hk, int ke
         }
 }
 
+// dK / dV: owns 128 keys, walks the queries of each of the key head's query heads in turn.  Four products per score; 2 x DHP accumulators and the owned key and value as operands
+// leave no registers for the look-ahead in fp32 at 64 channels (it spills; 214 - 230 us at 8 x 2048 without).
 template <typename A, int DHP, bool CHECK>
 __global__ __launch_bounds__(256, DHP == 128 || (A::NP == 3 && DHP == 64) ? 1 : 2) void attn_dkv_kernel(AttnOp p) {
     using T = typename A::T;
@@ -954,7 +970,8 @@ __global__ __launch_bounds__(256, DHP == 128 || (A::NP == 3 && DHP == 64) ? 1 : 
 
 // dK / dV for 128 channels in 16-bit types: 128 fp32 accumulators and 64 registers of operands leave a wave of the kernel above alone on its SIMD.  Here two waves share 32 keys:
 // wave h computes the scores of the h-th 32 rows of a tile, hands P and dS on through LDS (in the operand layout they are used in), and sums its half of the channels over
-// both.  No product is computed twice; 64 accumulators, two waves per SIMD.
+// both.  No product is computed twice; 64 accumulators, two waves per SIMD: 1870 -> 1681 us at 8192 keys bf16 when it came, 1.24 ms with the buffer descriptors and addresses
+// formed again at use, 890 TF of a library product's 1127; what is left is the hand-over's two barriers per 32 rows.
 template <typename A, bool CHECK>
 __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
     using T = typename A::T;
