@@ -27,7 +27,7 @@
 //
 // What bounds it: the matrix work, and beside it the vector work per score (an exponential and about ten instructions; at 32 channels that is what bounds).  Measured
 // against what a large library product reaches on the same card (bf16 1127, f16 1082, fp32 152 TF):
-//   bf16, 16 heads over 4, 128 channels, 8192 x 8192    forward 0.58 ms = 950 TF   dQ 0.75 ms = 1100 TF (three products)   dK / dV 1.24 ms = 890 TF (four)   D 17 us
+//   bf16, 16 heads over 4, 128 channels, 8192 x 8192    forward 0.58 ms = 950 TF   dQ 0.75 ms = 1100 TF (three products)   dK / dV 1.16 ms = 950 TF (four)   D 17 us
 //   fp32, 8 x 4 heads, 64 channels, 2048 x 2048         forward 124 us = 277 TF (830 executed)   dQ 170 us = 303   dK / dV 220 us = 312   scales 10 - 13 us   D 7 us
 //   f16, 16 ragged pairs x 4 heads, 32 channels, 1531 x 1777    forward 47 us   dQ 62 us   dK / dV 63 us   D 9 us
 //   bf16, 1 query x 4096 keys x 4 heads of 64            walk 6 us (32 shares)   join 4 us
@@ -970,8 +970,9 @@ __global__ __launch_bounds__(256, DHP == 128 || (A::NP == 3 && DHP == 64) ? 1 : 
 
 // dK / dV for 128 channels in 16-bit types: 128 fp32 accumulators and 64 registers of operands leave a wave of the kernel above alone on its SIMD.  Here two waves share 32 keys:
 // wave h computes the scores of the h-th 32 rows of a tile, hands P and dS on through LDS (in the operand layout they are used in), and sums its half of the channels over
-// both.  No product is computed twice; 64 accumulators, two waves per SIMD: 1870 -> 1681 us at 8192 keys bf16 when it came, 1.24 ms with the buffer descriptors and addresses
-// formed again at use, 890 TF of a library product's 1127; what is left is the hand-over's two barriers per 32 rows.
+// both.  No product is computed twice; 64 accumulators, two waves per SIMD: 1870 -> 1681 us at 8192 keys bf16 when it came, 1246 with the buffer descriptors and addresses formed
+// again at use, 1160 with the matrix work before the other wave's, 950 TF of a library product's 1127.  What is left: LDS, of which eight waves read 320 KB per 2048 cycles of
+// matrix work (156 bytes a cycle, the peak is 128).
 template <typename A, bool CHECK>
 __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
     using T = typename A::T;
@@ -1062,6 +1063,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
             if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
         };
         f32x16 s = zero16(), dp = zero16();
+        __builtin_amdgcn_s_setprio(1);   // matrix work goes before the other wave's vector work: 1246 -> 1160 us (the kernels above gain nothing by it)
         if (PIPE) read(0);
 #pragma unroll
         for (int i = 0; i < 2 * SG; ++i) {
@@ -1071,6 +1073,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
             else first_product<A, KS>(buf[i & 1], vf, (i - SG) * GN, dp);
             if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const f32x4 rv = *(const f32x4*)(refs + 32 * h + 8 * g + 4 * half);
@@ -1103,6 +1106,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
                 hand[wave][(2 * k + 1) * WP + w][lane] = df[k][w];
             }
         }
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int k = 0; k < 2; ++k) sums(2 * SG + k, pf[k], df[k]);
         __syncthreads();
@@ -1116,6 +1120,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_pair_kernel(AttnOp p) {
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) sums(2 * SG + 2 + k, pf[k], df[k]);
+        __builtin_amdgcn_s_setprio(0);
     }
     if (key >= p.nk) return;
     if (!live) {
