@@ -248,7 +248,7 @@ __global__ __launch_bounds__(256) void logp_forward_kernel(LogpOp p) {
                 for (int i = 0; i < V; ++i) bad |= f[j][i] != f[j][i];
         }
         if constexpr (TOP) {
-            if (out) put(out_l, out_j, out_i, m);
+            if (out) list.insert(m, base + ((out_j * W + part) * 64 + out_l) * V + out_i, lane);       // larger than all before it, and already taken out
             for (float last = list.last();;) {
                 best = vm[0];
 #pragma unroll
