@@ -249,7 +249,8 @@ __global__ __launch_bounds__(256) void logp_forward_kernel(LogpOp p) {
         }
         if constexpr (TOP) {
             if (out) list.insert(m, base + ((out_j * W + part) * 64 + out_l) * V + out_i, lane);       // larger than all before it, and already taken out
-            for (float last = list.last();;) {
+            float last = list.last();
+            for (int n = out; n < p.top; ++n) {      // (`top` places from one piece: nothing larger is left in it)
                 best = vm[0];
 #pragma unroll
                 for (int j = 1; j < U; ++j) best = fmaxf(best, vm[j]);
