@@ -11,9 +11,9 @@
 //   m = max, s = s_a + (s_b + 1) f, U = U_a + f (U_b + d (s_b + 1)), f = exp(-d), d = m_a - m_b >= 0            (the smaller maximum becomes an ordinary element)
 // waves and - when there are few rows - shares of a row are joined in a fixed order.  The alternatives are taken out of the registers one by one, largest first, as long as the
 // piece holds something larger than the last place of the wave's list.  Measured (a large copy on this card: 5.0 TB/s):
-//   8192 x 2048 fp32 with a dustbin and four alternatives 23 us (2.9 TB/s; each place taken out costs a wave-wide maximum)
+//   8192 x 2048 fp32 with a dustbin and four alternatives 21.5 us (3.1 TB/s; each place taken out costs a wave-wide maximum)
 //   4096 x 50001 bf16: forward 113 - 118 us (3.5 TB/s, bound by the exponentials and conversions: 94 - 101 us where rows begin on 16 bytes), backward 160 us (5.1 TB/s)
-//   1 x 65537 fp32 with eight alternatives: 10 us, and 6 for the join
+//   1 x 65537 fp32 with eight alternatives: 9.3 us, and 5.8 for the join
 #include "../../include/imp_hip.h"
 #include "imp_kernels.h"
 
