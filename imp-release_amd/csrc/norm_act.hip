@@ -30,7 +30,7 @@ struct NormOp {
     float4* stats;                      // [batch][groups] mean (two floats), rstd (two floats)
     double2* part;                      // [batch][channels][chunks]
     double2* chan;                      // backward: [batch][channels] sums over the tokens
-    float2* mom;                        // backward: [batch][groups] mean(g), mean(g xh)
+    float2* mom;                        // backward: [batch][groups] m of dx_of
     float *dw, *db;
     int B, N, C, G, cg, act;
     float eps;
@@ -84,28 +84,30 @@ template <typename F> void with_act(int act, F f) {
     }
 }
 
-// What a thread needs of its V channels.  The slope of relu / lrelu jumps where z = w xh + b passes 0, that is where x passes mean - b / (w rstd): one threshold per channel,
+// What a thread needs of its V channels: z = w (x - mean) rstd + b = a (x - mh) + c, one subtraction and one fma per element (mh: the mean as a float; c takes the rest of it).
+// The slope of relu / lrelu jumps where z = w xh + b passes 0, that is where x passes mean - b / (w rstd): one threshold per channel,
 // formed in 64 bits and rounded down, decides for every x exactly (up: +-1, the sign of w; x is compared as up x)
 template <int V, int ACT> struct Chan {
     static constexpr bool JUMP = ACT == IMP_ACT_RELU || ACT == IMP_ACT_LRELU;
-    float mh[V], ml[V], rh[V], w[V], b[V], up[JUMP ? V : 1], edge[JUMP ? V : 1];
-    __device__ void set(const NormOp& p, int c, int i, const float4& s) {
-        mh[i] = s.x; ml[i] = s.y; rh[i] = s.z;
-        w[i] = p.w ? p.w[c] : 1.f;
-        b[i] = p.b ? p.b[c] : 0.f;
+    float mh[V], a[V], c[V], up[JUMP ? V : 1], edge[JUMP ? V : 1];
+    __device__ void set(const NormOp& p, int at, int i, const float4& s) {
+        const float w = p.w ? p.w[at] : 1.f, b = p.b ? p.b[at] : 0.f;
+        mh[i] = s.x;
+        a[i] = s.z * w;
+        c[i] = __builtin_fmaf(-s.y, a[i], b);
         if constexpr (JUMP) {
-            up[i] = w[i] < 0.f ? -1.f : 1.f;
-            const double e = (double)up[i] * (((double)s.x + s.y) - (double)b[i] / (((double)s.z + s.w) * w[i]));
+            up[i] = w < 0.f ? -1.f : 1.f;
+            const double e = (double)up[i] * (((double)s.x + s.y) - (double)b / (((double)s.z + s.w) * w));
             float f = (float)e;
             if ((double)f > e) f = nextafterf(f, -INFINITY);
-            edge[i] = w[i] == 0.f ? (b[i] > 0.f ? -INFINITY : INFINITY) : f;
+            edge[i] = w == 0.f ? (b > 0.f ? -INFINITY : INFINITY) : f;
         }
     }
     __device__ void load(const NormOp& p, int bi, int c0) {
 #pragma unroll
         for (int i = 0; i < V; ++i) set(p, c0 + i, i, p.stats[(int64_t)bi * p.G + (c0 + i) / p.cg]);
     }
-    __device__ float xh(float x, int i) const { return ((x - mh[i]) - ml[i]) * rh[i]; }
+    __device__ float z(float x, int i) const { return __builtin_fmaf(x - mh[i], a[i], c[i]); }
     __device__ bool above(float x, int i) const {
         if constexpr (JUMP) return up[i] * x > edge[i];
         else return false;
@@ -180,7 +182,7 @@ __global__ __launch_bounds__(256) void norm_sums_kernel(NormOp p) {
 // mean and rstd (two floats each) from the sums around the pivot
 __device__ __forceinline__ float4 stats_of(const NormOp& p, int len, double s, double t, float pivot) {
     const double cnt = (double)len * p.cg, off = cnt > 0 ? s / cnt : 0, var = cnt > 0 ? t / cnt - off * off : 0;
-    const double mean = (double)pivot + off, r = 1.0 / sqrt((var < 0 ? 0 : var) + (double)p.eps);
+    const double mean = cnt > 0 ? (double)pivot + off : 0, r = 1.0 / sqrt((var < 0 ? 0 : var) + (double)p.eps);
     float4 o;
     o.x = (float)mean; o.y = (float)(mean - (double)o.x);
     o.z = (float)r; o.w = (float)(r - (double)o.z);
@@ -234,15 +236,24 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormOp p) {
     rows_by<P, 4>(q, min(q.r1, len), [&](int r) { return *(const P*)(x + (int64_t)r * p.C); }, [&](int r, const P& v) {
         P o;
 #pragma unroll
-        for (int i = 0; i < V; ++i) o.v[i] = (T)act_of<ACT>(__builtin_fmaf(ch.xh((float)v.v[i], i), ch.w[i], ch.b[i]));
+        for (int i = 0; i < V; ++i) o.v[i] = (T)act_of<ACT>(ch.z((float)v.v[i], i));
         *(P*)(y + (int64_t)r * p.C) = o;
     });
     zero_rows<T, V>(p, q, len, y);
 }
 
-template <int V, int ACT> __device__ __forceinline__ float dz_of(const Chan<V, ACT>& ch, int i, float x, float dy, float& xh) {
-    xh = ch.xh(x, i);
-    return dy * slope_of<ACT>(__builtin_fmaf(xh, ch.w[i], ch.b[i]), ch.above(x, i));
+// The backward: sums of dz and dz (x - mh) per channel; a group's two means become dx = a dz - m.x - m.y (x - mh), where m.x = rstd mean(g) - m.y (mean - mh), m.y = rstd^2 mean(g xh)
+template <int V, int ACT> __device__ __forceinline__ float dz_of(const Chan<V, ACT>& ch, int i, float x, float dy) { return dy * slope_of<ACT>(ch.z(x, i), ch.above(x, i)); }
+template <int V, int ACT> __device__ __forceinline__ float dx_of(const Chan<V, ACT>& ch, int i, float x, float dy, float m1, float m2) {
+    return __builtin_fmaf(-(x - ch.mh[i]), m2, __builtin_fmaf(dz_of<V, ACT>(ch, i, x, dy), ch.a[i], -m1));
+}
+// sum dz (x - mh) -> sum dz xh
+__device__ __forceinline__ double2 of_xh(double2 v, const float4& s) { return double2{v.x, (v.y - s.y * v.x) * ((double)s.z + s.w)}; }
+// sums over the channels and tokens of a group of g and g xh -> m
+__device__ __forceinline__ float2 mom_of(double g, double gx, double cnt, const float4& s) {
+    if (!(cnt > 0)) return float2{0.f, 0.f};
+    const double r = (double)s.z + s.w, m2 = r * r * gx / cnt;
+    return float2{(float)(r * g / cnt - m2 * s.y), (float)m2};
 }
 
 // Bound by the vector instructions of gelu's slope in 16-bit types (eight elements per 16 bytes; sums of eight rows in 32 bits first did not make it faster)
@@ -262,10 +273,9 @@ __global__ __launch_bounds__(256, 4) void norm_grad_sums_kernel(NormOp p) {
         rows_by<Two<P>, V == 8 ? 2 : 4>(q, end, [&](int r) { return Two<P>{*(const P*)(x + (int64_t)r * p.C), *(const P*)(dy + (int64_t)r * p.C)}; }, [&](int, const Two<P>& v) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                float xh;
-                const double dz = dz_of<V, ACT>(ch, i, (float)v.x.v[i], (float)v.d.v[i], xh);
+                const double dz = dz_of<V, ACT>(ch, i, (float)v.x.v[i], (float)v.d.v[i]);
                 s[i] += dz;
-                t[i] += dz * xh;
+                t[i] += dz * ((float)v.x.v[i] - ch.mh[i]);
             }
         });
     }
@@ -276,17 +286,17 @@ __global__ __launch_bounds__(256, 4) void norm_grad_sums_kernel(NormOp p) {
 __global__ __launch_bounds__(256) void norm_grad_means_kernel(NormOp p) {
     __shared__ double2 sm[4];
     const int b = blockIdx.y, g = blockIdx.x, at = b * p.G + g, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const float4 st = p.stats[at];
     double m1 = 0, m2 = 0;
     for (int c = g * p.cg + wave; c < (g + 1) * p.cg; c += 4) {
         const double2* part = p.part + ((int64_t)b * p.C + c) * p.chunks;
         double s = 0, t = 0;
         for (int i = lane; i < p.chunks; i += 64) { s += part[i].x; t += part[i].y; }
-        s = wave_sum(s);
-        t = wave_sum(t);
-        if (lane == 0) p.chan[(int64_t)b * p.C + c] = double2{s, t};
+        const double2 v = of_xh(double2{wave_sum(s), wave_sum(t)}, st);
+        if (lane == 0) p.chan[(int64_t)b * p.C + c] = v;
         const double w = p.w ? p.w[c] : 1.0;
-        m1 += w * s;
-        m2 += w * t;
+        m1 += w * v.x;
+        m2 += w * v.y;
     }
     if (lane == 0) sm[wave] = double2{m1, m2};
     __syncthreads();
@@ -294,7 +304,7 @@ __global__ __launch_bounds__(256) void norm_grad_means_kernel(NormOp p) {
     const double cnt = (double)len_of(p, b) * p.cg;
     m1 = (sm[0].x + sm[1].x) + (sm[2].x + sm[3].x);
     m2 = (sm[0].y + sm[1].y) + (sm[2].y + sm[3].y);
-    p.mom[at] = float2{cnt > 0 ? (float)(m1 / cnt) : 0.f, cnt > 0 ? (float)(m2 / cnt) : 0.f};
+    p.mom[at] = mom_of(m1, m2, cnt, st);
 }
 
 // dw, db: sums over the batch, 16 channels x 16 parts of it per workgroup
@@ -331,9 +341,7 @@ __global__ __launch_bounds__(256, 4) void norm_grad_kernel(NormOp p) {
         P o;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            float xh;
-            const float dz = dz_of<V, ACT>(ch, i, (float)v.x.v[i], (float)v.d.v[i], xh);
-            o.v[i] = (T)((dz * ch.w[i] - m1[i] - xh * m2[i]) * ch.rh[i]);
+            o.v[i] = (T)dx_of<V, ACT>(ch, i, (float)v.x.v[i], (float)v.d.v[i], m1[i], m2[i]);
         }
         *(P*)(dx + (int64_t)r * p.C) = o;
     });
@@ -424,7 +432,7 @@ __global__ __launch_bounds__(HELD_THREADS) void norm_held_kernel(NormOp p) {
         if (r < len) {
             const P vk = unpack<T, V>(v[k]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) o.v[i] = (T)act_of<ACT>(__builtin_fmaf(ch.xh((float)vk.v[i], i), ch.w[i], ch.b[i]));
+            for (int i = 0; i < V; ++i) o.v[i] = (T)act_of<ACT>(ch.z((float)vk.v[i], i));
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i) o.v[i] = (T)0.f;
@@ -462,24 +470,25 @@ __global__ __launch_bounds__(HELD_THREADS) void norm_grad_held_kernel(NormOp p) 
             const P vk = unpack<T, V>(v[k]), dk = unpack<T, V>(d[k]);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                float xh;
-                const double dz = dz_of<V, ACT>(ch, i, (float)vk.v[i], (float)dk.v[i], xh);
+                const double dz = dz_of<V, ACT>(ch, i, (float)vk.v[i], (float)dk.v[i]);
                 s[i] += dz;
-                t[i] += dz * xh;
+                t[i] += dz * ((float)vk.v[i] - ch.mh[i]);
             }
         }
     reduce_rows<V>(sm, p.tc, s, t, chan);
     const int here = min(slab, p.C - c0), groups = here / p.cg;
-    if ((int)threadIdx.x < here && p.chan) p.chan[(int64_t)b * p.C + c0 + threadIdx.x] = chan[threadIdx.x];
+    const float4* stats = p.stats + (int64_t)b * p.G + c0 / p.cg;
+    if ((int)threadIdx.x < here && p.chan) p.chan[(int64_t)b * p.C + c0 + threadIdx.x] = of_xh(chan[threadIdx.x], stats[threadIdx.x / p.cg]);
     if ((int)threadIdx.x < groups) {
+        const float4 st = stats[threadIdx.x];
         double m1 = 0, m2 = 0;
         for (int i = 0; i < p.cg; ++i) {
             const double w = p.w ? p.w[c0 + threadIdx.x * p.cg + i] : 1.0;
-            m1 += w * chan[threadIdx.x * p.cg + i].x;
-            m2 += w * chan[threadIdx.x * p.cg + i].y;
+            const double2 v = of_xh(chan[threadIdx.x * p.cg + i], st);
+            m1 += w * v.x;
+            m2 += w * v.y;
         }
-        const double cnt = (double)len * p.cg;
-        mom[threadIdx.x] = float2{cnt > 0 ? (float)(m1 / cnt) : 0.f, cnt > 0 ? (float)(m2 / cnt) : 0.f};
+        mom[threadIdx.x] = mom_of(m1, m2, (double)len * p.cg, st);
     }
     __syncthreads();
     if (!on) return;
@@ -494,9 +503,7 @@ __global__ __launch_bounds__(HELD_THREADS) void norm_grad_held_kernel(NormOp p) 
             const P vk = unpack<T, V>(v[k]), dk = unpack<T, V>(d[k]);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                float xh;
-                const float dz = dz_of<V, ACT>(ch, i, (float)vk.v[i], (float)dk.v[i], xh);
-                o.v[i] = (T)((dz * ch.w[i] - m1[i] - xh * m2[i]) * ch.rh[i]);
+                o.v[i] = (T)dx_of<V, ACT>(ch, i, (float)vk.v[i], (float)dk.v[i], m1[i], m2[i]);
             }
         } else {
 #pragma unroll
