@@ -270,7 +270,7 @@ __global__ __launch_bounds__(256, 4) void norm_grad_sums_kernel(NormOp p) {
         Chan<V, ACT> ch;
         ch.load(p, q.b, q.c0);
         using P = Pack<T, V>;
-        rows_by<Two<P>, V == 8 ? 2 : 4>(q, end, [&](int r) { return Two<P>{*(const P*)(x + (int64_t)r * p.C), *(const P*)(dy + (int64_t)r * p.C)}; }, [&](int, const Two<P>& v) {
+        rows_by<Two<P>, 4>(q, end, [&](int r) { return Two<P>{*(const P*)(x + (int64_t)r * p.C), *(const P*)(dy + (int64_t)r * p.C)}; }, [&](int, const Two<P>& v) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const double dz = dz_of<V, ACT>(ch, i, (float)v.x.v[i], (float)v.d.v[i]);
