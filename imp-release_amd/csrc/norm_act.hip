@@ -11,8 +11,8 @@
 // Two ways, both bound by memory.  HELD: a workgroup takes whole groups of one batch element, 64 bytes of channels or more, and keeps all their tokens in registers (16 vectors of
 // 16 bytes per thread): one launch, x (and dy) read once.  Where the tokens do not fit: a launch that sums parts, a small one that joins them in a fixed order, and an
 // elementwise one - x is read twice, the second time from the 256-MB cache where it fits.  Measured (a large copy on this card: 5.0 TB/s, 8.0 from the cache):
-//   held, 8 x 2048 x 512 fp32, relu: forward 18 us (3.7 TB/s), backward 24 us (4.2); 16 x 4095 x 256 fp32 in 32 groups, ragged: 29 us
-//   4 x 307200 x 64 bf16 in 8 groups, gelu: sums 30 us (5.2 TB/s), elementwise 70 - 76 (4.3), gradient sums 94 - 106 (3.1: bound by gelu's slope), gradient 87 - 97 (5.1)
+//   held, 8 x 2048 x 512 fp32, relu: forward 17 us (4.0 TB/s), backward 23 us (4.4); 16 x 4095 x 256 fp32 in 32 groups, ragged: 30 us
+//   4 x 307200 x 64 bf16 in 8 groups, gelu: sums 30 us (5.2 TB/s), elementwise 63 - 67 (4.8), gradient sums 91 - 93 (3.4: bound by gelu's slope), gradient 87 - 89 (5.4)
 // The smallest cases are bound by the launch: 5 us.
 #include "../../include/imp_hip.h"
 #include "imp_kernels.h"
@@ -48,13 +48,13 @@ __device__ __forceinline__ int len_of(const NormOp& p, int b) { return p.lens ? 
 // the normal distribution function and (unscaled) density of z, by the rational approximation 7.1.26 of Abramowitz & Stegun's handbook (|error| of erf below 1.5e-7, what fp32
 // leaves of 1 + erf): one exponential serves both
 __device__ __forceinline__ float normal_cdf(float z, float& e) {
-    const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.f));
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.f));
     e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);               // exp(-z^2 / 2)
-    float q = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-    q = __builtin_fmaf(q, t, 1.421413741f);
-    q = __builtin_fmaf(q, t, -0.284496736f);
-    q = __builtin_fmaf(q, t, 0.254829592f);
-    q *= 0.5f * t * e;
+    float q = __builtin_fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+    q = __builtin_fmaf(q, t, 0.5f * 1.421413741f);
+    q = __builtin_fmaf(q, t, 0.5f * -0.284496736f);
+    q = __builtin_fmaf(q, t, 0.5f * 0.254829592f);
+    q *= t * e;
     return z > 0.f ? 1.f - q : q;
 }
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f)); }
